@@ -61,6 +61,12 @@ def _gpu(*tensors: Optional[torch.Tensor]) -> None:
             raise KernelError("kernel operands are on different devices")
 
 
+def on_current_device(device: torch.device, what: str) -> None:
+    """Kernels go to the current device's stream: operands on another one are refused."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: the operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 def _rows(t: torch.Tensor, what: str) -> None:
     if t.dim() != 2 or t.stride(1) != 1:
         raise KernelError(f"{what}: need a 2-d tensor with contiguous rows, got shape {tuple(t.shape)} "
@@ -2692,3 +2698,185 @@ def decay_scan(rows: torch.Tensor, offsets: Dict[str, int], state: torch.Tensor,
 def decay_state_floats(heads: int, key_dim: int, value_dim: int, gated: bool) -> int:
     """What a request's state takes in ``decay_scan``: the matrices, and with gates a normaliser and a maximum per head."""
     return heads * key_dim * value_dim + (heads * (key_dim + 1) if gated else 0)
+
+
+# ------------------------------------------------------------------ weights in 4 bits
+
+MX4_BLOCK = 32            # numbers along k that share a scale
+_MX4_PAIR = 256           # k that the products' order is filled up to
+
+
+@dataclass
+class Mx4:
+    """Rows of microscaled 4-bit numbers (the MXFP4 format): ``codes`` (uint8 ``[rows, 16 * blocks]``, two a byte, the first in the low half: a sign
+    and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6) times ``2 ** (scales - 127)`` (uint8 ``[rows, blocks]``, 255: not a number), 32 neighbours of the
+    ``k`` numbers of a row to a block; codes behind ``k`` are zero."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    k: int
+    _filled: bool = False         # both are the front of memory that goes on, with zeros, to a multiple of 256 k
+
+    @property
+    def shape(self):
+        return torch.Size((self.codes.shape[0], self.k))
+
+
+def _mx4_checked(q: Mx4, what: str) -> Tuple[int, int]:
+    """``(rows, blocks)`` of a well-formed Mx4."""
+    if not isinstance(q, Mx4):
+        raise KernelError(f"{what}: need an Mx4 (mx4_quantize), got {type(q).__name__}")
+    blocks = -(-int(q.k) // MX4_BLOCK)
+    if q.k < 0 or q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or q.codes.dim() != 2 or q.scales.dim() != 2 \
+            or q.codes.shape[1] != 16 * blocks or q.scales.shape != (q.codes.shape[0], blocks):
+        raise KernelError(f"{what}: codes {q.codes.dtype} {tuple(q.codes.shape)} and scales {q.scales.dtype} {tuple(q.scales.shape)} are not those of rows of {q.k} numbers")
+    for t, name in ((q.codes, "codes"), (q.scales, "scales")):
+        if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise KernelError(f"{what}: the {name}' rows must be contiguous and apart, got strides {t.stride()}")
+    return q.codes.shape[0], blocks
+
+
+def _mx4_here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    _gpu(*tensors)
+    on_current_device(next(t for t in tensors if t is not None).device, what)
+
+
+def _mx4_source(x: torch.Tensor, what: str) -> torch.Tensor:
+    """Rows that the conversion kernels read: contiguous ones, any distance apart."""
+    _type(x, what)
+    if x.dim() != 2:
+        raise KernelError(f"{what}: need rows [m, k], got shape {tuple(x.shape)}")
+    _mx4_here(what, x)
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x
+
+
+def mx4_quantize(x: torch.Tensor) -> Mx4:
+    """Rows ``[m, k]`` (bfloat16 or float32) as microscaled 4-bit numbers: a block's scale is ``2 ** (floor(log2(max |x|)) - 2)``, at least ``2 ** -127``; a
+    number goes to the nearest code, ties to the even one, and beyond 6 scales to 6.  A block that holds an infinity or a NaN becomes NaN."""
+    x = _mx4_source(x, "mx4_quantize")
+    m, k = x.shape
+    filled, blocks = -(-k // _MX4_PAIR) * _MX4_PAIR, -(-k // MX4_BLOCK)
+    codes = torch.empty((m, filled // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((m, filled // MX4_BLOCK), dtype=torch.uint8, device=x.device)
+    if m and k:
+        _check(build.load("mx4").lcu_mx4_quantize(_ptr(x), ctypes.c_longlong(x.stride(0)), _type(x, "mx4_quantize"), ctypes.c_longlong(m), k, _ptr(codes), _ptr(scales), _stream()),
+               "mx4_quantize")
+    return Mx4(codes[:, :16 * blocks], scales[:, :blocks], k, True)
+
+
+def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """What the codes stand for, ``[rows, k]`` in bfloat16 or float32: exact, but for what lies beyond the type's range."""
+    m, _ = _mx4_checked(q, "mx4_values")
+    if out_dtype not in _TYPE:
+        raise KernelError(f"mx4_values: type {out_dtype} is not supported (float32 or bfloat16)")
+    _mx4_here("mx4_values", q.codes, q.scales)
+    out = torch.empty((m, q.k), dtype=out_dtype, device=q.codes.device)
+    if m and q.k:
+        _check(build.load("mx4").lcu_mx4_values(_ptr(q.codes), ctypes.c_longlong(q.codes.stride(0)), _ptr(q.scales), ctypes.c_longlong(q.scales.stride(0)), ctypes.c_longlong(m),
+                                                q.k, _ptr(out), ctypes.c_longlong(q.k), _type(out, "mx4_values"), _stream()), "mx4_values")
+    return out
+
+
+class PackedMx4:
+    """A 4-bit weight ``[n, k]`` in the order in which the products read it (``pack_mx4``)."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int):
+        self.codes, self.scales, self.n, self.k = codes, scales, n, k
+        self.pairs = -(-k // _MX4_PAIR)
+
+    @property
+    def shape(self):
+        return torch.Size((self.n, self.k))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def pack_mx4(q: Mx4) -> PackedMx4:
+    """A quantised weight ``[n, k]`` laid out for ``gemm_mx4``, once: features filled up to tiles of 16 and ``k`` to pairs of 128; a tile's codes of a pair in
+    ``[macro-step][block][feature][16 bytes]``, its scales in ``[feature][macro-step][block]``."""
+    n, blocks = _mx4_checked(q, "pack_mx4")
+    if n < 1 or q.k < 1:
+        raise KernelError(f"pack_mx4: a weight of {n} x {q.k} has nothing to multiply")
+    _mx4_here("pack_mx4", q.codes, q.scales)
+    tiles, pairs = -(-n // 16), -(-q.k // _MX4_PAIR)
+    codes = torch.zeros((tiles * 16, pairs * 128), dtype=torch.uint8, device=q.codes.device)
+    codes[:n, :16 * blocks] = q.codes
+    scales = torch.full((tiles * 16, pairs * 8), 127, dtype=torch.uint8, device=q.codes.device)
+    scales[:n, :blocks] = q.scales
+    codes = codes.view(tiles, 16, pairs, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous().view(-1)
+    scales = scales.view(tiles, 16, pairs, 8).permute(0, 2, 1, 3).contiguous().view(-1)
+    return PackedMx4(codes, scales, n, int(q.k))
+
+
+def _mx4_rows(x: torch.Tensor, k: int) -> Tuple[torch.Tensor, int]:
+    """Rows as the 4-bit products read them, and how (``x_kind`` in mx4_stream.hip): bfloat16 rows of whole macro-steps as they are, others filled up, float32
+    ones as three planes of bfloat16."""
+    if x.dtype == torch.bfloat16 and k % 128 == 0 and x.stride(1) == 1 and x.data_ptr() % 16 == 0 \
+            and (x.shape[0] == 1 or (x.stride(0) % 8 == 0 and k <= x.stride(0) < 1 << 24)):
+        return x, 1
+    x = _mx4_source(x, "gemm_mx4")
+    planes = 3 if x.dtype == torch.float32 else 1
+    out = torch.empty((x.shape[0], planes * (-(-k // _MX4_PAIR) * _MX4_PAIR)), dtype=torch.bfloat16, device=x.device)
+    _check(build.load("mx4").lcu_mx4_rows(_ptr(x), ctypes.c_longlong(x.stride(0)), _type(x, "gemm_mx4"), ctypes.c_longlong(x.shape[0]), k, _ptr(out), _stream()), "gemm_mx4 rows")
+    return out, planes
+
+
+def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
+    """Rows in 4 bits as the products read them: whole macro-steps of 128, rows on 16 bytes, scales on 4."""
+    fits = (q._filled or blocks % 4 == 0) and q.codes.data_ptr() % 16 == 0 and q.scales.data_ptr() % 4 == 0 \
+        and (q.codes.shape[0] == 1 or (q.codes.stride(0) % 16 == 0 and q.codes.stride(0) < 1 << 24 and q.scales.stride(0) % 4 == 0))
+    if fits:
+        return q
+    whole = -(-blocks // 8) * 8
+    codes = torch.zeros((q.codes.shape[0], 16 * whole), dtype=torch.uint8, device=q.codes.device)
+    scales = torch.zeros((q.codes.shape[0], whole), dtype=torch.uint8, device=q.codes.device)
+    codes[:, :16 * blocks] = q.codes
+    scales[:, :blocks] = q.scales
+    return Mx4(codes[:, :16 * blocks], scales[:, :blocks], q.k, True)
+
+
+def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, swiglu: bool = False) -> torch.Tensor:
+    """``x @ w.T`` with a weight in 4 bits and 32-bit sums, any number of rows.  ``x``: rows ``[m, k]`` in bfloat16 (multiplied as they are, the weight's
+    numbers are bfloat16 numbers) or float32 (in full: three products of eight bits of the mantissa each), or an Mx4 (4 bits times 4 bits).  ``out [m, n]``
+    bfloat16 or float32 (default: the rows' type, bfloat16 for an Mx4).  ``swiglu``: ``w`` holds ``n / 2`` gate rows, then the up rows, and
+    the result is ``silu(gate) * up``, ``[m, n / 2]``."""
+    if not isinstance(w, PackedMx4):
+        raise KernelError(f"gemm_mx4: the weight must be a PackedMx4 (pack_mx4), got {type(w).__name__}")
+    four = isinstance(x, Mx4)
+    if four:
+        m, blocks = _mx4_checked(x, "gemm_mx4 x")
+        k, device = x.k, x.codes.device
+    else:
+        _type(x, "gemm_mx4 x")
+        if x.dim() != 2:
+            raise KernelError(f"gemm_mx4: need rows [m, k], got shape {tuple(x.shape)}")
+        (m, k), device = x.shape, x.device
+    if k != w.k:
+        raise KernelError(f"gemm_mx4: rows of {k} numbers with a weight of {w.k}")
+    if swiglu and w.n % 2:
+        raise KernelError(f"gemm_mx4: {w.n} features are not as many gate as up rows")
+    cols = w.n // 2 if swiglu else w.n
+    dtype = out.dtype if out is not None else out_dtype or (torch.bfloat16 if four else x.dtype)
+    if dtype not in _TYPE or (out is not None and out_dtype not in (None, dtype)):
+        raise KernelError(f"gemm_mx4 out: type {dtype} is not supported (float32 or bfloat16, that of out)")
+    _mx4_here("gemm_mx4", x.codes if four else x, x.scales if four else None, w.codes, out)
+    if out is None:
+        out = torch.empty((m, cols), dtype=dtype, device=device)
+    elif out.shape != (m, cols) or (cols > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < cols):
+        raise KernelError(f"gemm_mx4 out: need {(m, cols)} with contiguous rows apart, got {tuple(out.shape)} with strides {out.stride()}")
+    if m == 0:
+        return out
+    if four:
+        q = _mx4_whole(x, blocks)
+        rows, kind, ld, scales, lds = q.codes, 4, q.codes.stride(0), q.scales, q.scales.stride(0)
+    else:
+        rows, kind = _mx4_rows(x, k)
+        ld, scales, lds = rows.stride(0), None, 0
+    if m == 1:                             # (the one row's stride says nothing)
+        ld, lds = (128 * w.pairs, 8 * w.pairs) if four else (rows.shape[1], 0)
+    _check(build.load("mx4_stream").lcu_mx4_stream(_ptr(rows), ctypes.c_longlong(ld), kind, _ptr(scales), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), w.pairs, _ptr(out),
+                                                   ctypes.c_longlong(out.stride(0) if m > 1 else cols), m, w.n, k, (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0), _stream()), "gemm_mx4")
+    return out
