@@ -1,0 +1,182 @@
+// Verification of drafted tokens: which of a request's drafts stand, and the token after them.
+//
+// Request b has the rows starts[b] .. starts[b + 1] - 1 of the target's probabilities p, one more than it has drafts.  Draft i, drawn from q_i (or
+// certain, where no q is given), stands if u_i q_i(d_i) < p_i(d_i), that is with the probability min(1, p / q); the first that does not ends the
+// run of a drafts that do.  The token after them is drawn from max(p_a - q_a, 0) where a draft was refused (from p_a where that leaves nothing)
+// and from p_a where all stand: the first v whose sum C(v) of what precedes it, itself included, is more than u C(V).  Tokens come out distributed as
+// the target's are.  Probabilities that are no finite positive numbers count as zero.
+//
+// Only the row at which the run ends is read (two, with the draft's): first its parts' sums, a workgroup each, in 64 bits and a fixed order; then a
+// workgroup a request finds the part, and reads that again to find the token.  Bound by memory: 4 or 8 bytes a token of the vocabulary.
+#include "common.h"
+
+constexpr int VF_THREADS = 512, VF_MAX_PARTS = 64, VF_MAX_DRAFTS = 1024;
+
+__device__ __forceinline__ float vf_clean(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
+
+// What has become of a request's drafts.
+struct VfRun {
+    int row, draft, count, taken;     // its first row and draft, how many drafts, how many stand
+    bool bad;                         // starts that make no sense
+};
+
+// Every thread of the workgroup calls it and gets the answer.
+__device__ VfRun vf_run(const float *__restrict__ p, size_t ldp, int rows, const int *__restrict__ starts, const int *__restrict__ drafts, int n_drafts,
+                        const float *__restrict__ q, size_t ldq, const float *__restrict__ accept, int vocab, int most) {
+    __shared__ int first;
+    VfRun v;
+    const int b = blockIdx.x;
+    const long long row = starts[b], count = (long long)starts[b + 1] - row - 1;
+    v.row = (int)row;
+    v.count = (int)count;
+    v.draft = (int)(row - b);
+    v.taken = 0;
+    v.bad = row < 0 || count < 0 || count > most || row + count >= rows || row - b < 0 || row - b + count > n_drafts;
+    if (v.bad) return v;
+    if (threadIdx.x == 0) first = v.count;
+    __syncthreads();
+    for (int i = threadIdx.x; i < v.count; i += VF_THREADS) {
+        const int d = drafts[v.draft + i];
+        bool stands = false;
+        if (d >= 0 && d < vocab) {
+            const float pd = vf_clean(p[(size_t)(v.row + i) * ldp + d]), qd = q ? vf_clean(q[(size_t)(v.draft + i) * ldq + d]) : 1.f;
+            stands = (double)accept[v.draft + i] * (double)qd < (double)pd;
+        }
+        if (!stands) atomicMin(&first, i);
+    }
+    __syncthreads();
+    v.taken = first;
+    return v;
+}
+
+// What is left of the target's probability of token i for the token after the run.
+struct VfLeft {
+    const float *p, *q;
+    int without;                      // the certain draft that was refused, or -1
+    __device__ __forceinline__ double operator()(int i) const {
+        const double v = vf_clean(p[i]);
+        if (i == without) return 0.0;
+        if (!q) return v;
+        const double left = v - (double)vf_clean(q[i]);
+        return left > 0.0 ? left : 0.0;
+    }
+};
+__device__ __forceinline__ VfLeft vf_left(const VfRun &v, const float *p, size_t ldp, const int *drafts, const float *q, size_t ldq) {
+    const bool refused = v.taken < v.count;
+    return {p + (size_t)(v.row + v.taken) * ldp, refused && q ? q + (size_t)(v.draft + v.taken) * ldq : nullptr, refused && !q ? drafts[v.draft + v.taken] : -1};
+}
+
+__device__ __forceinline__ double vf_wave_sum(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, WAVE);
+    return v;
+}
+
+// sums: [requests][parts][2], of what is left and of the target's own.
+__global__ void __launch_bounds__(VF_THREADS)
+vf_sum_kernel(const float *__restrict__ p, size_t ldp, int rows, const int *__restrict__ starts, const int *__restrict__ drafts, int n_drafts, const float *__restrict__ q,
+              size_t ldq, const float *__restrict__ accept, int vocab, int most, double *__restrict__ sums) {
+    __shared__ double all[VF_THREADS / WAVE][2];
+    const VfRun run = vf_run(p, ldp, rows, starts, drafts, n_drafts, q, ldq, accept, vocab, most);
+    if (run.bad) return;
+    const VfLeft left = vf_left(run, p, ldp, drafts, q, ldq);
+    const int parts = gridDim.y, each = (vocab + parts - 1) / parts, lo = min(vocab, (int)blockIdx.y * each), hi = min(vocab, lo + each);
+    double mine = 0.0, own = 0.0;
+    for (int i = lo + threadIdx.x; i < hi; i += VF_THREADS) { mine += left(i); own += vf_clean(left.p[i]); }
+    mine = vf_wave_sum(mine);
+    own = vf_wave_sum(own);
+    if ((threadIdx.x & 63) == 0) { all[threadIdx.x >> 6][0] = mine; all[threadIdx.x >> 6][1] = own; }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        double t = 0.0;
+        for (int w = 0; w < VF_THREADS / WAVE; ++w) t += all[w][threadIdx.x];
+        sums[((size_t)blockIdx.x * parts + blockIdx.y) * 2 + threadIdx.x] = t;
+    }
+}
+
+__global__ void __launch_bounds__(VF_THREADS)
+vf_token_kernel(const float *__restrict__ p, size_t ldp, int rows, const int *__restrict__ starts, const int *__restrict__ drafts, int n_drafts, const float *__restrict__ q,
+                size_t ldq, const float *__restrict__ accept, const float *__restrict__ final_u, int vocab, int most, const double *__restrict__ sums, int parts,
+                int *__restrict__ accepted, int *__restrict__ tokens) {
+    __shared__ double wave_sums[VF_THREADS / WAVE];
+    __shared__ int found, last;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const VfRun run = vf_run(p, ldp, rows, starts, drafts, n_drafts, q, ldq, accept, vocab, most);
+    int *out = tokens + (size_t)b * (most + 1);
+    for (int i = threadIdx.x; i <= most; i += VF_THREADS)
+        if (run.bad || i != run.taken) out[i] = !run.bad && i < run.taken ? drafts[run.draft + i] : -1;
+    if (threadIdx.x == 0) { accepted[b] = run.bad ? 0 : run.taken; found = 0x7fffffff; last = -1; }
+    if (run.bad) return;
+    VfLeft left = vf_left(run, p, ldp, drafts, q, ldq);
+    const double *s = sums + (size_t)b * parts * 2;
+    double total = 0.0;
+    for (int i = 0; i < parts; ++i) total += s[2 * i];
+    int which = 0;
+    if (!(total > 0.0)) {                              // nothing is left: the target's own
+        left.q = nullptr;
+        left.without = -1;
+        which = 1;
+        for (int i = 0; i < parts; ++i) total += s[2 * i + 1];
+    }
+    const double goal = (double)final_u[b] * total;
+    // the part in which the sum passes the goal, else the last that holds anything
+    int part = -1;
+    double before = 0.0, sum = 0.0;
+    for (int i = 0; i < parts; ++i) {
+        const double v = s[2 * i + which];
+        if (v > 0.0) { part = i; before = sum; }
+        sum += v;
+        if (sum > goal) break;
+    }
+    if (part < 0) {
+        if (threadIdx.x == 0) out[run.taken] = -1;
+        return;
+    }
+    const int each = (vocab + parts - 1) / parts, lo = min(vocab, part * each), hi = min(vocab, lo + each);
+    const int piece = (hi - lo + VF_THREADS - 1) / VF_THREADS, from = min(hi, lo + (int)threadIdx.x * piece), to = min(hi, from + piece);
+    double mine = 0.0;
+    for (int i = from; i < to; ++i) mine += left(i);
+    double scan = mine;
+#pragma unroll
+    for (int off = 1; off < WAVE; off <<= 1) {
+        const double up = __shfl_up(scan, off, WAVE);
+        if (lane >= off) scan += up;
+    }
+    if (lane == WAVE - 1) wave_sums[wave] = scan;
+    __syncthreads();
+    double at = before;
+    for (int w = 0; w < wave; ++w) at += wave_sums[w];
+    at += scan - mine;
+    if (mine > 0.0) {
+        int mine_last = -1;
+        bool got = false;
+        for (int i = from; i < to; ++i) {
+            const double v = left(i);
+            at += v;
+            if (v > 0.0) {
+                mine_last = i;
+                if (!got && at > goal) { atomicMin(&found, i); got = true; }
+            }
+        }
+        atomicMax(&last, mine_last);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) out[run.taken] = found < vocab ? found : last;      // (the goal lies a rounding beyond the part: its last)
+}
+
+// probs: [rows, ldp] float32, drafts, accept: [n_drafts], draft_probs: null or [n_drafts, ldq], starts: [requests + 1], final_u: [requests]; accepted: [requests],
+// tokens: [requests, most + 1]; parts: workgroups a request, 1 to 64; sums: [requests][parts][2] doubles.
+LCU_API int lcu_verify_drafts(const float *probs, long long ldp, int rows, const int *starts, int requests, const int *drafts, int n_drafts, const float *draft_probs,
+                              long long ldq, const float *accept, const float *final_u, int vocab, int most, int parts, double *sums, int *accepted, int *tokens,
+                              hipStream_t stream) {
+    if (requests <= 0) return LCU_OK;
+    if (rows < 0 || vocab <= 0 || most < 0 || most > VF_MAX_DRAFTS || n_drafts < 0 || parts < 1 || parts > VF_MAX_PARTS || !probs || !starts || !final_u || !sums || !accepted ||
+        !tokens || (n_drafts && (!drafts || !accept)) || (rows > 1 && ldp < vocab) || (draft_probs && n_drafts > 1 && ldq < vocab))
+        return LCU_BAD_ARGUMENT;
+    vf_sum_kernel<<<dim3(requests, parts), dim3(VF_THREADS), 0, stream>>>(probs, (size_t)ldp, rows, starts, drafts, n_drafts, draft_probs, (size_t)ldq, accept, vocab, most, sums);
+    LCU_LAUNCH_CHECK();
+    vf_token_kernel<<<dim3(requests), dim3(VF_THREADS), 0, stream>>>(probs, (size_t)ldp, rows, starts, drafts, n_drafts, draft_probs, (size_t)ldq, accept, final_u, vocab, most,
+                                                                    sums, parts, accepted, tokens);
+    LCU_LAUNCH_CHECK();
+    return LCU_OK;
+}

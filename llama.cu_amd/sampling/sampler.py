@@ -7,7 +7,7 @@ depend on what else is in the batch or on how its prompt was cut.
 from __future__ import annotations
 
 import ctypes
-from typing import List, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -16,6 +16,8 @@ from ..kernels.ops import KernelError, _check, _gpu, _ptr, _stream, to_device as
 from .params import SamplingParams
 
 _MASK = (1 << 64) - 1
+MAX_VOCAB = 1 << 19          # what the kernels' 64-bit sums of weights allow
+MAX_DRAFTS = 1024            # drafts a request in one verification
 
 
 def _splitmix64(x: int) -> int:
@@ -91,6 +93,117 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     lib = build.load("sampling")
     _check(lib.lcu_token_logprob(_ptr(logits), logits.stride(0), rows, vocab, _ptr(tokens), _ptr(out), _stream()), "token_logprobs")
     return out
+
+
+def _options(values, dtype: torch.dtype, rows: int, device, what: str, fine, why: str) -> torch.Tensor:
+    """A number a row, on the device: a sequence, which is looked at here, or a tensor that is there already, which is not."""
+    if isinstance(values, torch.Tensor) and values.is_cuda:
+        if values.device != device or values.dtype != dtype or values.shape != (rows,) or not values.is_contiguous():
+            raise KernelError(f"token_probs: {what} on the device must be contiguous {dtype} [{rows}], got {values.dtype} {tuple(values.shape)}")
+        return values
+    values = values.tolist() if isinstance(values, torch.Tensor) else list(values)
+    if len(values) != rows or not all(fine(v) for v in values):
+        raise KernelError(f"token_probs: {what} must be {rows} numbers {why}")
+    return values
+
+
+def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The distribution that ``sample_rows`` draws each row's token from, float32 ``[rows, vocab]``: with the logits in descending order
+    (equal ones by index), weights ``w_i = exp((l_i - l_0) / T)`` and sums ``c`` of them, entry ``i`` has the share
+    ``(min(c_i, L) - min(c_{i-1}, L)) / L``, ``L = min(top_p * c_n, c_{top_k})``.  A temperature of 0, or ``top_k`` 1, leaves the first
+    of the largest logits.  A NaN counts as -inf, which has no share; a row of nothing else is all zeros.
+
+    ``temperature``, ``top_p``, ``top_k``: a sequence of one number a row, or (float32, float32, int32) tensors on the logits' device,
+    whose numbers are not looked at: a temperature or top_p that is not positive, or a top_k below 1, then acts as a temperature of 0."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KernelError("token_probs: logits must be float32 [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    if not 0 < vocab <= MAX_VOCAB:
+        raise KernelError(f"token_probs: a vocabulary of {vocab} is not supported (1 to {MAX_VOCAB})")
+    dev = logits.device
+    temperature = _options(temperature, torch.float32, rows, dev, "temperature", lambda t: 0 <= t < float("inf"), ">= 0")
+    top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda p: p > 0, "> 0")
+    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda k: k >= 1, ">= 1")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
+    elif out.shape != (rows, vocab) or out.dtype != torch.float32 or not out.is_contiguous():
+        raise KernelError(f"token_probs out: must be contiguous float32 {(rows, vocab)}, got {out.dtype} {tuple(out.shape)}")
+    _gpu(logits, out)
+    ops.on_current_device(dev, "token_probs")
+    if rows == 0:
+        return out
+    # whether some row is cut: known of sequences, taken as given of tensors
+    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or any(p < 1 for p in top_p) or any(k < vocab for k in top_k)
+    floats = [v for v in (temperature, top_p) if not isinstance(v, torch.Tensor)]
+    there = iter(_to_device(floats, torch.float32, dev)) if floats else None
+    temperature, top_p = (v if isinstance(v, torch.Tensor) else next(there) for v in (temperature, top_p))
+    if not isinstance(top_k, torch.Tensor):
+        top_k = _to_device([min(int(k), vocab) for k in top_k], torch.int32, dev)
+    lib = build.load("token_probs")
+    # a long row is cut into parts of 4,096 logits at least, one workgroup each, up to about four workgroups a compute unit in all
+    parts = max(1, min(32, 4 * ops.TUNING.compute_units // rows, vocab // 4096))
+    lib.lcu_token_probs_scratch_bytes.restype = ctypes.c_size_t
+    scratch = torch.empty(int(lib.lcu_token_probs_scratch_bytes(rows, parts, int(cuts))), dtype=torch.uint8, device=dev)
+    _check(lib.lcu_token_probs(_ptr(logits), ctypes.c_longlong(logits.stride(0)), rows, vocab, _ptr(temperature), _ptr(top_p), _ptr(top_k), _ptr(out), parts,
+                               int(cuts), _ptr(scratch), _stream()), "token_probs")
+    return out
+
+
+def _rows_of(t: torch.Tensor, what: str, vocab: Optional[int] = None, rows: Optional[int] = None) -> None:
+    if t.dim() != 2 or t.dtype != torch.float32 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) \
+            or vocab not in (None, t.shape[1]) or rows not in (None, t.shape[0]):
+        raise KernelError(f"verify_drafts: {what} must be float32 [{'rows' if rows is None else rows}, {'vocab' if vocab is None else vocab}] with contiguous rows, "
+                          f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+
+
+def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tensor, accept: torch.Tensor, final: torch.Tensor, max_drafts: int,
+                  draft_probs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which of the requests' drafted tokens stand, and the token after them, so that what comes out is distributed as the target's tokens are.
+
+    ``probs`` (float32 ``[rows, vocab]``): the target's probabilities (``token_probs``), for every request one row more than it has drafts, the
+    requests one after the other; request ``b`` has the rows ``starts[b]`` to ``starts[b + 1]`` (int32, one entry more than requests, the first 0).
+    ``drafts`` (int32), ``accept`` (float32 in [0, 1)) and ``draft_probs`` (float32 ``[drafts, vocab]``, what the drafts were drawn from; without it
+    they were certain) hold all requests' drafts one after the other; ``final`` (float32 in [0, 1)) one number a request.
+
+    Draft ``i`` stands if ``accept * q_i(d_i) < p_i(d_i)``, and the first that does not is the last looked at.  The token after those that stand is the
+    first ``v`` whose sum of ``max(p - q, 0)`` up to ``v`` is more than ``final`` times the whole (of ``p`` itself where all stand, and where ``max(p - q,
+    0)`` leaves nothing).  Probabilities that are no finite positive numbers count as zero, a draft outside the vocabulary never stands.
+
+    Returns ``(accepted [requests], tokens [requests, max_drafts + 1])``, int32 on the device: a request's drafts that stand, the token after them (-1 if
+    its row holds no probability at all), and -1 behind.  A request whose ``starts`` make no sense, or that has more than ``max_drafts`` drafts, gets 0
+    and -1 only."""
+    _rows_of(probs, "probs")
+    rows, vocab = probs.shape
+    if starts.dtype != torch.int32 or starts.dim() != 1 or starts.numel() < 1 or not starts.is_contiguous():
+        raise KernelError("verify_drafts: starts must be a contiguous int32 [requests + 1]")
+    requests = starts.numel() - 1
+    n = rows - requests
+    if drafts.dtype != torch.int32 or drafts.shape != (n,) or not drafts.is_contiguous():
+        raise KernelError(f"verify_drafts: {rows} rows of {requests} requests judge {n} drafts: drafts must be contiguous int32 [{n}], got {drafts.dtype} {tuple(drafts.shape)}")
+    for t, what, size in ((accept, "accept", n), (final, "final", requests)):
+        if t.dtype != torch.float32 or t.shape != (size,) or not t.is_contiguous():
+            raise KernelError(f"verify_drafts: {what} must be contiguous float32 [{size}], got {t.dtype} {tuple(t.shape)}")
+    if draft_probs is not None:
+        _rows_of(draft_probs, "draft_probs", vocab, n)
+    if not 0 <= int(max_drafts) <= MAX_DRAFTS:
+        raise KernelError(f"verify_drafts: max_drafts {max_drafts} is not supported (0 to {MAX_DRAFTS})")
+    if not 0 < vocab <= MAX_VOCAB:
+        raise KernelError(f"verify_drafts: a vocabulary of {vocab} is not supported (1 to {MAX_VOCAB})")
+    _gpu(probs, starts, drafts, accept, final, draft_probs)
+    dev = probs.device
+    ops.on_current_device(dev, "verify_drafts")
+    accepted = torch.empty(requests, dtype=torch.int32, device=dev)
+    tokens = torch.empty((requests, int(max_drafts) + 1), dtype=torch.int32, device=dev)
+    if requests == 0:
+        return accepted, tokens
+    # the row at which a run ends is cut into parts of 2,048 tokens at least, up to about four workgroups a compute unit in all
+    parts = max(1, min(64, 4 * ops.TUNING.compute_units // requests, vocab // 2048))
+    sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev)
+    lib = build.load("verify")
+    _check(lib.lcu_verify_drafts(_ptr(probs), ctypes.c_longlong(probs.stride(0)), rows, _ptr(starts), requests, _ptr(drafts), n, _ptr(draft_probs),
+                                 ctypes.c_longlong(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(accept), _ptr(final), vocab, int(max_drafts), parts,
+                                 _ptr(sums), _ptr(accepted), _ptr(tokens), _stream()), "verify_drafts")
+    return accepted, tokens
 
 
 class Sampler:
