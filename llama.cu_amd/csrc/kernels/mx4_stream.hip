@@ -2,10 +2,11 @@
 //
 // A workgroup takes NT tiles of 16 features (for SwiGLU the gate rows of a tile and the up rows that meet them) and 16 MT rows; its eight waves share
 // out K in pairs of macro-steps (256 k) and add their partial sums through LDS in a fixed order.  Rows of bfloat16: the codes become bfloat16
-// in registers, exactly and with their scale, two a conversion, in the order in which v_mfma_f32_16x16x32_bf16 wants its operand.  Rows of
-// float32 come as three planes of bfloat16 whose sum they are, each multiplied with the same codes.  Rows in 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4
+// in registers, exactly and with their scale, two a conversion, in the order in which the matrix instruction of 16 x 16 x 32 wants its operand.  Rows of
+// float32 come as three planes of bfloat16 whose sum they are, each multiplied with the same codes.  Rows in 4 bits: the scaled instruction of 16 x 16 x 128
 // takes both sides' codes and scales as they are.
 #include "mx4.h"
+#include "mx4/matrix.h"
 #include "gate_act.h"
 #include "quad_rows.h"
 
@@ -140,7 +141,7 @@ mx4_stream_kernel(const bf16_t *__restrict__ X, int ldx, int plane, Mx4Args a) {
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
-                        acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx4_bf16x8, w[n][j]), __builtin_bit_cast(mx4_bf16x8, x[j]), acc[n][m], 0, 0, 0);
+                        acc[n][m] = mx4_multiply_16(w[n][j], x[j], acc[n][m]);
                 if (next < a.macros) fetch_x(m, q, next);
             }
         wait_for_sums();
@@ -190,24 +191,23 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[n][m] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; ++s) {
-        mx4_i32x8 w[NT], x[MT];
+        mx4_u32x4 w[NT], x[MT];
         uint32_t wscale[NT], xscale[MT];
-        auto operand = [](const mx4_u32x4 &v) { return mx4_i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            w[n] = operand(__builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)s * 1024)));
+            w[n] = __builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)s * 1024));
             wscale[n] = *(const uint32_t *)(ws[n] + (size_t)(s >> 1) * MX4_PAIR_SCALES + 4 * (s & 1)) >> 8 * g;
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            x[m] = operand(*(const mx4_u32x4 *)(xc[m] + (size_t)s * 64));
+            x[m] = *(const mx4_u32x4 *)(xc[m] + (size_t)s * 64);
             xscale[m] = *(const uint32_t *)(xs[m] + (size_t)s * 4) >> 8 * g;
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                acc[n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[n], x[m], acc[n][m], 4, 4, 0, (int)wscale[n], 0, (int)xscale[m]);
+                acc[n][m] = mx4_multiply_codes_16<0>(w[n], x[m], acc[n][m], wscale[n], xscale[m]);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)

@@ -1,0 +1,373 @@
+// Y[M, N] = X[M, K] * W[N, K]^T with W in microscaled 4-bit numbers (mx4.h), 32-bit sums: many rows, in tiles.
+//
+// A workgroup has a tile of F features and T tokens.  Both operands come by loads that write into LDS themselves, in rings of their own of SF and ST
+// steps; a wave multiplies 32 FT features and 32 TT tokens.  One barrier a step, in the middle of it: the products of a step's last slice, and then of
+// each slice, run while the next slice is read, so the matrix cores have work on both sides of the barrier.
+//
+//   rows in bfloat16   a step is 64 k.  A lane reads a block of 32 codes of a feature at once, a step's worth, and makes the operands of the four
+//                      slices (32 x 32 x 16) out of it as they are needed; W takes a quarter of the LDS and of its bandwidth that bfloat16 would.
+//                      The waves stand four by features and two by tokens, since every wave converts its own features' codes.
+//   rows in float32    are bfloat16 rows of three times the k (planes one behind the other), with W gone through three times.
+//   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, eight bytes a row and step, come into registers.
+#include <type_traits>
+#include "mx4.h"
+#include "mx4/matrix.h"
+#include "gate_act.h"
+
+enum { MT_EPI_BF16 = 0, MT_EPI_F32 = 1, MT_EPI_SWIGLU = 2, MT_EPI_SWIGLU_F32 = 3 };
+
+template <int LEFT>
+__device__ __forceinline__ void mt_wait_loads() {
+    static_assert(LEFT >= 0 && LEFT < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// FOUR: rows in 4 bits.  SF, ST: steps of features and of tokens that the rings hold.
+template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_> struct MtShape {
+    static constexpr bool FOUR = FOUR_;
+    static constexpr int FT = FT_, TT = TT_, WF = WF_, WT = WT_, SF = SF_, ST = ST_, SLICES = 4;
+    static constexpr int WAVES = WF * WT, THREADS = WAVES * WAVE, F = 32 * FT * WF, T = 32 * TT * WT;
+    static constexpr int FP = FOUR ? 8 : 2, TP = 8;                    // pieces (16 bytes) of a row a stage
+    static constexpr int STEP_CODES = FOUR ? 2048 : 512;               // bytes of a tile of 16 features a step
+    static constexpr int LF = F * FP / WAVE / WAVES, LT = T * TP / WAVE / WAVES;       // loads of a wave a stage
+    static constexpr int LS = FOUR ? FT + TT : FT;                     // and of scales, into registers
+    static constexpr int LDS = SF * F * FP + ST * T * TP;              // pieces
+    static constexpr int LEFT = (SF > ST ? LF : 0) + (ST - 2) * (LF + LT + LS);        // loads that may be on their way when a step begins
+    static_assert(FT % 2 == 0 && F * FP % (WAVE * WAVES) == 0 && T * TP % (WAVE * WAVES) == 0 && SF >= ST && ST >= 2 && LDS * 16 <= 160 * 1024, "whole loads, and room for the stages");
+};
+
+template <class S> struct MtFrags { mx4_u32x4 f[S::FT], t[S::TT]; };
+
+// The scales of a step: FOUR: a row's eight bytes, moved so that the lane's own are bytes 0 and 2 of each half; else the lane's one byte of each tile.
+template <class S> struct MtScales { uint32_t f[S::FT][S::FOUR ? 2 : 1], t[S::FOUR ? S::TT : 1][2]; };
+
+__device__ __forceinline__ void mt_read(mx4_u32x4 &to, const mx4_u32x4 *from) {
+    to = *from;
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The last slice of one step's products while the first of the next is read, and so on through that step's slices but the last, whose operands are in
+// registers in the end.  nf, nt: the next step's stages; df, dt: the stages that the loads of a later step go to (parameters of one function with
+// __restrict__: else the compiler lets every read from LDS wait for every load in flight).  codes: the step's codes of bfloat16 rows' features.
+template <class S, class IssueT, class IssueF>
+__device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const mx4_u32x4 *__restrict__ nt, mx4_u32x4 *__restrict__ df, mx4_u32x4 *__restrict__ dt, IssueT &&issue_t,
+                                        IssueF &&issue_f, const int (&at_f)[S::SLICES], const int (&at_t)[S::SLICES], MtFrags<S> (&op)[2], mx4_u32x4 (&codes)[S::FT],
+                                        const MtScales<S> &before, const MtScales<S> &now, mx4_f32x16 (&acc)[S::FT][S::TT]) {
+    auto slice = [&](auto number) {
+        constexpr int s = decltype(number)::value, PRODUCTS = S::FT * S::TT, used = (s + 3) % 4;         // the slice that is multiplied
+        MtFrags<S> &use = op[(s + 1) & 1], &get = op[s & 1];
+#pragma unroll
+        for (int i = 0; i < PRODUCTS; ++i) {
+            const int f = i / S::TT, t = i % S::TT;
+            if constexpr (S::FOUR) {
+                const MtScales<S> &sc = s == 0 ? before : now;
+                acc[f][t] = mx4_multiply_codes_32<2 * (used & 1)>(use.f[f], use.t[t], acc[f][t], sc.f[f][used / 2], sc.t[t][used / 2]);
+            } else {
+                acc[f][t] = mx4_multiply_32(use.f[f], use.t[t], acc[f][t]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                constexpr int ALL = PRODUCTS * (S::SLICES - 1), L = S::LF + S::LT;
+                const int n = s * PRODUCTS + i, l0 = n * L / ALL, l1 = (n + 1) * L / ALL;
+#pragma unroll
+                for (int l = l0; l < l1; ++l) {
+                    if (l < S::LT) issue_t(dt, l);
+                    else if (l < L) issue_f(df, l - S::LT);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (S::FOUR) {
+                constexpr int READS = S::FT + S::TT;
+                const int r0 = i * READS / PRODUCTS, r1 = (i + 1) * READS / PRODUCTS;
+#pragma unroll
+                for (int r = r0; r < r1; ++r) {
+                    if (r < S::TT) mt_read(get.t[r], nt + at_t[s] + 32 * S::TP * r);
+                    else mt_read(get.f[r - S::TT], nf + at_f[s] + 32 * S::FP * (r - S::TT));
+                }
+            } else {
+                constexpr int READS = S::TT + (s == 0 ? S::FT : 0);
+                const int r0 = i * READS / PRODUCTS, r1 = (i + 1) * READS / PRODUCTS;
+#pragma unroll
+                for (int r = r0; r < r1; ++r) {
+                    if (s == 0 && r < S::FT) mt_read(codes[r], nf + at_f[0] + 32 * S::FP * r);
+                    else mt_read(get.t[r - (s == 0 ? S::FT : 0)], nt + at_t[s] + 32 * S::TP * (r - (s == 0 ? S::FT : 0)));
+                }
+                // the next slice's features, in the second half of this one's products
+                constexpr int HALF = PRODUCTS / 2;
+                if (i >= HALF) {
+                    const int f0 = (i - HALF) * S::FT / (PRODUCTS - HALF), f1 = (i + 1 - HALF) * S::FT / (PRODUCTS - HALF);
+#pragma unroll
+                    for (int x = f0; x < f1; ++x) {
+                        get.f[x] = mx4_to_bf16(codes[x][s], mx4_scale(now.f[x][0]));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+        }
+    };
+    slice(std::integral_constant<int, 0>{});
+    slice(std::integral_constant<int, 1>{});
+    slice(std::integral_constant<int, 2>{});
+    slice(std::integral_constant<int, 3>{});
+}
+
+struct MtArgs {
+    const void *x, *xs;             // rows (bfloat16, or codes) and the codes' scales
+    uint32_t ldx, lds, x_bytes, xs_bytes;     // bytes from row to row; of the whole
+    const uint8_t *codes, *scales;
+    uint32_t codes_bytes, scales_bytes;
+    int pairs;
+    void *y;
+    long long ldy;
+    int M, N, steps, w_steps;       // steps of X; of W, which begins anew where it ends
+    int wide_out;
+};
+
+template <class S, int EPI>
+__global__ void __launch_bounds__(S::THREADS, 1)
+mx4_tiles_kernel(MtArgs a) {
+    extern __shared__ __attribute__((aligned(16))) mx4_u32x4 mt_lds[];
+    constexpr int FT = S::FT, TT = S::TT;
+    constexpr bool FOUR = S::FOUR, SWIGLU = EPI >= MT_EPI_SWIGLU, OUT32 = EPI == MT_EPI_F32 || EPI == MT_EPI_SWIGLU_F32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
+    const int wf = wave % S::WF, wt = wave / S::WF;
+    // ---- which tile: workgroups go to the eight dies in turn; a die takes a run of tiles, those of a few feature tiles side by side
+    const int t_tiles = (a.M + S::T - 1) / S::T, f_tiles = (a.N + S::F - 1) / S::F, tiles = t_tiles * f_tiles;
+    const int each = (tiles + 7) / 8, item = blockIdx.x % 8 * each + blockIdx.x / 8;
+    if ((int)blockIdx.x / 8 >= each || item >= tiles) return;
+    const int ft0 = item / t_tiles, tt0 = item - ft0 * t_tiles, half_n = a.N / 2;
+    // row r of the tile's features in W (SwiGLU: in turns 32 gate rows and the up rows that meet them)
+    auto feature = [&](int r) { return SWIGLU ? (r / 32 & 1) * half_n + ft0 * (S::F / 2) + r / 64 * 32 + r % 32 : ft0 * S::F + r; };
+    const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.codes), 0, a.codes_bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t sb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.scales), 0, a.scales_bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(a.x), 0, a.x_bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t xsb = __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(a.xs), 0, a.xs_bytes, 0x00020000);
+    // ---- the loads of a stage: load i of wave w brings the 64 pieces from (i * WAVES + w) * 64 on
+    uint32_t from_f[S::LF], from_t[S::LT];
+#pragma unroll
+    for (int i = 0; i < S::LF; ++i) {
+        const int chunk = i * S::WAVES + wave;
+        // a stage is [tile of 16][step's blocks][feature]
+        const int tile = FOUR ? chunk / 2 : chunk * 2 + lane / 32, block = FOUR ? chunk % 2 * 4 + lane / 16 : lane / 16 & 1, row = feature(tile * 16 + lane % 16);
+        from_f[i] = (uint32_t)mx4_row_codes(row, a.pairs) + block * 256;
+    }
+#pragma unroll
+    for (int i = 0; i < S::LT; ++i) {
+        const int r = (i * S::WAVES + wave) * 8 + lane / 8;
+        from_t[i] = (uint32_t)(tt0 * S::T + r) * a.ldx + 16u * ((lane % 8) ^ (r & 7));
+    }
+    mx4_u32x4 *const lds_f = mt_lds, *const lds_t = mt_lds + S::SF * S::F * S::FP;
+    // (a later step than there are: the last once more, which nobody reads)
+    auto issue_f = [&](mx4_u32x4 *dst, int w_step, int i) {
+        auto *to = (__attribute__((address_space(3))) void *)(dst + (i * S::WAVES + wave) * WAVE);
+        const uint32_t from = from_f[i] + (uint32_t)w_step * S::STEP_CODES;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wb, to, 16, from, 0, 0, 0);
+    };
+    auto issue_t = [&](mx4_u32x4 *dst, int step, int i) {
+        auto *to = (__attribute__((address_space(3))) void *)(dst + (i * S::WAVES + wave) * WAVE);
+        const uint32_t from = from_t[i] + (uint32_t)min(step, a.steps - 1) * 128u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, to, 16, from, 0, 0, 0);
+    };
+    // ---- where the lane's operands stand in a stage
+    int at_f[S::SLICES], at_t[S::SLICES];
+#pragma unroll
+    for (int s = 0; s < S::SLICES; ++s) {
+        at_f[s] = FOUR ? l32 / 16 * 128 + (s * 2 + hi) * 16 + l32 % 16 : l32 / 16 * 32 + hi * 16 + l32 % 16;
+        at_t[s] = l32 * S::TP + ((FOUR ? 2 * s + hi : 4 * hi + s) ^ (l32 & 7));
+    }
+    const int of_f = wf * 32 * FT * S::FP, of_t = wt * 32 * TT * S::TP;
+    uint32_t sf[FT], st[TT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f) sf[f] = (uint32_t)mx4_row_scales(feature(wf * 32 * FT + 32 * f + l32), a.pairs) + (FOUR ? 0 : hi);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) st[t] = (uint32_t)(tt0 * S::T + wt * 32 * TT + 32 * t + l32) * a.lds;
+    auto fetch_scales = [&](MtScales<S> &to, int step, int w_step) {
+        if constexpr (FOUR) {
+            typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+#pragma unroll
+            for (int f = 0; f < FT; ++f) {
+                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sb, sf[f] + (uint32_t)w_step * MX4_PAIR_SCALES, 0, 0));
+                to.f[f][0] = v[0]; to.f[f][1] = v[1];
+            }
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(xsb, st[t] + (uint32_t)step * 8u, 0, 0));
+                to.t[t][0] = v[0]; to.t[t][1] = v[1];
+            }
+        } else {
+#pragma unroll
+            for (int f = 0; f < FT; ++f) to.f[f][0] = __builtin_amdgcn_raw_buffer_load_b8(sb, sf[f] + (uint32_t)(w_step >> 2) * MX4_PAIR_SCALES + 2u * (w_step & 3), 0, 0);
+        }
+    };
+    auto moved = [&](const MtScales<S> &v) {
+        MtScales<S> o = v;
+        if constexpr (FOUR) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int f = 0; f < FT; ++f) o.f[f][h] = v.f[f][h] >> 8 * hi;
+#pragma unroll
+                for (int t = 0; t < TT; ++t) o.t[t][h] = v.t[t][h] >> 8 * hi;
+            }
+        }
+        return o;
+    };
+    mx4_f32x16 acc[FT][TT];
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[f][t][i] = 0.f;
+    MtFrags<S> op[2];
+    mx4_u32x4 codes[FT];
+    MtScales<S> before, now, next;
+#pragma unroll
+    for (int f = 0; f < FT; ++f) {
+        op[1].f[f] = codes[f] = mx4_u32x4{0u, 0u, 0u, 0u};
+        before.f[f][0] = before.f[f][FOUR ? 1 : 0] = 0;
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        op[1].t[t] = mx4_u32x4{0u, 0u, 0u, 0u};
+        before.t[FOUR ? t : 0][0] = before.t[FOUR ? t : 0][1] = 0;
+    }
+    // W's step of the features' ring: one that goes round
+    int wf_step = 0;
+    auto next_w = [&](int s) { return s + 1 == a.w_steps ? 0 : s + 1; };
+    // what SF - 1 turns before the first would have asked for
+    fetch_scales(next, 0, 0);
+#pragma unroll
+    for (int j = 1 - S::SF; j < 0; ++j) {
+        if (j + S::ST - 1 >= 0) {
+#pragma unroll
+            for (int i = 0; i < S::LT; ++i) issue_t(lds_t + (j + S::ST - 1) * S::T * S::TP, j + S::ST - 1, i);
+        }
+#pragma unroll
+        for (int i = 0; i < S::LF; ++i) issue_f(lds_f + (j + S::SF - 1) * S::F * S::FP, wf_step, i);
+        wf_step = next_w(wf_step);
+    }
+    int rf = 0, rt = 0, df = S::SF - 1, dt = S::ST - 1, s_step = 0;
+    for (int t = 0; t < a.steps; ++t) {
+        now = moved(next);
+        s_step = next_w(s_step);
+        fetch_scales(next, min(t + 1, a.steps - 1), s_step);
+        mt_wait_loads<S::LEFT>();                              // this step's stages are there
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        mt_turn<S>(lds_f + rf * S::F * S::FP + of_f, lds_t + rt * S::T * S::TP + of_t, lds_f + df * S::F * S::FP, lds_t + dt * S::T * S::TP,
+                   [&](mx4_u32x4 *dst, int i) { issue_t(dst, t + S::ST - 1, i); }, [&](mx4_u32x4 *dst, int i) { issue_f(dst, wf_step, i); }, at_f, at_t, op, codes, before, now, acc);
+        before = now;
+        wf_step = next_w(wf_step);
+        rf = rf + 1 == S::SF ? 0 : rf + 1;
+        rt = rt + 1 == S::ST ? 0 : rt + 1;
+        df = df + 1 == S::SF ? 0 : df + 1;
+        dt = dt + 1 == S::ST ? 0 : dt + 1;
+    }
+    // the last slice
+#pragma unroll
+    for (int i = 0; i < FT * TT; ++i) {
+        const int f = i / TT, t = i % TT;
+        if constexpr (FOUR) acc[f][t] = mx4_multiply_codes_32<2>(op[1].f[f], op[1].t[t], acc[f][t], before.f[f][1], before.t[t][1]);
+        else acc[f][t] = mx4_multiply_32(op[1].f[f], op[1].t[t], acc[f][t]);
+    }
+    mt_wait_loads<0>();                                        // (the copies that nobody reads have landed before LDS is used otherwise)
+    __syncthreads();
+    // ---- out: a wave turns 32 tokens at a time through LDS of its own, and stores whole rows of its features
+    constexpr int OUT_F = SWIGLU ? 16 * FT : 32 * FT, ELEM = OUT32 ? 4 : 2, PITCH = OUT_F * ELEM + 16, CH = OUT_F * ELEM / 16;
+    static_assert(S::WAVES * 32 * PITCH <= S::LDS * 16, "room for the waves' rows");
+    char *mine = (char *)mt_lds + wave * 32 * PITCH;
+    const int out_n = SWIGLU ? half_n : a.N, f0 = (SWIGLU ? ft0 * (S::F / 2) : ft0 * S::F) + wf * OUT_F;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+        for (int f = 0; f < (SWIGLU ? FT / 2 : FT); ++f)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {                      // features 32 f + 8 q + 4 hi ..
+                char *to = mine + l32 * PITCH + (32 * f + 8 * q + 4 * hi) * ELEM;
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = SWIGLU ? gate_up<GATE_SILU>(acc[2 * f % FT][t][4 * q + e], acc[(2 * f + 1) % FT][t][4 * q + e], 0.f, 0.f) : acc[f][t][4 * q + e];
+                if constexpr (OUT32) *(mx4_f32x4 *)to = mx4_f32x4{o[0], o[1], o[2], o[3]};
+                else *(uint2 *)to = make_uint2(pack2_bf16(o[0], o[1]), pack2_bf16(o[2], o[3]));
+            }
+        const int tok0 = tt0 * S::T + wt * 32 * TT + 32 * t;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (a.wide_out) {
+#pragma unroll
+            for (int x = 0; x < 32 * CH / WAVE; ++x) {
+                const int i = x * WAVE + lane, row = i / CH, c = i % CH, col = f0 + c * (16 / ELEM);
+                const mx4_u32x4 v = *(const mx4_u32x4 *)(mine + row * PITCH + c * 16);
+                if (tok0 + row < a.M && col < out_n) *(mx4_u32x4 *)((char *)a.y + ((size_t)(tok0 + row) * a.ldy + col) * ELEM) = v;
+            }
+        } else {
+            for (int i = lane; i < 32 * OUT_F; i += WAVE) {
+                const int row = i / OUT_F, col = f0 + i % OUT_F;
+                if (tok0 + row >= a.M || col >= out_n) continue;
+                if constexpr (OUT32) ((float *)a.y)[(size_t)(tok0 + row) * a.ldy + col] = *(const float *)(mine + row * PITCH + i % OUT_F * 4);
+                else ((uint16_t *)a.y)[(size_t)(tok0 + row) * a.ldy + col] = *(const uint16_t *)(mine + row * PITCH + i % OUT_F * 2);
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+template <class S, int EPI>
+static int mt_go(const MtArgs &a, hipStream_t stream) {
+    const int tiles = ((a.M + S::T - 1) / S::T) * ((a.N + S::F - 1) / S::F);
+    constexpr int bytes = S::LDS * 16;
+    static bool asked = false;
+    if (!asked && bytes > 64 * 1024) {                         // more LDS than a launch gets unasked
+        const hipError_t e = hipFuncSetAttribute((const void *)mx4_tiles_kernel<S, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return (int)e;
+        asked = true;
+    }
+    mx4_tiles_kernel<S, EPI><<<dim3((tiles + 7) / 8 * 8), dim3(S::THREADS), bytes, stream>>>(a);
+    LCU_LAUNCH_CHECK();
+    return LCU_OK;
+}
+
+// Arguments as lcu_mx4_stream's; rows in 4 bits and their scales in whole pairs of macro-steps (256 k), bfloat16 rows in multiples of 64 k.  shape: 0: tiles of 128 x 128
+// (features x tokens), 1: 256 x 256.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
+LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *xs, long long lds, const void *codes, const void *scales, int pairs, void *y, long long ldy,
+                          int M, int N, int K, int epi, int shape, hipStream_t stream) {
+    if (M <= 0 || N <= 0) return LCU_OK;
+    const int macros = (K + 127) / 128, cols = epi >= MT_EPI_SWIGLU ? N / 2 : N, elem = epi == MT_EPI_F32 || epi == MT_EPI_SWIGLU_F32 ? 4 : 2;
+    const long long w_rows = (N + 15) / 16 * 16, row_bytes = x_kind == 4 ? ldx : ldx * 2, limit = 1ll << 32;
+    if (K <= 0 || pairs < (macros + 1) / 2 || ldy < cols || epi < 0 || epi > MT_EPI_SWIGLU_F32 || (epi >= MT_EPI_SWIGLU && N % 2) || !x || !codes || !scales || !y ||
+        ((uintptr_t)x | (uintptr_t)codes) % 16 || (uintptr_t)scales % 8 || row_bytes <= 0 || row_bytes % 16 || (M + 512ll) * row_bytes >= limit || (w_rows + 512) * pairs * 128 >= limit)
+        return LCU_BAD_ARGUMENT;
+    if (x_kind == 1 ? ldx < 128ll * macros : x_kind == 3 ? ldx % 768 || ldx < 3ll * macros * 128
+        : x_kind == 4 ? !xs || lds % 8 || (uintptr_t)xs % 8 || ldx < 128ll * ((macros + 1) / 2) || lds < 8ll * ((macros + 1) / 2) || (M + 512ll) * lds >= limit : true)
+        return LCU_BAD_ARGUMENT;
+    MtArgs a = {};
+    a.x = x; a.xs = xs;
+    a.ldx = (uint32_t)row_bytes; a.lds = (uint32_t)lds;
+    a.codes = (const uint8_t *)codes; a.scales = (const uint8_t *)scales;
+    a.codes_bytes = (uint32_t)(w_rows * pairs * 128); a.scales_bytes = (uint32_t)(w_rows * pairs * 8);
+    a.pairs = pairs; a.y = y; a.ldy = ldy; a.M = M; a.N = N;
+    // steps: 256 k in 4 bits, else 64; three planes one behind the other are rows of three times as many, filled up to whole pairs
+    const int two = (macros + 1) / 2;
+    a.w_steps = x_kind == 4 ? two : x_kind == 3 ? (int)(ldx / 3 / 64) : macros * 2;
+    a.steps = x_kind == 3 ? 3 * a.w_steps : a.w_steps;
+    if (x_kind == 3 && a.w_steps > pairs * 4) return LCU_BAD_ARGUMENT;
+    a.x_bytes = (uint32_t)((M - 1) * row_bytes + (long long)a.steps * 128);
+    a.xs_bytes = x_kind == 4 ? (uint32_t)((M - 1) * lds + two * 8ll) : 0u;
+    a.wide_out = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % 16 == 0;
+#define EPIS(...)                                                            \
+    do {                                                                     \
+        typedef MtShape<__VA_ARGS__> S;                                       \
+        if (epi == MT_EPI_BF16) return mt_go<S, MT_EPI_BF16>(a, stream);      \
+        if (epi == MT_EPI_F32) return mt_go<S, MT_EPI_F32>(a, stream);        \
+        if (epi == MT_EPI_SWIGLU) return mt_go<S, MT_EPI_SWIGLU>(a, stream);  \
+        return mt_go<S, MT_EPI_SWIGLU_F32>(a, stream);                        \
+    } while (0)
+    if (x_kind == 4) {
+        if (shape == 0) EPIS(true, 2, 2, 2, 2, 4, 4);
+        if (shape == 1) EPIS(true, 4, 2, 2, 4, 3, 2);
+    } else {
+        if (shape == 0) EPIS(false, 2, 2, 2, 2, 6, 6);
+        if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
+    }
+#undef EPIS
+    return LCU_BAD_ARGUMENT;
+}

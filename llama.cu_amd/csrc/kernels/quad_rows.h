@@ -1,7 +1,7 @@
 #pragma once
 #include "common.h"
 
-// Rows of bfloat16 as the second operand of v_mfma_f32_16x16x32_bf16 (a column of sixteen a row, lane group g of sixteen lanes the k from
+// Rows of bfloat16 as the second operand of the matrix instruction of 16 x 16 x 32 (a column of sixteen a row, lane group g of sixteen lanes the k from
 // 8 g on), straight from memory into registers.  A compute unit looks a cache line up for every four neighbouring lanes of a 16-byte load:
 // lanes that lie side by side in the operand are different rows, so a load in the operand's order takes a cycle for every lane, 16 bytes
 // a cycle, where four lanes that read 64 bytes of one row take one cycle together (a product of 16 rows with K = 2048 in every workgroup:

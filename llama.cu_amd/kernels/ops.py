@@ -2825,9 +2825,9 @@ def _mx4_rows(x: torch.Tensor, k: int) -> Tuple[torch.Tensor, int]:
 
 
 def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
-    """Rows in 4 bits as the products read them: whole macro-steps of 128, rows on 16 bytes, scales on 4."""
-    fits = (q._filled or blocks % 4 == 0) and q.codes.data_ptr() % 16 == 0 and q.scales.data_ptr() % 4 == 0 \
-        and (q.codes.shape[0] == 1 or (q.codes.stride(0) % 16 == 0 and q.codes.stride(0) < 1 << 24 and q.scales.stride(0) % 4 == 0))
+    """Rows in 4 bits as the products read them: whole pairs of macro-steps, rows on 16 bytes, scales on 8."""
+    fits = (q._filled or blocks % 8 == 0) and q.codes.data_ptr() % 16 == 0 and q.scales.data_ptr() % 8 == 0 \
+        and (q.codes.shape[0] == 1 or (q.codes.stride(0) % 16 == 0 and q.codes.stride(0) < 1 << 24 and q.scales.stride(0) % 8 == 0 and q.scales.stride(0) < 1 << 24))
     if fits:
         return q
     whole = -(-blocks // 8) * 8
@@ -2836,6 +2836,14 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     codes[:, :16 * blocks] = q.codes
     scales[:, :blocks] = q.scales
     return Mx4(codes[:, :16 * blocks], scales[:, :blocks], q.k, True)
+
+
+def mx4_choice(m: int, n: int, k: int, kind: int, swiglu: bool) -> int:
+    """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: -1 the one that streams the weight, else the shape of the
+    tiles (mx4_tiles.hip)."""
+    if m <= 64:
+        return -1
+    return 1 if m > 128 and (m + 255) // 256 * ((n + 255) // 256) * 2 > TUNING.compute_units else 0
 
 
 def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, swiglu: bool = False) -> torch.Tensor:
@@ -2877,6 +2885,20 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         ld, scales, lds = rows.stride(0), None, 0
     if m == 1:                             # (the one row's stride says nothing)
         ld, lds = (128 * w.pairs, 8 * w.pairs) if four else (rows.shape[1], 0)
-    _check(build.load("mx4_stream").lcu_mx4_stream(_ptr(rows), ctypes.c_longlong(ld), kind, _ptr(scales), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), w.pairs, _ptr(out),
-                                                   ctypes.c_longlong(out.stride(0) if m > 1 else cols), m, w.n, k, (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0), _stream()), "gemm_mx4")
+    shape = mx4_choice(m, w.n, k, kind, swiglu)
+    row_bytes = ld if four else 2 * ld
+    most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
+    if shape >= 0 and (most < 512 or (w.n + 528) * w.pairs * 128 >= 1 << 32):
+        shape = -1
+    head = (w.pairs, _ptr(out), ctypes.c_longlong(out.stride(0) if m > 1 else cols))
+    tail = (w.n, k, (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0))
+    if shape < 0:
+        _check(build.load("mx4_stream").lcu_mx4_stream(_ptr(rows), ctypes.c_longlong(ld), kind, _ptr(scales), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), *head, m, *tail,
+                                                       _stream()), "gemm_mx4")
+        return out
+    lib = build.load("mx4_tiles")
+    for r in range(0, m, most):
+        part, sc, to = (rows, scales, out) if m <= most else (rows[r:r + most], None if scales is None else scales[r:r + most], out[r:r + most])
+        _check(lib.lcu_mx4_tiles(_ptr(part), ctypes.c_longlong(ld), kind, _ptr(sc), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), w.pairs, _ptr(to), head[2],
+                                 min(most, m - r), *tail, shape, _stream()), "gemm_mx4")
     return out

@@ -154,6 +154,54 @@ def test_product(n, k, kind):
                 assert_close(ops.gemm_mx4(rows, w, out_dtype=dtype, swiglu=True), act, REL[dtype] + 2e-5, f"swiglu of {m} rows to {dtype}")
 
 
+@pytest.mark.parametrize("shape", [0, 1])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "four"])
+# fewer steps of k than a ring holds, as many, and more; tiles that end within rows and features; gate and up that meet within a tile of 16
+@pytest.mark.parametrize("m,n,k", [(1, 48, 32), (127, 130, 128), (130, 258, 640), (257, 600, 1000), (300, 72, 1536), (515, 1030, 384)])
+def test_product_in_tiles(m, n, k, kind, shape, monkeypatch):
+    from llama_cu_amd.kernels import ops
+    monkeypatch.setattr(ops, "mx4_choice", lambda *a: shape)
+    w, exact = weight(n, k)
+    x = rnd(m, k, seed=m).to(torch.float32 if kind == "float32" else torch.bfloat16)
+    x[:, ::7] *= 20.0
+    rows, mine = (ops.mx4_quantize(x.cuda()), values(*quantised(x), k)) if kind == "four" else (x.cuda(), x.double())
+    want = mine @ exact.T
+    gate, up = want.chunk(2, 1)
+    act = gate * torch.sigmoid(gate) * up
+    for dtype in (torch.bfloat16, torch.float32):
+        for swiglu in (False, True):
+            cols = n // 2 if swiglu else n
+            got = ops.gemm_mx4(rows, w, out_dtype=dtype, swiglu=swiglu)
+            assert_close(got, act if swiglu else want, REL[dtype] + 2e-5 * swiglu, f"{dtype} swiglu {swiglu}")
+            for shift in (0, 3):
+                room = torch.full((m + 2, cols + 11), 7.0, dtype=dtype, device="cuda")
+                ops.gemm_mx4(rows, w, out=room[1:1 + m, shift:shift + cols], swiglu=swiglu)
+                assert torch.equal(room[1:1 + m, shift:shift + cols], got)
+                assert (room[0] == 7).all() and (room[m + 1:] == 7).all() and (room[:, :shift] == 7).all() and (room[:, shift + cols:] == 7).all()
+
+
+@pytest.mark.parametrize("shape", [0, 1])
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "four"])
+def test_rows_and_features_know_nothing_of_each_other(kind, shape, monkeypatch):
+    """A row of NaN and a feature of NaN reach their own row and column only; what lies behind the rows' k and behind the last row is not looked at."""
+    from llama_cu_amd.kernels import ops
+    monkeypatch.setattr(ops, "mx4_choice", lambda *a: shape)
+    m, n, k = 200, 144, 128
+    wide = rnd(m + 1, 2 * k, seed=1).to(torch.float32 if kind == "float32" else torch.bfloat16)
+    wide[:, k:] = float("nan")
+    wide[m] = float("nan")
+    wide[70, :k] = float("nan")
+    source = rnd(n, k, seed=2).bfloat16()
+    source[9] = float("inf")
+    w = ops.pack_mx4(ops.mx4_quantize(source.cuda()))
+    x = wide.cuda()[:m, :k]
+    y = ops.gemm_mx4(ops.mx4_quantize(x) if kind == "four" else x, w).float().cpu()
+    good = torch.ones(m, n, dtype=torch.bool)
+    good[70] = False
+    good[:, 9] = False
+    assert torch.isfinite(y[good]).all() and torch.isnan(y[70]).all() and torch.isnan(y[:, 9]).all()
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "four"])
 def test_where_the_product_goes(kind):
     """Into rows of wider memory, aligned or not, and nowhere else; from rows of wider memory, on any address."""
