@@ -2,15 +2,18 @@
 //
 // With the logits in descending order (equal ones by index), weights w_i = exp((l_i - l_0) / T) and prefix sums c, a draw takes the first
 // entry with c_i >= u L, L = min(top_p c_n, c_k): entry i has the share (min(c_i, L) - min(c_{i-1}, L)) / L, so the entry at the cut
-// keeps the part of its weight that lies within.  Nothing is sorted.  Four launches, a row cut into parts in the first three:
+// keeps the part of its weight that lies within.  Nothing is sorted.  Six launches, a row cut into parts in those that read or write it:
 //   max     the largest logit, where it stands, and the sum of all weights, in one pass with a running maximum;
-//   count   a histogram of the distances (l_0 - l) / T, counts alone: a bin's weights are known to within its width, so the bins in which
-//           the cut can lie are known from it, and which entries are kept in full;
+//   count   a histogram of the distances (l_0 - l) / T, counts alone;
+//   bracket a bin's weights are known to within its width, so the bins in which the cut can lie are known from the counts, and which entries are kept in
+//           full;
 //   write   rows without a cut are written.  Of the others what is not kept becomes zero; entries that are, or may be, are gathered;
-//   cut     one workgroup a row finds the cut among the gathered entries bit by bit of their order, on sums of 64-bit fixed-point
+//   cut     one workgroup a row finds the cut among the gathered entries, eight bits of their order at a time, on sums of 64-bit fixed-point
 //           weights (w 2^44: no order of additions changes them), and writes their shares.
 // Where more entries are kept than are gathered (a flat row) only those near the cut are, with the exact sum of what lies above, and the
-// last launch writes the whole row; where even those are too many (tens of thousands of equal logits) it searches the row itself.
+// last launch
+//   store   writes the whole row.
+// Where even those near the cut are too many (tens of thousands of equal logits) `cut` searches the row itself.
 //
 // A NaN counts as -inf, which has no share; a row of nothing else becomes zeros.  Infinities of the one sign share alike.  A temperature
 // that is not positive leaves the first of the largest logits.
@@ -18,16 +21,23 @@
 
 constexpr int TP_THREADS = 512, TP_CUT_THREADS = 1024, TP_BINS = 8192, TP_GATHER = 8192, TP_EACH = TP_GATHER / TP_CUT_THREADS, TP_MAX_PARTS = 32, TP_MAX_VOCAB = 1 << 19;
 constexpr double TP_ONE = 17592186044416.0;          // 2^44: 2^19 weights of 1 are 2^63
-constexpr float TP_NOTHING = 104.f;                  // exp(-104) is no 32-bit number any more
+constexpr float TP_NOTHING = 126.f;                  // the exponential ends at 2^-126
+constexpr float TP_LOG2E = 1.44269504088896341f;
 
-struct TpPart {                                      // of a part of a row: its largest logit and where, its smallest but -inf, its weights' sum
+struct TpPart {                                      // of a part of a row: its largest logit and where, its smallest, its weights' sum
     double sum;
     float most, least;
     int at, pad;
 };
 struct TpRow {
     unsigned long long mass_above;                   // of entries kept in full that are not gathered
-    unsigned int gathered, pad;
+    unsigned int gathered;
+    int bin_lo, bin_hi;                              // the bins in which the cut can lie
+    unsigned int before, upto;                       // how many entries lie in the bins before them, and up to the last of them
+    // the cut: which key, which of the equal ones is the last that is kept, and the part that it has, the scale of what is kept whole
+    unsigned int border;
+    int last, store;                                 // store: the row is yet to be written
+    float kept, inv;
 };
 struct TpEntry { unsigned int key; int at; };
 
@@ -37,32 +47,40 @@ __device__ __forceinline__ unsigned int tp_key(float x) {
 }
 __device__ __forceinline__ float tp_logit(unsigned int k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// What a row's options are, and what the parts have found.
+// What a row's options are, and what the parts have found.  Distances are those of the exponents of two: (l_0 - l) / T log2(e).
 struct TpCut {
-    float most, inv_t, per_bin;                      // per_bin: bins for one unit of distance
+    float most, inv_t, per_bin;                      // inv_t: log2(e) / T; per_bin: bins for one unit of distance
     double sum, limit_p;                             // limit_p: top_p times the sum
     int k, at;
     bool empty, greedy, cuts;
 };
-__device__ __forceinline__ float tp_distance(const TpCut &c, float l) { return l == c.most ? 0.f : (c.most - l) * c.inv_t; }
-__device__ __forceinline__ float tp_weight(float distance) { return expf(-distance); }
-__device__ __forceinline__ unsigned long long tp_fixed(float w) { return (unsigned long long)((double)w * TP_ONE); }
+// (the maximum with 0 makes 0 of what is no number: an infinite logit's distance from itself, and 0 times an infinite 1 / T)
+__device__ __forceinline__ float tp_apart(float most, float l, float inv_t) { return fmaxf((most - l) * inv_t, 0.f); }
+__device__ __forceinline__ float tp_distance(const TpCut &c, float l) { return tp_apart(c.most, l, c.inv_t); }
+__device__ __forceinline__ float tp_weight(float distance) { return __builtin_amdgcn_exp2f(-distance); }
+// w 2^44, w at most 1: the mantissa where the exponent puts it
+__device__ __forceinline__ unsigned long long tp_fixed(float w) {
+    const unsigned int bits = __float_as_uint(w), down = 127u - (bits >> 23);
+    return down < 64u ? (unsigned long long)((bits & 0x7fffffu) | 0x800000u) << 21 >> down : 0ull;
+}
 __device__ __forceinline__ int tp_bin(const TpCut &c, float distance) { return min((int)(distance * c.per_bin), TP_BINS - 1); }
-__device__ __forceinline__ float tp_clean(float l) { return l != l ? -INFINITY : l; }
+__device__ __forceinline__ float tp_clean(float l) { return fmaxf(l, -INFINITY); }      // (of a NaN and a number the maximum is the number)
 
+// Every lane of a wave calls it and gets the answer: a lane a part (one after the other they are a trip to memory each, 10 us of 31 parts).
 __device__ __forceinline__ TpCut tp_row(const TpPart *__restrict__ part, int parts, int vocab, float temperature, float top_p, int top_k) {
+    static_assert(TP_MAX_PARTS <= 32, "half a wave");
+    const int lane = threadIdx.x & 31;
+    const TpPart mine = part[lane < parts ? lane : 0];
     TpCut c;
-    c.most = -INFINITY;
-    c.at = 0x7fffffff;
-    float least = INFINITY;
-    for (int p = 0; p < parts; ++p) {
-        if (part[p].most > c.most) { c.most = part[p].most; c.at = part[p].at; }       // (parts in order: the first of equal ones stays)
-        least = fminf(least, part[p].least);
-    }
-    c.inv_t = 1.0f / temperature;
-    c.sum = 0.0;
-    for (int p = 0; p < parts; ++p)
-        if (part[p].most > -INFINITY) c.sum += part[p].sum * (double)tp_weight(tp_distance(c, part[p].most));
+    c.most = mine.most;
+    float least = mine.least;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) { c.most = fmaxf(c.most, __shfl_xor(c.most, off, WAVE)); least = fminf(least, __shfl_xor(least, off, WAVE)); }
+    c.inv_t = TP_LOG2E / temperature;
+    c.at = mine.most == c.most ? mine.at : 0x7fffffff;
+    c.sum = lane < parts && mine.most > -INFINITY ? mine.sum * (double)tp_weight(tp_distance(c, mine.most)) : 0.0;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) { c.at = min(c.at, __shfl_xor(c.at, off, WAVE)); c.sum += __shfl_xor(c.sum, off, WAVE); }
     c.empty = c.most == -INFINITY;
     c.k = top_k;
     c.greedy = !(temperature > 0.f) || top_k <= 1 || !(top_p > 0.f);
@@ -73,21 +91,45 @@ __device__ __forceinline__ TpCut tp_row(const TpPart *__restrict__ part, int par
     return c;
 }
 
-// A stretch of a row, at borders of four: f(index, logit) of every entry.
+// A stretch of a row, at borders of four: f(index, four logits) of every four (WIDE; else one at a time, the others -inf), loads of four such on their way
+// at once: with one the row came at 3.4 TB/s.
+template <bool WIDE, class F>
+__device__ __forceinline__ void tp_fours(const float *__restrict__ row, int lo, int hi, F f) {
+    constexpr int AT_ONCE = 4, V = WIDE ? 4 : 1;
+    const int step = V * (int)blockDim.x;
+    auto load = [&](int i) {
+        if constexpr (WIDE) return *(const float4 *)(row + i);
+        else return make_float4(row[i], -INFINITY, -INFINITY, -INFINITY);
+    };
+    auto give = [&](int i, const float4 &v) {
+        const float l[4] = {tp_clean(v.x), tp_clean(v.y), tp_clean(v.z), tp_clean(v.w)};
+        f(i, l);
+    };
+    int i = lo + V * (int)threadIdx.x;
+    for (; i + (AT_ONCE - 1) * step < hi; i += AT_ONCE * step) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) v[u] = load(i + u * step);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) give(i + u * step, v[u]);
+    }
+    for (; i < hi; i += step) give(i, load(i));
+}
+// f(index, logit) of every entry.
 template <bool WIDE, class F>
 __device__ __forceinline__ void tp_scan(const float *__restrict__ row, int lo, int hi, F f) {
-    if constexpr (WIDE) {
-        for (int i = lo + 4 * (int)threadIdx.x; i < hi; i += 4 * (int)blockDim.x) {
-            if (i + 4 <= hi) {
-                const float4 v = *(const float4 *)(row + i);
-                f(i, tp_clean(v.x)); f(i + 1, tp_clean(v.y)); f(i + 2, tp_clean(v.z)); f(i + 3, tp_clean(v.w));
-            } else {
-                for (int j = i; j < hi; ++j) f(j, tp_clean(row[j]));
-            }
-        }
-    } else {
-        for (int i = lo + (int)threadIdx.x; i < hi; i += (int)blockDim.x) f(i, tp_clean(row[i]));
-    }
+    tp_fours<WIDE>(row, lo, hi, [&](int i, const float (&l)[4]) {
+#pragma unroll
+        for (int e = 0; e < (WIDE ? 4 : 1); ++e) f(i + e, l[e]);
+    });
+}
+// The shares of every entry, share(index, logit), to `to`.
+template <bool WIDE, class F>
+__device__ __forceinline__ void tp_store_shares(const float *__restrict__ row, int lo, int hi, float *__restrict__ to, F share) {
+    tp_fours<WIDE>(row, lo, hi, [&](int i, const float (&l)[4]) {
+        if constexpr (WIDE) *(float4 *)(to + i) = make_float4(share(i, l[0]), share(i + 1, l[1]), share(i + 2, l[2]), share(i + 3, l[3]));
+        else to[i] = share(i, l[0]);
+    });
 }
 __device__ __forceinline__ void tp_stretch(int vocab, int part, int parts, int &lo, int &hi) {
     const int fours = (vocab + 3) / 4, each = (fours + parts - 1) / parts;
@@ -106,25 +148,35 @@ tp_max_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
         for (int b = (int)blockIdx.y * TP_THREADS + threadIdx.x; b < TP_BINS; b += TP_THREADS * parts) hist[(size_t)r * TP_BINS + b] = 0u;
         if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].mass_above = 0; rows[r].gathered = 0; }
     }
-    const float inv_t = 1.0f / temperature[r];
+    const float inv_t = TP_LOG2E / temperature[r];
     float most = -INFINITY, least = INFINITY;
     double sum = 0.0;
     int at = 0x7fffffff;
-    tp_scan<WIDE>(logits + r * ld, lo, hi, [&](int i, float l) {
-        if (l > most) {
-            sum = most > -INFINITY ? sum * (double)expf((most - l) * inv_t) : 0.0;
-            most = l;
-            at = i;
+    // four at a time: what they add is summed in 32 bits, the sum of it all in 64
+    auto four = [&](int i, const float (&l)[4]) {
+        const float top = fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3]));
+        if (top > most) {
+            sum = most > -INFINITY ? sum * (double)tp_weight(tp_apart(top, most, inv_t)) : 0.0;
+            most = top;
+            at = i + (l[0] == top ? 0 : l[1] == top ? 1 : l[2] == top ? 2 : 3);
         }
-        if (l > -INFINITY) { sum += l == most ? 1.0 : (double)expf((l - most) * inv_t); least = fminf(least, l); }
-    });
+        if (most > -INFINITY) {
+            float add = 0.f;
+#pragma unroll
+            for (int e = 0; e < (WIDE ? 4 : 1); ++e) add += tp_weight(tp_apart(most, l[e], inv_t));
+            sum += (double)add;
+        }
+#pragma unroll
+        for (int e = 0; e < (WIDE ? 4 : 1); ++e) least = fminf(least, l[e]);
+    };
+    tp_fours<WIDE>(logits + r * ld, lo, hi, four);
     __shared__ TpPart mine[TP_THREADS / WAVE];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float all = wave_max(most);
     int first = most == all ? at : 0x7fffffff;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) { first = min(first, __shfl_xor(first, off, WAVE)); least = fminf(least, __shfl_xor(least, off, WAVE)); }
-    sum = most > -INFINITY ? (most == all ? sum : sum * (double)expf((most - all) * inv_t)) : 0.0;
+    sum = most > -INFINITY ? (most == all ? sum : sum * (double)tp_weight(tp_apart(all, most, inv_t))) : 0.0;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, WAVE);
     if (lane == 0) mine[wave] = {sum, all, least, first, 0};
@@ -137,7 +189,7 @@ tp_max_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
         }
         t.sum = 0.0;
         for (int w = 0; w < TP_THREADS / WAVE; ++w)
-            if (mine[w].most > -INFINITY) t.sum += mine[w].most == t.most ? mine[w].sum : mine[w].sum * (double)expf((mine[w].most - t.most) * inv_t);
+            if (mine[w].most > -INFINITY) t.sum += mine[w].most == t.most ? mine[w].sum : mine[w].sum * (double)tp_weight(tp_apart(t.most, mine[w].most, inv_t));
         part[(size_t)r * parts + blockIdx.y] = t;
     }
 }
@@ -163,29 +215,31 @@ tp_count_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
         if (count[b]) atomicAdd(&hist[(size_t)r * TP_BINS + b], count[b]);
 }
 
-// The bins lo .. hi in which the cut can lie; how many entries lie in the bins before lo and up to hi.
-struct TpBracket { int lo, hi; unsigned int before, upto; };
-
-// Every thread of the workgroup calls it and gets the answer.
-template <int THREADS>
-__device__ TpBracket tp_bracket(const TpCut &c, const unsigned int *__restrict__ hist) {
-    constexpr int EACH = TP_BINS / THREADS, WAVES = THREADS / WAVE;
+// The bins in which the cut can lie.
+__global__ void __launch_bounds__(TP_CUT_THREADS)
+tp_bracket_kernel(int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k, const TpPart *__restrict__ part, int parts,
+                  TpRow *__restrict__ rows, const unsigned int *__restrict__ hists) {
+    constexpr int EACH = TP_BINS / TP_CUT_THREADS, WAVES = TP_CUT_THREADS / WAVE;
+    const int r = blockIdx.x;
+    const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
+    if (c.empty || c.greedy || !c.cuts) return;
+    const unsigned int *__restrict__ hist = hists + (size_t)r * TP_BINS;
     __shared__ unsigned int wave_n[WAVES];
     __shared__ double wave_lo[WAVES], wave_hi[WAVES];
     __shared__ int found_k, found_lo, found_hi;
-    __shared__ unsigned int n_before, n_upto;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) { found_k = found_lo = found_hi = TP_BINS - 1; n_before = n_upto = 0; }
+    if (threadIdx.x == 0) { found_k = found_lo = found_hi = TP_BINS - 1; }
     // a bin's weights lie between its borders': with room for the roundings of the distances and of the weights
     const float wide = c.per_bin > 0.f ? 1.0f / c.per_bin : 0.f;
     unsigned int n[EACH], n_mine = 0;
-    double least[EACH], least_mine = 0.0, most_mine = 0.0, most[EACH];
+    double least[EACH], least_mine = 0.0, most[EACH], most_mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) n[e] = hist[threadIdx.x * EACH + e];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int b = (int)threadIdx.x * EACH + e;
-        n[e] = hist[b];
-        most[e] = n[e] ? (double)n[e] * expf(-(float)b * wide) * 1.0001 : 0.0;
-        least[e] = n[e] ? (double)n[e] * expf(-(float)(b + 1) * wide) * 0.9999 : 0.0;
+        most[e] = (double)n[e] * (double)(tp_weight((float)b * wide) * 1.0001f);
+        least[e] = (double)n[e] * (double)(tp_weight((float)(b + 1) * wide) * 0.9999f);
         n_mine += n[e]; most_mine += most[e]; least_mine += least[e];
     }
     unsigned int n_scan = n_mine;
@@ -202,40 +256,42 @@ __device__ TpBracket tp_bracket(const TpCut &c, const unsigned int *__restrict__
     double most_at = most_scan - most_mine, least_at = least_scan - least_mine;
     for (int w = 0; w < wave; ++w) { n_at += wave_n[w]; most_at += wave_hi[w]; least_at += wave_lo[w]; }
     const unsigned int n_first = n_at;
+    int first_k = TP_BINS, first_lo = TP_BINS, first_hi = TP_BINS;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int b = (int)threadIdx.x * EACH + e;
         n_at += n[e]; most_at += most[e]; least_at += least[e];
-        if (n_at >= (unsigned int)c.k) atomicMin(&found_k, b);
-        if (most_at >= c.limit_p) atomicMin(&found_lo, b);
-        if (least_at >= c.limit_p) atomicMin(&found_hi, b);
+        if (first_k == TP_BINS && n_at >= (unsigned int)c.k) first_k = b;
+        if (first_lo == TP_BINS && most_at >= c.limit_p) first_lo = b;
+        if (first_hi == TP_BINS && least_at >= c.limit_p) first_hi = b;
     }
+    // (a wave's first lane that is over has the wave's first bin; all lanes behind it are over too, and their minima would be taken one after the other)
+    auto first_of = [&](int mine, int *to) {
+        const unsigned long long over = __ballot(mine < TP_BINS);
+        if (over && lane == __ffsll(over) - 1) atomicMin(to, mine);
+    };
+    first_of(first_k, &found_k);
+    first_of(first_lo, &found_lo);
+    first_of(first_hi, &found_hi);
     __syncthreads();
-    TpBracket out;
-    out.lo = min(found_k, found_lo);
-    out.hi = min(found_k, found_hi);
+    const int lo = min(found_k, found_lo), hi = min(found_k, found_hi);
     n_at = n_first;
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
         const int b = (int)threadIdx.x * EACH + e;
-        if (b == out.lo) n_before = n_at;
+        if (b == lo) { rows[r].bin_lo = lo; rows[r].before = n_at; }
         n_at += n[e];
-        if (b == out.hi) n_upto = n_at;
+        if (b == hi) { rows[r].bin_hi = hi; rows[r].upto = n_at; }
     }
-    __syncthreads();
-    out.before = n_before;
-    out.upto = n_upto;
-    __syncthreads();
-    return out;
 }
 
 enum { TP_ALL = 0, TP_NEAR = 1, TP_SEARCH = 2 };      // what of a row is gathered: all that is kept, what is near the cut, nothing
-__device__ __forceinline__ int tp_how(const TpBracket &b) { return b.upto <= TP_GATHER ? TP_ALL : b.upto - b.before <= TP_GATHER ? TP_NEAR : TP_SEARCH; }
+__device__ __forceinline__ int tp_how(const TpRow &b) { return b.upto <= TP_GATHER ? TP_ALL : b.upto - b.before <= TP_GATHER ? TP_NEAR : TP_SEARCH; }
 
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_THREADS)
 tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
-                const TpPart *__restrict__ part, TpRow *__restrict__ rows, const unsigned int *__restrict__ hist, TpEntry *__restrict__ entries, float *__restrict__ out) {
+                const TpPart *__restrict__ part, TpRow *__restrict__ rows, TpEntry *__restrict__ entries, float *__restrict__ out) {
     const int r = blockIdx.x, parts = gridDim.y;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
     int lo, hi;
@@ -248,33 +304,47 @@ tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
     const float *row = logits + r * ld;
     if (!c.cuts) {
         const float inv = (float)(1.0 / c.sum);
-        if constexpr (WIDE) {
-            for (int i = lo + 4 * (int)threadIdx.x; i < hi; i += 4 * TP_THREADS) {
-                const float4 v = *(const float4 *)(row + i);
-                *(float4 *)(to + i) = make_float4(tp_weight(tp_distance(c, tp_clean(v.x))) * inv, tp_weight(tp_distance(c, tp_clean(v.y))) * inv,
-                                                  tp_weight(tp_distance(c, tp_clean(v.z))) * inv, tp_weight(tp_distance(c, tp_clean(v.w))) * inv);
-            }
-        } else {
-            tp_scan<WIDE>(row, lo, hi, [&](int i, float l) { to[i] = tp_weight(tp_distance(c, l)) * inv; });
-        }
+        tp_store_shares<WIDE>(row, lo, hi, to, [&](int, float l) { return tp_weight(tp_distance(c, l)) * inv; });
         return;
     }
-    const TpBracket b = tp_bracket<TP_THREADS>(c, hist + (size_t)r * TP_BINS);
+    const TpRow b = rows[r];
     const int how = tp_how(b);
     if (how == TP_SEARCH) return;
-    const int from = how == TP_ALL ? 0 : b.lo;
+    const int from = how == TP_ALL ? 0 : b.bin_lo;
     unsigned long long above = 0;
-    tp_scan<WIDE>(row, lo, hi, [&](int i, float l) {
+    // a workgroup's entries come together in LDS first: one place of them all in the row's list (an atomic addition a wave and four entries took 25 us of
+    // 31 parts' 39)
+    __shared__ TpEntry mine[TP_GATHER / 2];
+    __shared__ unsigned int mine_n, place;
+    if (threadIdx.x == 0) mine_n = 0;
+    __syncthreads();
+    auto flush = [&]() {
+        __syncthreads();
+        const unsigned int n = mine_n;
+        if (threadIdx.x == 0 && n) place = atomicAdd(&rows[r].gathered, n);
+        __syncthreads();
+        for (unsigned int i = threadIdx.x; i < n; i += TP_THREADS)
+            if (place + i < TP_GATHER) entries[(size_t)r * TP_GATHER + place + i] = mine[i];
+        __syncthreads();
+        if (threadIdx.x == 0) mine_n = 0;
+        __syncthreads();
+    };
+    auto entry = [&](int i, float l) {
         const float d = tp_distance(c, l);
         const int bin = d <= TP_NOTHING ? tp_bin(c, d) : TP_BINS;
-        if (how == TP_ALL) to[i] = 0.f;
-        if (bin >= from && bin <= b.hi) {
-            const unsigned int place = atomicAdd(&rows[r].gathered, 1u);
-            if (place < TP_GATHER) entries[(size_t)r * TP_GATHER + place] = {tp_key(l), i};
-        } else if (bin < from) {
-            above += tp_fixed(tp_weight(d));
-        }
-    });
+        if (bin >= from && bin <= b.bin_hi) mine[atomicAdd(&mine_n, 1u)] = {tp_key(l), i};
+        if (bin < from) above += tp_fixed(tp_weight(d));
+    };
+    // as much of the stretch at a time as fits whatever is kept of it
+    for (int at = lo; at < hi; at += TP_GATHER / 2) {
+        if (at > lo) flush();
+        const int end = min(hi, at + TP_GATHER / 2);
+        if (how == TP_ALL)
+            tp_store_shares<WIDE>(row, at, end, to, [&](int i, float l) { entry(i, l); return 0.f; });
+        else
+            tp_scan<WIDE>(row, at, end, entry);
+    }
+    flush();
     if (how == TP_NEAR) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) above += __shfl_xor(above, off, WAVE);
@@ -284,112 +354,212 @@ tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
 
 struct TpSum { unsigned long long mass; unsigned int count; };
 
-// Sums over the workgroup, for every thread.
-__device__ __forceinline__ TpSum tp_total(TpSum v, TpSum *scratch) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { v.mass += __shfl_xor(v.mass, off, WAVE); v.count += __shfl_xor(v.count, off, WAVE); }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-    TpSum t = {0, 0};
-    for (int w = 0; w < TP_CUT_THREADS / WAVE; ++w) { t.mass += scratch[w].mass; t.count += scratch[w].count; }
-    return t;
+// What an entry of key k at index i keeps.
+__device__ __forceinline__ float tp_share(const TpRow &t, unsigned int k, int i, float w) {
+    if (k < t.border || (k == t.border && i > t.last)) return 0.f;
+    if (k == t.border && i == t.last && t.kept >= 0.f) return t.kept;
+    return w * t.inv;
 }
 
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_CUT_THREADS)
 tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
-              const TpPart *__restrict__ part, int parts, const TpRow *__restrict__ rows, const unsigned int *__restrict__ hist, const TpEntry *__restrict__ entries,
-              float *__restrict__ out) {
-    __shared__ TpSum scratch[TP_CUT_THREADS / WAVE];
-    const int r = blockIdx.x;
+              const TpPart *__restrict__ part, int parts, TpRow *__restrict__ rows, const TpEntry *__restrict__ entries, float *__restrict__ out) {
+    __shared__ unsigned long long mass[256];
+    __shared__ unsigned int count[256];
+    __shared__ unsigned int found[2], key_lo, key_hi;
+    __shared__ TpSum found_above;
+    const int r = blockIdx.x, lane = threadIdx.x & 63;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
-    if (c.empty || c.greedy || !c.cuts) return;
-    const TpBracket b = tp_bracket<TP_CUT_THREADS>(c, hist + (size_t)r * TP_BINS);
+    if (c.empty || c.greedy || !c.cuts) {
+        if (threadIdx.x == 0) rows[r].store = 0;
+        return;
+    }
+    const TpRow b = rows[r];
     const int how = tp_how(b);
     const float *row = logits + r * ld;
     float *to = out + (size_t)r * vocab;
-    const unsigned int gathered = how == TP_SEARCH ? 0u : min(rows[r].gathered, (unsigned int)TP_GATHER);
+    const unsigned int gathered = how == TP_SEARCH ? 0u : min(b.gathered, (unsigned int)TP_GATHER);
     unsigned int key[TP_EACH];
     int at[TP_EACH];
-    unsigned long long fixed[TP_EACH];
 #pragma unroll
     for (int e = 0; e < TP_EACH; ++e) {
         const unsigned int i = e * TP_CUT_THREADS + threadIdx.x;
         const TpEntry t = i < gathered ? entries[(size_t)r * TP_GATHER + i] : TpEntry{0u, 0x7fffffff};
         key[e] = t.key;
         at[e] = t.at;
-        fixed[e] = i < gathered ? tp_fixed(tp_weight(tp_distance(c, tp_logit(t.key)))) : 0;
     }
-    // entries whose place in the order (key, then the lower index) satisfies `in`: their weights and number
-    auto sum_of = [&](auto in) {
-        TpSum t = {0, 0};
+    // the digits are those of the distance from the smallest key: the keys' own first digit is the exponent, which nearly all share, and their additions
+    // would wait for each other
+    if (threadIdx.x == 0) { key_lo = 0xffffffffu; key_hi = 0; }
+    __syncthreads();
+    unsigned int lowest = 0xffffffffu, highest = 0;
+#pragma unroll
+    for (int e = 0; e < TP_EACH; ++e)
+        if (e * TP_CUT_THREADS + threadIdx.x < gathered) { lowest = min(lowest, key[e]); highest = max(highest, key[e]); }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) { lowest = min(lowest, (unsigned int)__shfl_xor(lowest, off, WAVE)); highest = max(highest, (unsigned int)__shfl_xor(highest, off, WAVE)); }
+    if (lane == 0 && highest) { atomicMin(&key_lo, lowest); atomicMax(&key_hi, highest); }
+    __syncthreads();
+    const unsigned int base = how == TP_SEARCH || gathered == 0 ? 0u : key_lo, span = how == TP_SEARCH || gathered == 0 ? ~0u : key_hi - key_lo;
+    // f(key, index, weight) of every entry that is looked at
+    auto each = [&](auto f) {
         if (how == TP_SEARCH) {
             tp_scan<WIDE>(row, 0, vocab, [&](int i, float l) {
                 const float d = tp_distance(c, l);
-                if (d <= TP_NOTHING && in(tp_key(l), i)) { t.mass += tp_fixed(tp_weight(d)); ++t.count; }
+                if (d <= TP_NOTHING) f(tp_key(l), i, tp_weight(d));
             });
         } else {
 #pragma unroll
             for (int e = 0; e < TP_EACH; ++e)
-                if (e * TP_CUT_THREADS + threadIdx.x < gathered && in(key[e], at[e])) { t.mass += fixed[e]; ++t.count; }
+                if (e * TP_CUT_THREADS + threadIdx.x < gathered) f(key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
         }
-        t = tp_total(t, scratch);
-        if (how == TP_NEAR) { t.mass += rows[r].mass_above; t.count += b.before; }
-        return t;
     };
     const unsigned long long limit_p = c.limit_p < 524288.0 ? (unsigned long long)(c.limit_p * TP_ONE) : ~0ull;
-    auto reached = [&](const TpSum &t) { return t.count >= (unsigned int)c.k || t.mass >= limit_p; };
-    // the largest key at which the entries down to it reach one of the limits
-    unsigned int border = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned int t = border | 1u << bit;
-        if (reached(sum_of([&](unsigned int k, int) { return k >= t; }))) border = t;
-    }
-    const TpSum above = sum_of([&](unsigned int k, int) { return k > border; }), with = sum_of([&](unsigned int k, int) { return k >= border; });
-    const bool all = !reached(with);                   // (the limit lies a rounding beyond all there is)
-    const unsigned long long each = with.count > above.count ? (with.mass - above.mass) / (with.count - above.count) : 0;
-    unsigned long long limit = with.mass;
-    int last = 0x7fffffff;                             // the index of the last of the equal entries that keeps anything
-    unsigned long long kept = each;                    // and what it keeps
-    if (!all) {
-        limit = limit_p;
-        if (with.count >= (unsigned int)c.k) limit = min(limit, above.mass + ((unsigned int)c.k - above.count) * each);
-        unsigned int rank = each ? (unsigned int)((limit - above.mass + each - 1) / each) : (unsigned int)c.k - above.count;
-        rank = max(1u, min(rank, with.count - above.count));
-        kept = limit - above.mass - (unsigned long long)(rank - 1) * each;
-        if (with.count - above.count > 1) {
-            // the rank-th smallest index among them
-            unsigned int index = 0;
-            for (int bit = 30; bit >= 0; --bit) {
-                const unsigned int t = index | 1u << bit;
-                if (t >= (unsigned int)vocab) continue;
-                TpSum below = sum_of([&](unsigned int k, int i) { return k == border && (unsigned int)i < t; });
-                if (how == TP_NEAR) below.count -= b.before;
-                if (below.count < rank) index = t;
+    // the digits of the largest key at which the entries down to it reach one of the limits; `above`: what lies over the keys with the digits so far
+    TpSum above = how == TP_NEAR ? TpSum{b.mass_above, b.before} : TpSum{0, 0};
+    unsigned int border = 0;                           // (less the smallest key)
+    bool all = false;                                  // (the limits lie a rounding beyond all there is)
+    int open = span ? 32 - __clz(span) : 1;            // bits that are not decided yet
+    while (open > 0) {
+        const int shift = max(0, open - 8);
+        __syncthreads();
+        if (threadIdx.x < 256) { mass[threadIdx.x] = 0; count[threadIdx.x] = 0; }
+        __syncthreads();
+        each([&](unsigned int k, int, float w) {
+            const unsigned int digit = ((k - base) >> shift) - (border >> shift);       // (border's undecided bits are zeros)
+            if (digit < 256u && k - base >= border) {
+                atomicAdd(&count[digit], 1u);
+                atomicAdd(&mass[digit], tp_fixed(w));
             }
-            last = (int)index;
-        } else {
-            last = -1;                                  // (a single one: its own index)
+        });
+        __syncthreads();
+        if (threadIdx.x < WAVE) {                      // a wave walks the digits from the largest on, four a lane
+            TpSum mine = {0, 0}, digit[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 255 - (4 * lane + e);
+                digit[e] = {mass[d], count[d]};
+                mine.mass += digit[e].mass; mine.count += digit[e].count;
+            }
+            TpSum scan = mine;
+#pragma unroll
+            for (int off = 1; off < WAVE; off <<= 1) {
+                const unsigned long long m = __shfl_up(scan.mass, off, WAVE);
+                const unsigned int n = __shfl_up(scan.count, off, WAVE);
+                if (lane >= off) { scan.mass += m; scan.count += n; }
+            }
+            TpSum so_far = {above.mass + scan.mass - mine.mass, above.count + scan.count - mine.count};
+            int got = -1;
+            TpSum got_above = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const TpSum with = {so_far.mass + digit[e].mass, so_far.count + digit[e].count};
+                if (got < 0 && digit[e].count && (with.count >= (unsigned int)c.k || with.mass >= limit_p)) { got = 255 - (4 * lane + e); got_above = so_far; }
+                so_far = with;
+            }
+            const unsigned long long reached = __ballot(got >= 0);
+            if (reached == 0) {
+                if (lane == WAVE - 1) { found[0] = 256; found_above = so_far; }
+            } else if (lane == __ffsll((unsigned long long)reached) - 1) {
+                found[0] = (unsigned int)got;
+                found_above = got_above;
+            }
+        }
+        __syncthreads();
+        above = found_above;
+        if (found[0] == 256u) { all = true; break; }
+        border |= found[0] << shift;
+        open = shift;
+    }
+    TpRow t = {};
+    t.last = 0x7fffffff;
+    t.kept = -1.f;                                     // (what is kept whole has its weight's own digits, not those of the sums)
+    unsigned long long limit = above.mass;
+    if (!all) {
+        const unsigned int equal = count[found[0]];                        // of the last digit: all have the key
+        border += base;
+        const unsigned long long each_mass = tp_fixed(tp_weight(tp_distance(c, tp_logit(border))));
+        limit = limit_p;
+        if (above.count + equal >= (unsigned int)c.k) limit = min(limit, above.mass + ((unsigned int)c.k - above.count) * each_mass);
+        unsigned int rank = each_mass ? (unsigned int)min((limit - above.mass + each_mass - 1) / each_mass, (unsigned long long)equal) : min((unsigned int)c.k - above.count, equal);
+        rank = max(1u, rank);
+        const unsigned long long kept = limit - above.mass - (unsigned long long)(rank - 1) * each_mass;
+        if (kept < each_mass) t.kept = (float)((double)kept / (double)limit);
+        t.border = border;
+        // the rank-th smallest index among the equal ones, eight bits at a time
+        unsigned int index = 0;
+        if (equal > 1) {
+            unsigned int left = rank;
+            for (int shift = 16; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (threadIdx.x < 256) count[threadIdx.x] = 0;
+                __syncthreads();
+                each([&](unsigned int k, int i, float) {
+                    if (k == border && (shift == 16 || ((unsigned int)i ^ index) >> (shift + 8) == 0)) atomicAdd(&count[(unsigned int)i >> shift & 255], 1u);
+                });
+                __syncthreads();
+                if (threadIdx.x < WAVE) {
+                    unsigned int mine = 0, n[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { n[e] = count[4 * lane + e]; mine += n[e]; }
+                    unsigned int scan = mine;
+#pragma unroll
+                    for (int off = 1; off < WAVE; off <<= 1) {
+                        const unsigned int up = __shfl_up(scan, off, WAVE);
+                        if (lane >= off) scan += up;
+                    }
+                    unsigned int so_far = scan - mine;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (so_far < left && left <= so_far + n[e]) { found[0] = 4 * lane + e; found[1] = so_far; }
+                        so_far += n[e];
+                    }
+                }
+                __syncthreads();
+                index |= found[0] << shift;
+                left -= found[1];
+            }
+            t.last = (int)index;
+        }
+        // (a single one: whatever its index, it is the last)
+        if (equal == 1) {
+            __syncthreads();
+            each([&](unsigned int k, int i, float) { if (k == border) found[0] = (unsigned int)i; });
+            __syncthreads();
+            t.last = (int)found[0];
         }
     }
-    const double inv = limit ? TP_ONE / (double)limit : 0.0;
-    const bool part_of_it = kept < each;               // (what is kept whole has its weight's own digits, not those of the sums)
-    auto share = [&](unsigned int k, int i, float w) {
-        if (!all && (k < border || (k == border && last >= 0 && i > last))) return 0.f;
-        if (!all && part_of_it && k == border && (last < 0 || i == last)) return (float)((double)kept / (double)limit);
-        return (float)((double)w * inv);
-    };
+    t.inv = limit ? (float)(TP_ONE / (double)limit) : 0.f;
+    t.store = how != TP_ALL;
     if (how == TP_ALL) {
 #pragma unroll
         for (int e = 0; e < TP_EACH; ++e)
-            if (e * TP_CUT_THREADS + threadIdx.x < gathered) to[at[e]] = share(key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
-    } else {
-        tp_scan<WIDE>(row, 0, vocab, [&](int i, float l) {
-            const float d = tp_distance(c, l);
-            to[i] = d <= TP_NOTHING ? share(tp_key(l), i, tp_weight(d)) : 0.f;
-        });
+            if (e * TP_CUT_THREADS + threadIdx.x < gathered) to[at[e]] = tp_share(t, key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
     }
+    if (threadIdx.x == 0) {
+        rows[r].border = t.border; rows[r].last = t.last; rows[r].store = t.store;
+        rows[r].kept = t.kept; rows[r].inv = t.inv;
+    }
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(TP_THREADS)
+tp_store_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
+                const TpPart *__restrict__ part, const TpRow *__restrict__ rows, float *__restrict__ out) {
+    const int r = blockIdx.x, parts = gridDim.y;
+    const TpRow t = rows[r];
+    if (!t.store) return;
+    const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
+    int lo, hi;
+    tp_stretch(vocab, blockIdx.y, parts, lo, hi);
+    const float *row = logits + r * ld;
+    float *to = out + (size_t)r * vocab;
+    auto share = [&](int i, float l) {
+        const float d = tp_distance(c, l);
+        return d <= TP_NOTHING ? tp_share(t, tp_key(l), i, tp_weight(d)) : 0.f;
+    };
+    tp_store_shares<WIDE>(row, lo, hi, to, share);
 }
 
 // Bytes of scratch memory that lcu_token_probs needs, in whatever state they are (cuts: some row may have a cut).
@@ -420,11 +590,15 @@ LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int voc
         if (cuts) {                                                                                                                                 \
             tp_count_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, hist);                      \
             LCU_LAUNCH_CHECK();                                                                                                                     \
+            tp_bracket_kernel<<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(vocab, temperature, top_p, top_k, part, parts, state, hist);          \
+            LCU_LAUNCH_CHECK();                                                                                                                     \
         }                                                                                                                                           \
-        tp_write_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, hist, entries, out);     \
+        tp_write_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, entries, out);           \
         LCU_LAUNCH_CHECK();                                                                                                                         \
         if (cuts) {                                                                                                                                 \
-            tp_cut_kernel<WIDE><<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, parts, state, hist, entries, out); \
+            tp_cut_kernel<WIDE><<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, parts, state, entries, out); \
+            LCU_LAUNCH_CHECK();                                                                                                                     \
+            tp_store_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, out);               \
             LCU_LAUNCH_CHECK();                                                                                                                     \
         }                                                                                                                                           \
     } while (0)

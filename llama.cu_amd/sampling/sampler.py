@@ -196,8 +196,8 @@ def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tenso
     tokens = torch.empty((requests, int(max_drafts) + 1), dtype=torch.int32, device=dev)
     if requests == 0:
         return accepted, tokens
-    # the row at which a run ends is cut into parts of 2,048 tokens at least, up to about four workgroups a compute unit in all
-    parts = max(1, min(64, 4 * ops.TUNING.compute_units // requests, vocab // 2048))
+    # the row at which a run ends is cut into parts of 2,048 tokens, one workgroup each: what a workgroup of the second launch takes at once
+    parts = min(64, -(-vocab // 2048))
     sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev)
     lib = build.load("verify")
     _check(lib.lcu_verify_drafts(_ptr(probs), ctypes.c_longlong(probs.stride(0)), rows, _ptr(starts), requests, _ptr(drafts), n, _ptr(draft_probs),
