@@ -121,6 +121,8 @@ struct MtArgs {
     long long ldy;
     int M, N, steps, w_steps;       // steps of X; of W, which begins anew where it ends
     int wide_out;
+    int each;                       // steps of a slice of K; slice i's sums go to the i-th plane of y
+    long long plane;
 };
 
 template <class S, int EPI>
@@ -132,6 +134,7 @@ mx4_tiles_kernel(MtArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
     const int wf = wave % S::WF, wt = wave / S::WF;
     // ---- which tile: workgroups go to the eight dies in turn; a die takes a run of tiles, those of a few feature tiles side by side
+    const int first = blockIdx.y * a.each, steps = min(a.steps - first, a.each);
     const int t_tiles = (a.M + S::T - 1) / S::T, f_tiles = (a.N + S::F - 1) / S::F, tiles = t_tiles * f_tiles;
     const int each = (tiles + 7) / 8, item = blockIdx.x % 8 * each + blockIdx.x / 8;
     if ((int)blockIdx.x / 8 >= each || item >= tiles) return;
@@ -165,7 +168,7 @@ mx4_tiles_kernel(MtArgs a) {
     };
     auto issue_t = [&](mx4_u32x4 *dst, int step, int i) {
         auto *to = (__attribute__((address_space(3))) void *)(dst + (i * S::WAVES + wave) * WAVE);
-        const uint32_t from = from_t[i] + (uint32_t)min(step, a.steps - 1) * 128u;
+        const uint32_t from = from_t[i] + (uint32_t)(first + min(step, steps - 1)) * 128u;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, to, 16, from, 0, 0, 0);
     };
     // ---- where the lane's operands stand in a stage
@@ -233,10 +236,11 @@ mx4_tiles_kernel(MtArgs a) {
         before.t[FOUR ? t : 0][0] = before.t[FOUR ? t : 0][1] = 0;
     }
     // W's step of the features' ring: one that goes round
-    int wf_step = 0;
+    int wf_step = first % a.w_steps;
     auto next_w = [&](int s) { return s + 1 == a.w_steps ? 0 : s + 1; };
     // what SF - 1 turns before the first would have asked for
-    fetch_scales(next, 0, 0);
+    int s_step = wf_step;
+    fetch_scales(next, first, s_step);
 #pragma unroll
     for (int j = 1 - S::SF; j < 0; ++j) {
         if (j + S::ST - 1 >= 0) {
@@ -247,11 +251,11 @@ mx4_tiles_kernel(MtArgs a) {
         for (int i = 0; i < S::LF; ++i) issue_f(lds_f + (j + S::SF - 1) * S::F * S::FP, wf_step, i);
         wf_step = next_w(wf_step);
     }
-    int rf = 0, rt = 0, df = S::SF - 1, dt = S::ST - 1, s_step = 0;
-    for (int t = 0; t < a.steps; ++t) {
+    int rf = 0, rt = 0, df = S::SF - 1, dt = S::ST - 1;
+    for (int t = 0; t < steps; ++t) {
         now = moved(next);
         s_step = next_w(s_step);
-        fetch_scales(next, min(t + 1, a.steps - 1), s_step);
+        fetch_scales(next, first + min(t + 1, steps - 1), s_step);
         mt_wait_loads<S::LEFT>();                              // this step's stages are there
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         mt_turn<S>(lds_f + rf * S::F * S::FP + of_f, lds_t + rt * S::T * S::TP + of_t, lds_f + df * S::F * S::FP, lds_t + dt * S::T * S::TP,
@@ -275,7 +279,7 @@ mx4_tiles_kernel(MtArgs a) {
     // ---- out: a wave turns 32 tokens at a time through LDS of its own, and stores whole rows of its features
     constexpr int OUT_F = SWIGLU ? 16 * FT : 32 * FT, ELEM = OUT32 ? 4 : 2, PITCH = OUT_F * ELEM + 16, CH = OUT_F * ELEM / 16;
     static_assert(S::WAVES * 32 * PITCH <= S::LDS * 16, "room for the waves' rows");
-    char *mine = (char *)mt_lds + wave * 32 * PITCH;
+    char *mine = (char *)mt_lds + wave * 32 * PITCH, *const y = (char *)a.y + (size_t)blockIdx.y * a.plane * ELEM;
     const int out_n = SWIGLU ? half_n : a.N, f0 = (SWIGLU ? ft0 * (S::F / 2) : ft0 * S::F) + wf * OUT_F;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -297,22 +301,68 @@ mx4_tiles_kernel(MtArgs a) {
             for (int x = 0; x < 32 * CH / WAVE; ++x) {
                 const int i = x * WAVE + lane, row = i / CH, c = i % CH, col = f0 + c * (16 / ELEM);
                 const mx4_u32x4 v = *(const mx4_u32x4 *)(mine + row * PITCH + c * 16);
-                if (tok0 + row < a.M && col < out_n) *(mx4_u32x4 *)((char *)a.y + ((size_t)(tok0 + row) * a.ldy + col) * ELEM) = v;
+                if (tok0 + row < a.M && col < out_n) *(mx4_u32x4 *)(y + ((size_t)(tok0 + row) * a.ldy + col) * ELEM) = v;
             }
         } else {
             for (int i = lane; i < 32 * OUT_F; i += WAVE) {
                 const int row = i / OUT_F, col = f0 + i % OUT_F;
                 if (tok0 + row >= a.M || col >= out_n) continue;
-                if constexpr (OUT32) ((float *)a.y)[(size_t)(tok0 + row) * a.ldy + col] = *(const float *)(mine + row * PITCH + i % OUT_F * 4);
-                else ((uint16_t *)a.y)[(size_t)(tok0 + row) * a.ldy + col] = *(const uint16_t *)(mine + row * PITCH + i % OUT_F * 2);
+                if constexpr (OUT32) ((float *)y)[(size_t)(tok0 + row) * a.ldy + col] = *(const float *)(mine + row * PITCH + i % OUT_F * 4);
+                else ((uint16_t *)y)[(size_t)(tok0 + row) * a.ldy + col] = *(const uint16_t *)(mine + row * PITCH + i % OUT_F * 2);
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
+// The planes of the slices' sums, added up, and the epilogue: four columns a thread.
+template <int EPI>
+__global__ void __launch_bounds__(256)
+mx4_join_kernel(const float *__restrict__ planes, int slices, long long plane, int N, int M, void *__restrict__ y, long long ldy, int wide_out) {
+    constexpr bool SWIGLU = EPI >= MT_EPI_SWIGLU, OUT32 = EPI == MT_EPI_F32 || EPI == MT_EPI_SWIGLU_F32;
+    const int cols = SWIGLU ? N / 2 : N, fours = (cols + 3) / 4;
+    const long long at = blockIdx.x * 256ll + threadIdx.x;
+    if (at >= (long long)M * fours) return;
+    const int row = (int)(at / fours), col = (int)(at - (long long)row * fours) * 4, n = min(4, cols - col);
+    auto sum = [&](int c, float (&v)[4]) {
+        const float *from = planes + (size_t)row * N + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = 0.f;
+        if (N % 4 == 0 && c % 4 == 0) {
+#pragma unroll 4
+            for (int s = 0; s < slices; ++s) {
+                const mx4_f32x4 p = *(const mx4_f32x4 *)(from + s * plane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += p[e];
+            }
+        } else {
+            for (int s = 0; s < slices; ++s)
+                for (int e = 0; e < n; ++e) v[e] += from[s * plane + e];
+        }
+    };
+    float v[4];
+    sum(col, v);
+    if constexpr (SWIGLU) {
+        float up[4];
+        sum(col + cols, up);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = gate_up<GATE_SILU>(v[e], up[e], 0.f, 0.f);
+    }
+    if constexpr (OUT32) {
+        float *to = (float *)y + row * ldy + col;
+        if (wide_out) *(mx4_f32x4 *)to = mx4_f32x4{v[0], v[1], v[2], v[3]};
+        else
+            for (int e = 0; e < n; ++e) to[e] = v[e];
+    } else {
+        bf16_t *to = (bf16_t *)y + row * ldy + col;
+        if (wide_out) *(uint2 *)to = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+        else
+            for (int e = 0; e < n; ++e) to[e] = from_f32<bf16_t>(v[e]);
+    }
+}
+
 template <class S, int EPI>
-static int mt_go(const MtArgs &a, hipStream_t stream) {
+static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
     const int tiles = ((a.M + S::T - 1) / S::T) * ((a.N + S::F - 1) / S::F);
     constexpr int bytes = S::LDS * 16;
     static bool asked = false;
@@ -321,15 +371,16 @@ static int mt_go(const MtArgs &a, hipStream_t stream) {
         if (e != hipSuccess) return (int)e;
         asked = true;
     }
-    mx4_tiles_kernel<S, EPI><<<dim3((tiles + 7) / 8 * 8), dim3(S::THREADS), bytes, stream>>>(a);
+    mx4_tiles_kernel<S, EPI><<<dim3((tiles + 7) / 8 * 8, slices), dim3(S::THREADS), bytes, stream>>>(a);
     LCU_LAUNCH_CHECK();
     return LCU_OK;
 }
 
 // Arguments as lcu_mx4_stream's; rows in 4 bits and their scales in whole pairs of macro-steps (256 k), bfloat16 rows in multiples of 64 k.  shape: 0: tiles of 128 x 128
-// (features x tokens), 1: 256 x 256.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
+// (features x tokens), 1: 256 x 256, 2: 128 x 64.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats,
+// 16-byte aligned.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
 LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *xs, long long lds, const void *codes, const void *scales, int pairs, void *y, long long ldy,
-                          int M, int N, int K, int epi, int shape, hipStream_t stream) {
+                          int M, int N, int K, int epi, int shape, int slices, void *planes, hipStream_t stream) {
     if (M <= 0 || N <= 0) return LCU_OK;
     const int macros = (K + 127) / 128, cols = epi >= MT_EPI_SWIGLU ? N / 2 : N, elem = epi == MT_EPI_F32 || epi == MT_EPI_SWIGLU_F32 ? 4 : 2;
     const long long w_rows = (N + 15) / 16 * 16, row_bytes = x_kind == 4 ? ldx : ldx * 2, limit = 1ll << 32;
@@ -352,22 +403,44 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     if (x_kind == 3 && a.w_steps > pairs * 4) return LCU_BAD_ARGUMENT;
     a.x_bytes = (uint32_t)((M - 1) * row_bytes + (long long)a.steps * 128);
     a.xs_bytes = x_kind == 4 ? (uint32_t)((M - 1) * lds + two * 8ll) : 0u;
-    a.wide_out = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % 16 == 0;
-#define EPIS(...)                                                            \
-    do {                                                                     \
-        typedef MtShape<__VA_ARGS__> S;                                       \
-        if (epi == MT_EPI_BF16) return mt_go<S, MT_EPI_BF16>(a, stream);      \
-        if (epi == MT_EPI_F32) return mt_go<S, MT_EPI_F32>(a, stream);        \
-        if (epi == MT_EPI_SWIGLU) return mt_go<S, MT_EPI_SWIGLU>(a, stream);  \
-        return mt_go<S, MT_EPI_SWIGLU_F32>(a, stream);                        \
+    if (slices < 1 || slices > a.steps || (slices > 1 && (!planes || (uintptr_t)planes % 16))) return LCU_BAD_ARGUMENT;
+    a.each = (a.steps + slices - 1) / slices;
+    slices = (a.steps + a.each - 1) / a.each;                  // (as many as hold a step)
+    const bool wide = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % 16 == 0;
+    a.wide_out = wide;
+    if (slices > 1) {
+        a.y = planes; a.ldy = N; a.plane = (long long)M * N;
+        a.wide_out = N % 4 == 0;
+    }
+#define EPIS(...)                                                                    \
+    do {                                                                             \
+        typedef MtShape<__VA_ARGS__> S;                                               \
+        if (slices > 1 || epi == MT_EPI_F32) rc = mt_go<S, MT_EPI_F32>(a, slices, stream); \
+        else if (epi == MT_EPI_BF16) rc = mt_go<S, MT_EPI_BF16>(a, 1, stream);        \
+        else if (epi == MT_EPI_SWIGLU) rc = mt_go<S, MT_EPI_SWIGLU>(a, 1, stream);    \
+        else rc = mt_go<S, MT_EPI_SWIGLU_F32>(a, 1, stream);                          \
     } while (0)
+    int rc = LCU_BAD_ARGUMENT;
     if (x_kind == 4) {
         if (shape == 0) EPIS(true, 2, 2, 2, 2, 4, 4);
-        if (shape == 1) EPIS(true, 4, 2, 2, 4, 3, 2);
+        else if (shape == 1) EPIS(true, 4, 2, 2, 4, 3, 2);
+        else if (shape == 2) EPIS(true, 2, 1, 2, 2, 6, 6);
     } else {
         if (shape == 0) EPIS(false, 2, 2, 2, 2, 6, 6);
-        if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
+        else if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
+        else if (shape == 2) EPIS(false, 2, 1, 2, 2, 8, 8);
     }
 #undef EPIS
-    return LCU_BAD_ARGUMENT;
+    if (rc != LCU_OK || slices == 1) return rc;
+    const long long threads = (long long)M * ((cols + 3) / 4);
+    const int out_wide = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % (4 * elem) == 0;
+    const dim3 grid((unsigned int)((threads + 255) / 256)), block(256);
+#define JOIN(EPI) mx4_join_kernel<EPI><<<grid, block, 0, stream>>>((const float *)planes, slices, a.plane, N, M, y, ldy, out_wide)
+    if (epi == MT_EPI_BF16) JOIN(MT_EPI_BF16);
+    else if (epi == MT_EPI_F32) JOIN(MT_EPI_F32);
+    else if (epi == MT_EPI_SWIGLU) JOIN(MT_EPI_SWIGLU);
+    else JOIN(MT_EPI_SWIGLU_F32);
+#undef JOIN
+    LCU_LAUNCH_CHECK();
+    return LCU_OK;
 }

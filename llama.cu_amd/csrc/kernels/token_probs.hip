@@ -54,6 +54,8 @@ struct TpCut {
     int k, at;
     bool empty, greedy, cuts;
 };
+// (not below 1e-38: an infinite distance times 0 would be none)
+__device__ __forceinline__ float tp_inv_t(float temperature) { return fmaxf(TP_LOG2E / temperature, 1e-38f); }
 // (the maximum with 0 makes 0 of what is no number: an infinite logit's distance from itself, and 0 times an infinite 1 / T)
 __device__ __forceinline__ float tp_apart(float most, float l, float inv_t) { return fmaxf((most - l) * inv_t, 0.f); }
 __device__ __forceinline__ float tp_distance(const TpCut &c, float l) { return tp_apart(c.most, l, c.inv_t); }
@@ -76,7 +78,7 @@ __device__ __forceinline__ TpCut tp_row(const TpPart *__restrict__ part, int par
     float least = mine.least;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) { c.most = fmaxf(c.most, __shfl_xor(c.most, off, WAVE)); least = fminf(least, __shfl_xor(least, off, WAVE)); }
-    c.inv_t = TP_LOG2E / temperature;
+    c.inv_t = tp_inv_t(temperature);
     c.at = mine.most == c.most ? mine.at : 0x7fffffff;
     c.sum = lane < parts && mine.most > -INFINITY ? mine.sum * (double)tp_weight(tp_distance(c, mine.most)) : 0.0;
 #pragma unroll
@@ -148,7 +150,7 @@ tp_max_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
         for (int b = (int)blockIdx.y * TP_THREADS + threadIdx.x; b < TP_BINS; b += TP_THREADS * parts) hist[(size_t)r * TP_BINS + b] = 0u;
         if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].mass_above = 0; rows[r].gathered = 0; }
     }
-    const float inv_t = TP_LOG2E / temperature[r];
+    const float inv_t = tp_inv_t(temperature[r]);
     float most = -INFINITY, least = INFINITY;
     double sum = 0.0;
     int at = 0x7fffffff;

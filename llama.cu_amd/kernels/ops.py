@@ -63,8 +63,29 @@ def _gpu(*tensors: Optional[torch.Tensor]) -> None:
 
 def on_current_device(device: torch.device, what: str) -> None:
     """Kernels go to the current device's stream: operands on another one are refused."""
-    if device.index is not None and device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: the operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    current = torch._C._cuda_getDevice()
+    if device.index is not None and device.index != current:
+        raise KernelError(f"{what}: the operands are on {device}, the current device is cuda:{current}")
+
+
+_LETTERS = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int}
+_bound: Dict = {}
+
+
+def bind(library: str, name: str, arguments: str):
+    """The entry point ``name`` of a library, with the types of its arguments said once (a letter each: pointer, long long, int) and the current stream
+    as its last one: plain numbers then go straight into the call (``None`` is a null pointer), which a small kernel's call is mostly made of."""
+    f = _bound.get(name)
+    if f is None:
+        f = getattr(build.load(library), name)
+        f.argtypes = [_LETTERS[a] for a in arguments] + [ctypes.c_void_p]
+        _bound[name] = f
+    return f
+
+
+def raw_stream() -> int:
+    """The stream that kernels are launched on, as a number."""
+    return _scoped_stream.value or 0 if _scoped_stream is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _rows(t: torch.Tensor, what: str) -> None:
@@ -2760,8 +2781,9 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     codes = torch.empty((m, filled // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((m, filled // MX4_BLOCK), dtype=torch.uint8, device=x.device)
     if m and k:
-        _check(build.load("mx4").lcu_mx4_quantize(_ptr(x), ctypes.c_longlong(x.stride(0)), _type(x, "mx4_quantize"), ctypes.c_longlong(m), k, _ptr(codes), _ptr(scales), _stream()),
-               "mx4_quantize")
+        _check(bind("mx4", "lcu_mx4_quantize", "plilipp")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], m, k, codes.data_ptr(), scales.data_ptr(), raw_stream()), "mx4_quantize")
+    if filled == k:
+        return Mx4(codes, scales, k, True)
     return Mx4(codes[:, :16 * blocks], scales[:, :blocks], k, True)
 
 
@@ -2773,8 +2795,8 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     _mx4_here("mx4_values", q.codes, q.scales)
     out = torch.empty((m, q.k), dtype=out_dtype, device=q.codes.device)
     if m and q.k:
-        _check(build.load("mx4").lcu_mx4_values(_ptr(q.codes), ctypes.c_longlong(q.codes.stride(0)), _ptr(q.scales), ctypes.c_longlong(q.scales.stride(0)), ctypes.c_longlong(m),
-                                                q.k, _ptr(out), ctypes.c_longlong(q.k), _type(out, "mx4_values"), _stream()), "mx4_values")
+        _check(bind("mx4", "lcu_mx4_values", "plpllipli")(q.codes.data_ptr(), q.codes.stride(0), q.scales.data_ptr(), q.scales.stride(0), m, q.k, out.data_ptr(), q.k,
+                                                          _TYPE[out_dtype], raw_stream()), "mx4_values")
     return out
 
 
@@ -2820,7 +2842,7 @@ def _mx4_rows(x: torch.Tensor, k: int) -> Tuple[torch.Tensor, int]:
     x = _mx4_source(x, "gemm_mx4")
     planes = 3 if x.dtype == torch.float32 else 1
     out = torch.empty((x.shape[0], planes * (-(-k // _MX4_PAIR) * _MX4_PAIR)), dtype=torch.bfloat16, device=x.device)
-    _check(build.load("mx4").lcu_mx4_rows(_ptr(x), ctypes.c_longlong(x.stride(0)), _type(x, "gemm_mx4"), ctypes.c_longlong(x.shape[0]), k, _ptr(out), _stream()), "gemm_mx4 rows")
+    _check(bind("mx4", "lcu_mx4_rows", "plilip")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], x.shape[0], k, out.data_ptr(), raw_stream()), "gemm_mx4 rows")
     return out, planes
 
 
@@ -2838,12 +2860,14 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     return Mx4(codes[:, :16 * blocks], scales[:, :blocks], q.k, True)
 
 
-def mx4_choice(m: int, n: int, k: int, kind: int, swiglu: bool) -> int:
-    """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: -1 the one that streams the weight, else the shape of the
-    tiles (mx4_tiles.hip)."""
+def mx4_choice(m: int, n: int, k: int, kind: int, swiglu: bool) -> Tuple[int, int]:
+    """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: ``(-1, 1)`` the one that streams the weight, else the shape of
+    the tiles and into how many slices K is cut (mx4_tiles.hip)."""
+    if m <= 16:
+        return -1, 1
     if m <= 64:
-        return -1
-    return 1 if m > 128 and (m + 255) // 256 * ((n + 255) // 256) * 2 > TUNING.compute_units else 0
+        return 2, 8
+    return (1 if m > 128 and (m + 255) // 256 * ((n + 255) // 256) * 2 > TUNING.compute_units else 0), 1
 
 
 def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, swiglu: bool = False) -> torch.Tensor:
@@ -2885,20 +2909,23 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         ld, scales, lds = rows.stride(0), None, 0
     if m == 1:                             # (the one row's stride says nothing)
         ld, lds = (128 * w.pairs, 8 * w.pairs) if four else (rows.shape[1], 0)
-    shape = mx4_choice(m, w.n, k, kind, swiglu)
+    shape, slices = mx4_choice(m, w.n, k, kind, swiglu)
     row_bytes = ld if four else 2 * ld
     most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
     if shape >= 0 and (most < 512 or (w.n + 528) * w.pairs * 128 >= 1 << 32):
         shape = -1
-    head = (w.pairs, _ptr(out), ctypes.c_longlong(out.stride(0) if m > 1 else cols))
-    tail = (w.n, k, (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0))
+    of_out = out.stride(0) if m > 1 else cols
+    epilogue = (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0)
+    xs = scales.data_ptr() if four else None
+    weight = (w.codes.data_ptr(), w.scales.data_ptr(), w.pairs)
     if shape < 0:
-        _check(build.load("mx4_stream").lcu_mx4_stream(_ptr(rows), ctypes.c_longlong(ld), kind, _ptr(scales), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), *head, m, *tail,
-                                                       _stream()), "gemm_mx4")
+        _check(bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")(rows.data_ptr(), ld, kind, xs, lds, *weight, out.data_ptr(), of_out, m, w.n, k, epilogue, raw_stream()), "gemm_mx4")
         return out
-    lib = build.load("mx4_tiles")
+    steps = w.pairs if four else (-(-k // 128) * 2 if kind == 1 else 12 * w.pairs)
+    slices = max(1, min(slices, steps))
+    planes = torch.empty(slices * min(m, most) * w.n, dtype=torch.float32, device=device) if slices > 1 else None
+    f = bind("mx4_tiles", "lcu_mx4_tiles", "pliplppipliiiiiip")
     for r in range(0, m, most):
-        part, sc, to = (rows, scales, out) if m <= most else (rows[r:r + most], None if scales is None else scales[r:r + most], out[r:r + most])
-        _check(lib.lcu_mx4_tiles(_ptr(part), ctypes.c_longlong(ld), kind, _ptr(sc), ctypes.c_longlong(lds), _ptr(w.codes), _ptr(w.scales), w.pairs, _ptr(to), head[2],
-                                 min(most, m - r), *tail, shape, _stream()), "gemm_mx4")
+        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + r * lds if four else None, lds, *weight, out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r),
+                 w.n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), raw_stream()), "gemm_mx4")
     return out

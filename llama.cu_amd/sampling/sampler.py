@@ -6,6 +6,7 @@ depend on what else is in the batch or on how its prompt was cut.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 from typing import List, Optional, Sequence, Tuple, Union
 
@@ -102,7 +103,8 @@ def _options(values, dtype: torch.dtype, rows: int, device, what: str, fine, why
             raise KernelError(f"token_probs: {what} on the device must be contiguous {dtype} [{rows}], got {values.dtype} {tuple(values.shape)}")
         return values
     values = values.tolist() if isinstance(values, torch.Tensor) else list(values)
-    if len(values) != rows or not all(fine(v) for v in values):
+    # (the least, the largest and the sum, in which a NaN shows)
+    if len(values) != rows or (rows and not fine(min(values), max(values), sum(values))):
         raise KernelError(f"token_probs: {what} must be {rows} numbers {why}")
     return values
 
@@ -114,16 +116,17 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     of the largest logits.  A NaN counts as -inf, which has no share; a row of nothing else is all zeros.
 
     ``temperature``, ``top_p``, ``top_k``: a sequence of one number a row, or (float32, float32, int32) tensors on the logits' device,
-    whose numbers are not looked at: a temperature or top_p that is not positive, or a top_k below 1, then acts as a temperature of 0."""
+    whose numbers are not looked at: a temperature or top_p that is not positive, or a top_k below 1, then acts as a temperature of 0.
+    A call that is captured into a graph takes tensors."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("token_probs: logits must be float32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
     if not 0 < vocab <= MAX_VOCAB:
         raise KernelError(f"token_probs: a vocabulary of {vocab} is not supported (1 to {MAX_VOCAB})")
     dev = logits.device
-    temperature = _options(temperature, torch.float32, rows, dev, "temperature", lambda t: 0 <= t < float("inf"), ">= 0")
-    top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda p: p > 0, "> 0")
-    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda k: k >= 1, ">= 1")
+    temperature = _options(temperature, torch.float32, rows, dev, "temperature", lambda low, high, total: low >= 0 and high < float("inf") and total == total, ">= 0")
+    top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda low, high, total: low > 0 and total == total, "> 0")
+    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, high, total: low >= 1, ">= 1")
     if out is None:
         out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
     elif out.shape != (rows, vocab) or out.dtype != torch.float32 or not out.is_contiguous():
@@ -133,19 +136,25 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     if rows == 0:
         return out
     # whether some row is cut: known of sequences, taken as given of tensors
-    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or any(p < 1 for p in top_p) or any(k < vocab for k in top_k)
-    floats = [v for v in (temperature, top_p) if not isinstance(v, torch.Tensor)]
-    there = iter(_to_device(floats, torch.float32, dev)) if floats else None
-    temperature, top_p = (v if isinstance(v, torch.Tensor) else next(there) for v in (temperature, top_p))
-    if not isinstance(top_k, torch.Tensor):
-        top_k = _to_device([min(int(k), vocab) for k in top_k], torch.int32, dev)
-    lib = build.load("token_probs")
+    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or rows and (min(top_p) < 1 or min(top_k) < vocab)
+    given = [(i, array.array("i" if i == 2 else "f", [int(k) if k < vocab else vocab for k in v] if i == 2 else v)) for i, v in enumerate((temperature, top_p, top_k)) if not isinstance(v, torch.Tensor)]
+    if given:                                # the sequences go over together
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("token_probs: a captured call takes its options as tensors on the device (a replay would read a sequence's memory again, which is gone by then)")
+        host = torch.empty(4 * rows * len(given), dtype=torch.uint8, pin_memory=True)
+        host.copy_(torch.frombuffer(bytearray(b"".join(v.tobytes() for _, v in given)), dtype=torch.uint8))
+        there = host.to(dev, non_blocking=True)
+    options = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, top_k)]
+    at = [v.data_ptr() if v is not None else 0 for v in options]
+    for n, (i, _) in enumerate(given):
+        at[i] = there.data_ptr() + 4 * rows * n
     # a long row is cut into parts of 4,096 logits at least, one workgroup each, up to about four workgroups a compute unit in all
     parts = max(1, min(32, 4 * ops.TUNING.compute_units // rows, vocab // 4096))
-    lib.lcu_token_probs_scratch_bytes.restype = ctypes.c_size_t
-    scratch = torch.empty(int(lib.lcu_token_probs_scratch_bytes(rows, parts, int(cuts))), dtype=torch.uint8, device=dev)
-    _check(lib.lcu_token_probs(_ptr(logits), ctypes.c_longlong(logits.stride(0)), rows, vocab, _ptr(temperature), _ptr(top_p), _ptr(top_k), _ptr(out), parts,
-                               int(cuts), _ptr(scratch), _stream()), "token_probs")
+    size = build.load("token_probs").lcu_token_probs_scratch_bytes
+    size.restype = ctypes.c_size_t
+    scratch = torch.empty(size(rows, parts, int(cuts)), dtype=torch.uint8, device=dev)
+    _check(ops.bind("token_probs", "lcu_token_probs", "pliippppiip")(logits.data_ptr(), logits.stride(0), rows, vocab, *at, out.data_ptr(), parts, int(cuts), scratch.data_ptr(),
+                                                                    ops.raw_stream()), "token_probs")
     return out
 
 
@@ -199,10 +208,10 @@ def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tenso
     # the row at which a run ends is cut into parts of 2,048 tokens, one workgroup each: what a workgroup of the second launch takes at once
     parts = min(64, -(-vocab // 2048))
     sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev)
-    lib = build.load("verify")
-    _check(lib.lcu_verify_drafts(_ptr(probs), ctypes.c_longlong(probs.stride(0)), rows, _ptr(starts), requests, _ptr(drafts), n, _ptr(draft_probs),
-                                 ctypes.c_longlong(draft_probs.stride(0) if draft_probs is not None else 0), _ptr(accept), _ptr(final), vocab, int(max_drafts), parts,
-                                 _ptr(sums), _ptr(accepted), _ptr(tokens), _stream()), "verify_drafts")
+    _check(ops.bind("verify", "lcu_verify_drafts", "plipipiplppiiippp")(
+        probs.data_ptr(), probs.stride(0), rows, starts.data_ptr(), requests, drafts.data_ptr() if n else None, n, None if draft_probs is None else draft_probs.data_ptr(),
+        0 if draft_probs is None else draft_probs.stride(0), accept.data_ptr() if n else None, final.data_ptr(), vocab, int(max_drafts), parts, sums.data_ptr(), accepted.data_ptr(),
+        tokens.data_ptr(), ops.raw_stream()), "verify_drafts")
     return accepted, tokens
 
 

@@ -154,7 +154,7 @@ def test_product(n, k, kind):
                 assert_close(ops.gemm_mx4(rows, w, out_dtype=dtype, swiglu=True), act, REL[dtype] + 2e-5, f"swiglu of {m} rows to {dtype}")
 
 
-@pytest.mark.parametrize("shape", [0, 1])
+@pytest.mark.parametrize("shape", [(0, 1), (1, 1), (2, 1), (2, 3), (0, 2), (1, 5), (2, 100)])
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "four"])
 # fewer steps of k than a ring holds, as many, and more; tiles that end within rows and features; gate and up that meet within a tile of 16
 @pytest.mark.parametrize("m,n,k", [(1, 48, 32), (127, 130, 128), (130, 258, 640), (257, 600, 1000), (300, 72, 1536), (515, 1030, 384)])
@@ -180,7 +180,7 @@ def test_product_in_tiles(m, n, k, kind, shape, monkeypatch):
                 assert (room[0] == 7).all() and (room[m + 1:] == 7).all() and (room[:, :shift] == 7).all() and (room[:, shift + cols:] == 7).all()
 
 
-@pytest.mark.parametrize("shape", [0, 1])
+@pytest.mark.parametrize("shape", [(-1, 1), (0, 1), (1, 1), (2, 1), (2, 2)])
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "four"])
 def test_rows_and_features_know_nothing_of_each_other(kind, shape, monkeypatch):
     """A row of NaN and a feature of NaN reach their own row and column only; what lies behind the rows' k and behind the last row is not looked at."""

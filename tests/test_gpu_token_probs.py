@@ -9,6 +9,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from llama_cu_amd.kernels.ops import KernelError
 from test_gpu_divasun import rnd
 
 pytestmark = pytest.mark.gpu
@@ -135,6 +136,10 @@ def test_masked_logits():
         ts, ps, ks = [t] * 10, [p] * 10, [k] * 10
         check(run(logits, ts, ps, ks), logits, ts, ps, ks)
     assert (run(logits, [1.0] * 10, [1.0] * 10, [9] * 10)[1] == 0).all()
+    # whatever the temperature, -inf has no share
+    for t in (1e-38, 1e38, 3.4e38, 1e300):
+        got = run(logits[:1], [t], [1.0], [v])
+        assert (got[0, 10:] == 0).all() and abs(float(got.sum()) - 1) < 1e-5
 
 
 def test_where_it_reads_and_writes():
@@ -188,6 +193,8 @@ def test_captured():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got = sampling.token_probs(logits, *options)
+        with pytest.raises(KernelError, match="as tensors"):
+            sampling.token_probs(logits, [1.0] * rows, [1.0] * rows, [v] * rows)
     for seed in (2, 3, 4, 5):
         logits.copy_(rnd(rows, v, seed=seed, std=3.0))
         graph.replay()
