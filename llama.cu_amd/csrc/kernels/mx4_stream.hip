@@ -190,24 +190,44 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[n][m] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; ++s) {
-        mx4_u32x4 w[NT], x[MT];
-        uint32_t wscale[NT], xscale[MT];
+    // W comes from memory, four macro-steps on their way; the rows from the L2 caches, two
+    constexpr int AHEAD_W = 4, AHEAD_X = 2;
+    mx4_u32x4 w[AHEAD_W][NT], x[AHEAD_X][MT];
+    uint32_t wscale[AHEAD_W][NT], xscale[AHEAD_X][MT];
+    auto fetch_w = [&](int u, int s) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            w[n] = __builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)s * 1024));
-            wscale[n] = *(const uint32_t *)(ws[n] + (size_t)(s >> 1) * MX4_PAIR_SCALES + 4 * (s & 1)) >> 8 * g;
+            w[u][n] = __builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)s * 1024));
+            wscale[u][n] = *(const uint32_t *)(ws[n] + (size_t)(s >> 1) * MX4_PAIR_SCALES + 4 * (s & 1));
         }
+    };
+    auto fetch_x = [&](int u, int s) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            x[m] = *(const mx4_u32x4 *)(xc[m] + (size_t)s * 64);
-            xscale[m] = *(const uint32_t *)(xs[m] + (size_t)s * 4) >> 8 * g;
+            x[u][m] = *(const mx4_u32x4 *)(xc[m] + (size_t)s * 64);
+            xscale[u][m] = *(const uint32_t *)(xs[m] + (size_t)s * 4);
         }
+    };
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int u = 0; u < AHEAD_W; ++u)
+        if (s0 + u < s1) fetch_w(u, s0 + u);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-                acc[n][m] = mx4_multiply_codes_16<0>(w[n], x[m], acc[n][m], wscale[n], xscale[m]);
+    for (int u = 0; u < AHEAD_X; ++u)
+        if (s0 + u < s1) fetch_x(u, s0 + u);
+    for (int s = s0; s < s1; s += AHEAD_W) {
+#pragma unroll
+        for (int u = 0; u < AHEAD_W; ++u) {
+            if (s + u >= s1) break;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    acc[n][m] = mx4_multiply_codes_16<0>(w[u][n], x[u % AHEAD_X][m], acc[n][m], wscale[u][n] >> 8 * g, xscale[u % AHEAD_X][m] >> 8 * g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) asm volatile("s_nop 7" : "+v"(acc[n][MT - 1]));      // (the last products' wait, which the compiler leaves short behind a branch)
+            if (s + u + AHEAD_W < s1) fetch_w(u, s + u + AHEAD_W);
+            if (s + u + AHEAD_X < s1) fetch_x(u % AHEAD_X, s + u + AHEAD_X);
+        }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)

@@ -424,11 +424,12 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     if (x_kind == 4) {
         if (shape == 0) EPIS(true, 2, 2, 2, 2, 4, 4);
         else if (shape == 1) EPIS(true, 4, 2, 2, 4, 3, 2);
-        else if (shape == 2) EPIS(true, 2, 1, 2, 2, 6, 6);
+        else if (shape == 2) EPIS(true, 2, 1, 2, 2, 3, 3);
+        else if (shape == 3) EPIS(true, 2, 2, 2, 4, 3, 3);
     } else {
-        if (shape == 0) EPIS(false, 2, 2, 2, 2, 6, 6);
+        if (shape == 0) EPIS(false, 2, 2, 2, 2, 4, 4);
         else if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
-        else if (shape == 2) EPIS(false, 2, 1, 2, 2, 8, 8);
+        else if (shape == 2) EPIS(false, 2, 1, 2, 2, 4, 4);
     }
 #undef EPIS
     if (rc != LCU_OK || slices == 1) return rc;

@@ -2,7 +2,7 @@
 //
 // With the logits in descending order (equal ones by index), weights w_i = exp((l_i - l_0) / T) and prefix sums c, a draw takes the first
 // entry with c_i >= u L, L = min(top_p c_n, c_k): entry i has the share (min(c_i, L) - min(c_{i-1}, L)) / L, so the entry at the cut
-// keeps the part of its weight that lies within.  Nothing is sorted.  Six launches, a row cut into parts in those that read or write it:
+// keeps the part of its weight that lies within.  Nothing is sorted.  Rows of up to 8,192 entries: one launch, a row in a workgroup's registers.  Longer ones: six launches, a row cut into parts in those that read or write it:
 //   max     the largest logit, where it stands, and the sum of all weights, in one pass with a running maximum;
 //   count   a histogram of the distances (l_0 - l) / T, counts alone;
 //   bracket a bin's weights are known to within its width, so the bins in which the cut can lie are known from the counts, and which entries are kept in
@@ -19,7 +19,7 @@
 // that is not positive leaves the first of the largest logits.
 #include "common.h"
 
-constexpr int TP_THREADS = 512, TP_CUT_THREADS = 1024, TP_BINS = 8192, TP_GATHER = 8192, TP_EACH = TP_GATHER / TP_CUT_THREADS, TP_MAX_PARTS = 32, TP_MAX_VOCAB = 1 << 19;
+constexpr int TP_THREADS = 512, TP_CUT_THREADS = 1024, TP_BINS = 8192, TP_GATHER = 8192, TP_EACH = TP_GATHER / TP_CUT_THREADS, TP_MAX_PARTS = 32, TP_MAX_VOCAB = 1 << 19, TP_SMALL = 8 * TP_CUT_THREADS;
 constexpr double TP_ONE = 17592186044416.0;          // 2^44: 2^19 weights of 1 are 2^63
 constexpr float TP_NOTHING = 126.f;                  // the exponential ends at 2^-126
 constexpr float TP_LOG2E = 1.44269504088896341f;
@@ -40,6 +40,10 @@ struct TpRow {
     float kept, inv;
 };
 struct TpEntry { unsigned int key; int at; };
+
+// Up to 64 rows' options in the launch itself.
+constexpr int TP_GIVEN = 64;
+struct TpOptions { float temperature[TP_GIVEN], top_p[TP_GIVEN]; int top_k[TP_GIVEN]; };
 
 __device__ __forceinline__ unsigned int tp_key(float x) {
     const unsigned int u = x == 0.f ? 0u : __float_as_uint(x);
@@ -141,16 +145,21 @@ __device__ __forceinline__ void tp_stretch(int vocab, int part, int parts, int &
 
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_THREADS)
-tp_max_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, TpPart *__restrict__ part, TpRow *__restrict__ rows,
-              unsigned int *__restrict__ hist) {
+tp_max_kernel(const float *__restrict__ logits, size_t ld, int vocab, TpOptions given, const float *__restrict__ temperature, float *__restrict__ options,
+              TpPart *__restrict__ part, TpRow *__restrict__ rows, unsigned int *__restrict__ hist) {
     const int r = blockIdx.x, parts = gridDim.y;
+    if (options && blockIdx.y == 0 && threadIdx.x == 0) {            // for the launches that follow
+        options[r] = given.temperature[r];
+        options[gridDim.x + r] = given.top_p[r];
+        ((int *)options)[2 * gridDim.x + r] = given.top_k[r];
+    }
     int lo, hi;
     tp_stretch(vocab, blockIdx.y, parts, lo, hi);
     if (hist) {                                      // cleared for the next launch
         for (int b = (int)blockIdx.y * TP_THREADS + threadIdx.x; b < TP_BINS; b += TP_THREADS * parts) hist[(size_t)r * TP_BINS + b] = 0u;
         if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].mass_above = 0; rows[r].gathered = 0; }
     }
-    const float inv_t = tp_inv_t(temperature[r]);
+    const float inv_t = tp_inv_t(options ? given.temperature[r] : temperature[r]);
     float most = -INFINITY, least = INFINITY;
     double sum = 0.0;
     int at = 0x7fffffff;
@@ -363,14 +372,142 @@ __device__ __forceinline__ float tp_share(const TpRow &t, unsigned int k, int i,
     return w * t.inv;
 }
 
+// What the search for a cut needs of LDS.
+struct TpShared {
+    unsigned long long mass[256];
+    unsigned int count[256], found[2];
+    TpSum found_above;
+};
+
+// The cut among the entries that `each` goes through (f(key, index, weight)); above: what lies over all of them, base and span: the smallest key of them and how far the largest lies from
+// it.  Every thread of the workgroup (256 or more) calls it and gets the answer.
+template <class Each>
+__device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum above, unsigned int base, unsigned int span, Each each) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long limit_p = c.limit_p < 524288.0 ? (unsigned long long)(c.limit_p * TP_ONE) : ~0ull;
+    // the digits of the largest key at which the entries down to it reach one of the limits; `above`: what lies over the keys with the digits so far
+    unsigned int border = 0;                           // (less the smallest key)
+    bool all = false;                                  // (the limits lie a rounding beyond all there is)
+    int open = span ? 32 - __clz(span) : 1;            // bits that are not decided yet
+    while (open > 0) {
+        const int shift = max(0, open - 8);
+        __syncthreads();
+        if (threadIdx.x < 256) { sh.mass[threadIdx.x] = 0; sh.count[threadIdx.x] = 0; }
+        __syncthreads();
+        each([&](unsigned int k, int, float w) {
+            const unsigned int digit = ((k - base) >> shift) - (border >> shift);       // (border's undecided bits are zeros)
+            if (digit < 256u && k - base >= border) {
+                atomicAdd(&sh.count[digit], 1u);
+                atomicAdd(&sh.mass[digit], tp_fixed(w));
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x < WAVE) {                      // a wave walks the digits from the largest on, four a lane
+            TpSum mine = {0, 0}, digit[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 255 - (4 * lane + e);
+                digit[e] = {sh.mass[d], sh.count[d]};
+                mine.mass += digit[e].mass; mine.count += digit[e].count;
+            }
+            TpSum scan = mine;
+#pragma unroll
+            for (int off = 1; off < WAVE; off <<= 1) {
+                const unsigned long long m = __shfl_up(scan.mass, off, WAVE);
+                const unsigned int n = __shfl_up(scan.count, off, WAVE);
+                if (lane >= off) { scan.mass += m; scan.count += n; }
+            }
+            TpSum so_far = {above.mass + scan.mass - mine.mass, above.count + scan.count - mine.count};
+            int got = -1;
+            TpSum got_above = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const TpSum with = {so_far.mass + digit[e].mass, so_far.count + digit[e].count};
+                if (got < 0 && digit[e].count && (with.count >= (unsigned int)c.k || with.mass >= limit_p)) { got = 255 - (4 * lane + e); got_above = so_far; }
+                so_far = with;
+            }
+            const unsigned long long reached = __ballot(got >= 0);
+            if (reached == 0) {
+                if (lane == WAVE - 1) { sh.found[0] = 256; sh.found_above = so_far; }
+            } else if (lane == __ffsll((unsigned long long)reached) - 1) {
+                sh.found[0] = (unsigned int)got;
+                sh.found_above = got_above;
+            }
+        }
+        __syncthreads();
+        above = sh.found_above;
+        if (sh.found[0] == 256u) { all = true; break; }
+        border |= sh.found[0] << shift;
+        open = shift;
+    }
+    TpRow t = {};
+    t.last = 0x7fffffff;
+    t.kept = -1.f;                                     // (what is kept whole has its weight's own digits, not those of the sums)
+    unsigned long long limit = above.mass;
+    if (!all) {
+        const unsigned int equal = sh.count[sh.found[0]];                        // of the last digit: all have the key
+        border += base;
+        const unsigned long long each_mass = tp_fixed(tp_weight(tp_distance(c, tp_logit(border))));
+        limit = limit_p;
+        if (above.count + equal >= (unsigned int)c.k) limit = min(limit, above.mass + ((unsigned int)c.k - above.count) * each_mass);
+        unsigned int rank = each_mass ? (unsigned int)min((limit - above.mass + each_mass - 1) / each_mass, (unsigned long long)equal) : min((unsigned int)c.k - above.count, equal);
+        rank = max(1u, rank);
+        const unsigned long long kept = limit - above.mass - (unsigned long long)(rank - 1) * each_mass;
+        if (kept < each_mass) t.kept = (float)((double)kept / (double)limit);
+        t.border = border;
+        // the rank-th smallest index among the equal ones, eight bits at a time
+        unsigned int index = 0;
+        if (equal > 1) {
+            unsigned int left = rank;
+            for (int shift = 16; shift >= 0; shift -= 8) {
+                __syncthreads();
+                if (threadIdx.x < 256) sh.count[threadIdx.x] = 0;
+                __syncthreads();
+                each([&](unsigned int k, int i, float) {
+                    if (k == border && (shift == 16 || ((unsigned int)i ^ index) >> (shift + 8) == 0)) atomicAdd(&sh.count[(unsigned int)i >> shift & 255], 1u);
+                });
+                __syncthreads();
+                if (threadIdx.x < WAVE) {
+                    unsigned int mine = 0, n[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { n[e] = sh.count[4 * lane + e]; mine += n[e]; }
+                    unsigned int scan = mine;
+#pragma unroll
+                    for (int off = 1; off < WAVE; off <<= 1) {
+                        const unsigned int up = __shfl_up(scan, off, WAVE);
+                        if (lane >= off) scan += up;
+                    }
+                    unsigned int so_far = scan - mine;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (so_far < left && left <= so_far + n[e]) { sh.found[0] = 4 * lane + e; sh.found[1] = so_far; }
+                        so_far += n[e];
+                    }
+                }
+                __syncthreads();
+                index |= sh.found[0] << shift;
+                left -= sh.found[1];
+            }
+            t.last = (int)index;
+        }
+        // (a single one: whatever its index, it is the last)
+        if (equal == 1) {
+            __syncthreads();
+            each([&](unsigned int k, int i, float) { if (k == border) sh.found[0] = (unsigned int)i; });
+            __syncthreads();
+            t.last = (int)sh.found[0];
+        }
+    }
+    t.inv = limit ? (float)(TP_ONE / (double)limit) : 0.f;
+    return t;
+}
+
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_CUT_THREADS)
 tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
               const TpPart *__restrict__ part, int parts, TpRow *__restrict__ rows, const TpEntry *__restrict__ entries, float *__restrict__ out) {
-    __shared__ unsigned long long mass[256];
-    __shared__ unsigned int count[256];
-    __shared__ unsigned int found[2], key_lo, key_hi;
-    __shared__ TpSum found_above;
+    __shared__ TpShared sh;
+    __shared__ unsigned int key_lo, key_hi;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
     if (c.empty || c.greedy || !c.cuts) {
@@ -417,122 +554,7 @@ tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
                 if (e * TP_CUT_THREADS + threadIdx.x < gathered) f(key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
         }
     };
-    const unsigned long long limit_p = c.limit_p < 524288.0 ? (unsigned long long)(c.limit_p * TP_ONE) : ~0ull;
-    // the digits of the largest key at which the entries down to it reach one of the limits; `above`: what lies over the keys with the digits so far
-    TpSum above = how == TP_NEAR ? TpSum{b.mass_above, b.before} : TpSum{0, 0};
-    unsigned int border = 0;                           // (less the smallest key)
-    bool all = false;                                  // (the limits lie a rounding beyond all there is)
-    int open = span ? 32 - __clz(span) : 1;            // bits that are not decided yet
-    while (open > 0) {
-        const int shift = max(0, open - 8);
-        __syncthreads();
-        if (threadIdx.x < 256) { mass[threadIdx.x] = 0; count[threadIdx.x] = 0; }
-        __syncthreads();
-        each([&](unsigned int k, int, float w) {
-            const unsigned int digit = ((k - base) >> shift) - (border >> shift);       // (border's undecided bits are zeros)
-            if (digit < 256u && k - base >= border) {
-                atomicAdd(&count[digit], 1u);
-                atomicAdd(&mass[digit], tp_fixed(w));
-            }
-        });
-        __syncthreads();
-        if (threadIdx.x < WAVE) {                      // a wave walks the digits from the largest on, four a lane
-            TpSum mine = {0, 0}, digit[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = 255 - (4 * lane + e);
-                digit[e] = {mass[d], count[d]};
-                mine.mass += digit[e].mass; mine.count += digit[e].count;
-            }
-            TpSum scan = mine;
-#pragma unroll
-            for (int off = 1; off < WAVE; off <<= 1) {
-                const unsigned long long m = __shfl_up(scan.mass, off, WAVE);
-                const unsigned int n = __shfl_up(scan.count, off, WAVE);
-                if (lane >= off) { scan.mass += m; scan.count += n; }
-            }
-            TpSum so_far = {above.mass + scan.mass - mine.mass, above.count + scan.count - mine.count};
-            int got = -1;
-            TpSum got_above = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const TpSum with = {so_far.mass + digit[e].mass, so_far.count + digit[e].count};
-                if (got < 0 && digit[e].count && (with.count >= (unsigned int)c.k || with.mass >= limit_p)) { got = 255 - (4 * lane + e); got_above = so_far; }
-                so_far = with;
-            }
-            const unsigned long long reached = __ballot(got >= 0);
-            if (reached == 0) {
-                if (lane == WAVE - 1) { found[0] = 256; found_above = so_far; }
-            } else if (lane == __ffsll((unsigned long long)reached) - 1) {
-                found[0] = (unsigned int)got;
-                found_above = got_above;
-            }
-        }
-        __syncthreads();
-        above = found_above;
-        if (found[0] == 256u) { all = true; break; }
-        border |= found[0] << shift;
-        open = shift;
-    }
-    TpRow t = {};
-    t.last = 0x7fffffff;
-    t.kept = -1.f;                                     // (what is kept whole has its weight's own digits, not those of the sums)
-    unsigned long long limit = above.mass;
-    if (!all) {
-        const unsigned int equal = count[found[0]];                        // of the last digit: all have the key
-        border += base;
-        const unsigned long long each_mass = tp_fixed(tp_weight(tp_distance(c, tp_logit(border))));
-        limit = limit_p;
-        if (above.count + equal >= (unsigned int)c.k) limit = min(limit, above.mass + ((unsigned int)c.k - above.count) * each_mass);
-        unsigned int rank = each_mass ? (unsigned int)min((limit - above.mass + each_mass - 1) / each_mass, (unsigned long long)equal) : min((unsigned int)c.k - above.count, equal);
-        rank = max(1u, rank);
-        const unsigned long long kept = limit - above.mass - (unsigned long long)(rank - 1) * each_mass;
-        if (kept < each_mass) t.kept = (float)((double)kept / (double)limit);
-        t.border = border;
-        // the rank-th smallest index among the equal ones, eight bits at a time
-        unsigned int index = 0;
-        if (equal > 1) {
-            unsigned int left = rank;
-            for (int shift = 16; shift >= 0; shift -= 8) {
-                __syncthreads();
-                if (threadIdx.x < 256) count[threadIdx.x] = 0;
-                __syncthreads();
-                each([&](unsigned int k, int i, float) {
-                    if (k == border && (shift == 16 || ((unsigned int)i ^ index) >> (shift + 8) == 0)) atomicAdd(&count[(unsigned int)i >> shift & 255], 1u);
-                });
-                __syncthreads();
-                if (threadIdx.x < WAVE) {
-                    unsigned int mine = 0, n[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { n[e] = count[4 * lane + e]; mine += n[e]; }
-                    unsigned int scan = mine;
-#pragma unroll
-                    for (int off = 1; off < WAVE; off <<= 1) {
-                        const unsigned int up = __shfl_up(scan, off, WAVE);
-                        if (lane >= off) scan += up;
-                    }
-                    unsigned int so_far = scan - mine;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (so_far < left && left <= so_far + n[e]) { found[0] = 4 * lane + e; found[1] = so_far; }
-                        so_far += n[e];
-                    }
-                }
-                __syncthreads();
-                index |= found[0] << shift;
-                left -= found[1];
-            }
-            t.last = (int)index;
-        }
-        // (a single one: whatever its index, it is the last)
-        if (equal == 1) {
-            __syncthreads();
-            each([&](unsigned int k, int i, float) { if (k == border) found[0] = (unsigned int)i; });
-            __syncthreads();
-            t.last = (int)found[0];
-        }
-    }
-    t.inv = limit ? (float)(TP_ONE / (double)limit) : 0.f;
+    TpRow t = tp_search(c, sh, how == TP_NEAR ? TpSum{b.mass_above, b.before} : TpSum{0, 0}, base, span, each);
     t.store = how != TP_ALL;
     if (how == TP_ALL) {
 #pragma unroll
@@ -564,30 +586,143 @@ tp_store_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
     tp_store_shares<WIDE>(row, lo, hi, to, share);
 }
 
-// Bytes of scratch memory that lcu_token_probs needs, in whatever state they are (cuts: some row may have a cut).
-LCU_API size_t lcu_token_probs_scratch_bytes(int rows, int parts, int cuts) {
-    if (rows <= 0 || parts <= 0) return 0;
-    return (size_t)rows * (parts * sizeof(TpPart) + (cuts ? sizeof(TpRow) + TP_BINS * sizeof(unsigned int) + TP_GATHER * sizeof(TpEntry) : 0));
+// A row of up to 1,024 EACH entries as a whole, in registers: one launch for everything.
+template <int EACH>
+__global__ void __launch_bounds__(TP_CUT_THREADS)
+tp_small_kernel(const float *__restrict__ logits, size_t ld, int vocab, TpOptions given, const float *__restrict__ temperature, const float *__restrict__ top_p,
+                const int *__restrict__ top_k, float *__restrict__ out) {
+    constexpr int WAVES = TP_CUT_THREADS / WAVE;
+    __shared__ TpShared sh;
+    __shared__ float wave_most[WAVES];
+    __shared__ int wave_at[WAVES];
+    __shared__ double wave_sum[WAVES];
+    __shared__ unsigned int key_lo, key_hi;
+    const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float t_r = temperature ? temperature[r] : given.temperature[r], p_r = top_p ? top_p[r] : given.top_p[r];
+    const int k_r = top_k ? top_k[r] : given.top_k[r];
+    const float *row = logits + r * ld;
+    float *to = out + (size_t)r * vocab;
+    float l[EACH], most = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = e * TP_CUT_THREADS + threadIdx.x;
+        l[e] = i < vocab ? tp_clean(row[i]) : -INFINITY;
+        most = fmaxf(most, l[e]);
+    }
+    most = wave_max(most);
+    if (lane == 0) wave_most[wave] = most;
+    if (threadIdx.x == 0) { key_lo = 0xffffffffu; key_hi = 0; }
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, wave_most[w]);
+    TpCut c;
+    c.most = most;
+    c.inv_t = tp_inv_t(t_r);
+    c.k = k_r;
+    c.empty = most == -INFINITY;
+    c.greedy = !(t_r > 0.f) || k_r <= 1 || !(p_r > 0.f);
+    c.cuts = k_r < vocab || p_r < 1.f;
+    int at = 0x7fffffff;
+    double sum = 0.0;
+    unsigned int lowest = 0xffffffffu, highest = 0;
+#pragma unroll
+    for (int e = EACH - 1; e >= 0; --e) {
+        if (l[e] == most) at = e * TP_CUT_THREADS + threadIdx.x;
+        const float d = tp_distance(c, l[e]);
+        if (d <= TP_NOTHING) {
+            sum += (double)tp_weight(d);
+            lowest = min(lowest, tp_key(l[e]));
+            highest = max(highest, tp_key(l[e]));
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        at = min(at, __shfl_xor(at, off, WAVE));
+        sum += __shfl_xor(sum, off, WAVE);
+        lowest = min(lowest, (unsigned int)__shfl_xor(lowest, off, WAVE));
+        highest = max(highest, (unsigned int)__shfl_xor(highest, off, WAVE));
+    }
+    if (lane == 0) {
+        wave_at[wave] = at;
+        wave_sum[wave] = sum;
+        atomicMin(&key_lo, lowest);
+        atomicMax(&key_hi, highest);
+    }
+    __syncthreads();
+    c.at = 0x7fffffff;
+    c.sum = 0.0;
+    for (int w = 0; w < WAVES; ++w) { c.at = min(c.at, wave_at[w]); c.sum += wave_sum[w]; }
+    c.limit_p = p_r < 1.f ? (double)p_r * c.sum : INFINITY;
+    TpRow t = {};
+    t.last = 0x7fffffff;
+    t.kept = -1.f;
+    t.inv = (float)(1.0 / c.sum);
+    if (!c.empty && !c.greedy && c.cuts)
+        t = tp_search(c, sh, TpSum{0, 0}, key_lo, key_hi - key_lo, [&](auto f) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const float d = tp_distance(c, l[e]);
+                if (d <= TP_NOTHING && e * TP_CUT_THREADS + (int)threadIdx.x < vocab) f(tp_key(l[e]), e * TP_CUT_THREADS + (int)threadIdx.x, tp_weight(d));
+            }
+        });
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int i = e * TP_CUT_THREADS + threadIdx.x;
+        const float d = tp_distance(c, l[e]);
+        if (i < vocab) to[i] = c.empty ? 0.f : c.greedy ? (i == c.at ? 1.f : 0.f) : d <= TP_NOTHING ? tp_share(t, tp_key(l[e]), i, tp_weight(d)) : 0.f;
+    }
 }
 
-// logits: [rows, ld] float32; temperature, top_p, top_k: [rows], on the device; out: [rows, vocab] float32; parts: workgroups a row, 1 to 32; cuts: 0 if no row has
-// top_k < vocab or top_p < 1; scratch: lcu_token_probs_scratch_bytes(rows, parts, cuts) bytes, 8-byte aligned.
-LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int vocab, const float *temperature, const float *top_p, const int *top_k, float *out, int parts,
-                            int cuts, void *scratch, hipStream_t stream) {
+// Bytes of scratch memory that lcu_token_probs needs, in whatever state they are (cuts: some row may have a cut).
+LCU_API size_t lcu_token_probs_scratch_bytes(int rows, int vocab, int parts, int cuts) {
+    if (rows <= 0 || parts <= 0 || vocab <= TP_SMALL) return 0;
+    return (size_t)rows * (parts * sizeof(TpPart) + (cuts ? sizeof(TpRow) + TP_BINS * sizeof(unsigned int) + TP_GATHER * sizeof(TpEntry) : 0) + 3 * sizeof(float));
+}
+
+// logits: [rows, ld] float32; temperature, top_p, top_k: [rows], on the device, or null and `given` holds the three one after the other on the host (up to 64 rows); out: [rows,
+// vocab] float32; parts: workgroups a row, 1 to 32; cuts: 0 if no row has top_k < vocab or top_p < 1; scratch: lcu_token_probs_scratch_bytes bytes, 8-byte aligned.
+LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int vocab, const float *temperature, const float *top_p, const int *top_k, const float *given, float *out,
+                            int parts, int cuts, void *scratch, hipStream_t stream) {
     if (rows <= 0) return LCU_OK;
-    if (vocab <= 0 || vocab > TP_MAX_VOCAB || (rows > 1 && ld < vocab) || parts < 1 || parts > TP_MAX_PARTS || !logits || !temperature || !top_p || !top_k || !out || !scratch ||
-        (uintptr_t)scratch % 8)
+    const bool small = vocab <= TP_SMALL;
+    if (vocab <= 0 || vocab > TP_MAX_VOCAB || (rows > 1 && ld < vocab) || parts < 1 || parts > TP_MAX_PARTS || !logits || !out || (!small && (!scratch || (uintptr_t)scratch % 8)) ||
+        (given ? rows > TP_GIVEN : !temperature || !top_p || !top_k))
         return LCU_BAD_ARGUMENT;
+    TpOptions options;
+    if (given) {
+        temperature = top_p = nullptr;
+        top_k = nullptr;
+        for (int r = 0; r < rows; ++r) {
+            options.temperature[r] = given[r];
+            options.top_p[r] = given[rows + r];
+            options.top_k[r] = ((const int *)given)[2 * rows + r];
+        }
+    }
+    if (small) {
+#define SMALL(EACH) tp_small_kernel<EACH><<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(logits, (size_t)ld, vocab, options, temperature, top_p, top_k, out)
+        if (vocab <= TP_CUT_THREADS) SMALL(1);
+        else if (vocab <= 4 * TP_CUT_THREADS) SMALL(4);
+        else SMALL(8);
+#undef SMALL
+        LCU_LAUNCH_CHECK();
+        return LCU_OK;
+    }
     char *at = (char *)scratch;
     TpPart *part = (TpPart *)at;             at += (size_t)rows * parts * sizeof(TpPart);
     TpRow *state = (TpRow *)at;              at += cuts ? (size_t)rows * sizeof(TpRow) : 0;
     TpEntry *entries = (TpEntry *)at;        at += cuts ? (size_t)rows * TP_GATHER * sizeof(TpEntry) : 0;
     unsigned int *hist = cuts ? (unsigned int *)at : nullptr;
+    at += cuts ? (size_t)rows * TP_BINS * sizeof(unsigned int) : 0;
+    float *copied = given ? (float *)at : nullptr;
+    if (given) {
+        temperature = copied;
+        top_p = copied + rows;
+        top_k = (const int *)copied + 2 * rows;
+    }
     const bool wide = (uintptr_t)logits % 16 == 0 && ld % 4 == 0 && vocab % 4 == 0 && (uintptr_t)out % 16 == 0;
     const dim3 cut(rows, parts), block(TP_THREADS);
 #define GO(WIDE)                                                                                                                                    \
     do {                                                                                                                                            \
-        tp_max_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, part, state, hist);                                   \
+        tp_max_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, options, temperature, copied, part, state, hist);                  \
         LCU_LAUNCH_CHECK();                                                                                                                         \
         if (cuts) {                                                                                                                                 \
             tp_count_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, hist);                      \

@@ -7,7 +7,7 @@
 // the target's are.  Probabilities that are no finite positive numbers count as zero.
 //
 // Only the row at which the run ends is read (two, with the draft's): first its parts' sums, a workgroup each, in 64 bits and a fixed order; then a
-// workgroup a request finds the part, and reads that again to find the token.  Bound by memory: 4 or 8 bytes a token of the vocabulary.
+// workgroup a request finds the part, and reads that again to find the token; up to 8,192 tokens one workgroup a request does all.  Bound by memory: 4 or 8 bytes a token of the vocabulary.
 #include "common.h"
 
 constexpr int VF_THREADS = 512, VF_MAX_PARTS = 64, VF_MAX_DRAFTS = 1024;
@@ -186,16 +186,80 @@ vf_token_kernel(const float *__restrict__ p, size_t ldp, int rows, const int *__
     if (threadIdx.x == 0) out[run.taken] = found < vocab ? found : last;      // (the goal lies a rounding beyond the part: its last)
 }
 
+// A vocabulary of up to 512 PIECE tokens: one launch, a workgroup a request.
+template <int PIECE>
+__global__ void __launch_bounds__(VF_THREADS)
+vf_small_kernel(const float *__restrict__ p, size_t ldp, int rows, const int *__restrict__ starts, const int *__restrict__ drafts, int n_drafts, const float *__restrict__ q,
+                size_t ldq, const float *__restrict__ accept, const float *__restrict__ final_u, int vocab, int most, int *__restrict__ accepted, int *__restrict__ tokens) {
+    __shared__ double wave_sums[VF_THREADS / WAVE];
+    __shared__ int found, last;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const VfRun run = vf_run(p, ldp, rows, starts, drafts, n_drafts, q, ldq, accept, vocab, most);
+    int *out = tokens + (size_t)b * (most + 1);
+    for (int i = threadIdx.x; i <= most; i += VF_THREADS)
+        if (run.bad || i != run.taken) out[i] = !run.bad && i < run.taken ? drafts[run.draft + i] : -1;
+    if (threadIdx.x == 0) { accepted[b] = run.bad ? 0 : run.taken; found = 0x7fffffff; last = -1; }
+    if (run.bad) return;
+    VfLeft left = vf_left(run, p, ldp, drafts, q, ldq);
+    const int piece = (vocab + VF_THREADS - 1) / VF_THREADS, from = min(vocab, (int)threadIdx.x * piece), to = min(vocab, from + piece);
+    double v[PIECE], at = 0.0, mine = 0.0, total = 0.0;
+    for (int turn = 0; turn < 2; ++turn) {             // what is left; and where that is nothing the target's own
+        mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < PIECE; ++i) v[i] = from + i < to ? left(from + i) : 0.0;
+#pragma unroll
+        for (int i = 0; i < PIECE; ++i) mine += v[i];
+        const double scan = vf_wave_scan(mine, lane);
+        __syncthreads();
+        if (lane == WAVE - 1) wave_sums[wave] = scan;
+        __syncthreads();
+        at = scan - mine;
+        total = 0.0;
+        for (int w = 0; w < VF_THREADS / WAVE; ++w) {
+            if (w == wave) at += total;
+            total += wave_sums[w];
+        }
+        if (total > 0.0) break;
+        left.q = nullptr;
+        left.without = -1;
+    }
+    const double goal = (double)final_u[b] * total;
+    int mine_last = -1, mine_found = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < PIECE; ++i) {
+        at += v[i];
+        if (v[i] > 0.0) {
+            mine_last = from + i;
+            if (at > goal) mine_found = min(mine_found, from + i);
+        }
+    }
+    const unsigned long long founds = __ballot(mine_found < vocab), lasts = __ballot(mine_last >= 0);
+    if (founds && lane == __ffsll(founds) - 1) atomicMin(&found, mine_found);
+    if (lasts && lane == 63 - __clzll(lasts)) atomicMax(&last, mine_last);
+    __syncthreads();
+    if (threadIdx.x == 0) out[run.taken] = found < vocab ? found : last;
+}
+
 // probs: [rows, ldp] float32, drafts, accept: [n_drafts], draft_probs: null or [n_drafts, ldq], starts: [requests + 1], final_u: [requests]; accepted: [requests],
-// tokens: [requests, most + 1]; parts: workgroups a request, 1 to 64, of 8,192 tokens at most; sums: [requests][parts][2] doubles.
+// tokens: [requests, most + 1]; parts: workgroups a request, 1 to 64, of 8,192 tokens at most; sums: [requests][parts][2] doubles
+// (one part needs none).
 LCU_API int lcu_verify_drafts(const float *probs, long long ldp, int rows, const int *starts, int requests, const int *drafts, int n_drafts, const float *draft_probs,
                               long long ldq, const float *accept, const float *final_u, int vocab, int most, int parts, double *sums, int *accepted, int *tokens,
                               hipStream_t stream) {
     if (requests <= 0) return LCU_OK;
-    if (rows < 0 || vocab <= 0 || most < 0 || most > VF_MAX_DRAFTS || n_drafts < 0 || parts < 1 || parts > VF_MAX_PARTS || !probs || !starts || !final_u || !sums || !accepted ||
+    if (rows < 0 || vocab <= 0 || most < 0 || most > VF_MAX_DRAFTS || n_drafts < 0 || parts < 1 || parts > VF_MAX_PARTS || !probs || !starts || !final_u || !accepted || (parts > 1 && !sums) ||
         !tokens || (n_drafts && (!drafts || !accept)) || (rows > 1 && ldp < vocab) || (draft_probs && n_drafts > 1 && ldq < vocab) ||
         (vocab + parts - 1) / parts > 16 * VF_THREADS)
         return LCU_BAD_ARGUMENT;
+    if (parts == 1) {
+#define SMALL(PIECE) vf_small_kernel<PIECE><<<dim3(requests), dim3(VF_THREADS), 0, stream>>>(probs, (size_t)ldp, rows, starts, drafts, n_drafts, draft_probs, (size_t)ldq, accept, \
+                                                                                         final_u, vocab, most, accepted, tokens)
+        if (vocab <= 2 * VF_THREADS) SMALL(2);
+        else SMALL(16);
+#undef SMALL
+        LCU_LAUNCH_CHECK();
+        return LCU_OK;
+    }
     // few requests: a workgroup a part; many: four of them, whose loads are all on their way at once
 #define SUM(PARTS) vf_sum_kernel<PARTS><<<dim3(requests, (parts + PARTS - 1) / PARTS), dim3(VF_THREADS), 0, stream>>>(probs, (size_t)ldp, rows, starts, drafts, n_drafts, draft_probs, \
                                                                                                               (size_t)ldq, accept, vocab, most, parts, sums, accepted)

@@ -8,6 +8,7 @@ CPU path: a tensor that is not on the GPU is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -2860,14 +2861,60 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     return Mx4(codes[:, :16 * blocks], scales[:, :blocks], q.k, True)
 
 
-def mx4_choice(m: int, n: int, k: int, kind: int, swiglu: bool) -> Tuple[int, int]:
-    """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: ``(-1, 1)`` the one that streams the weight, else the shape of
-    the tiles and into how many slices K is cut (mx4_tiles.hip)."""
-    if m <= 16:
-        return -1, 1
+# What the kernels of the 4-bit products take, us, fitted to 12,000 timed products of 12 to 3,200 rows and 9,500 of 1 to 96 (64 to 128,256 features, K 128 to 28,672;
+# weights out of memory): the choice by these numbers takes 1.01 (many rows) to 1.05 (few) times what the best choice takes, geometric mean.
+# Tiles (features, tokens) by whether the rows are in 4 bits and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three workgroups
+# on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
+_MX4_TILES = {
+    (False, 0): (128, 128, 2, 3.56, 2.33, (0.45, 0.71, 0.95), 2.54, 0.24),
+    (False, 1): (256, 256, 1, 4.07, 5.26, (1.09,), 3.05, 0.17),
+    (False, 2): (128, 64, 3, 4.71, 0.01, (0.40, 0.54, 0.65), 2.44, 0.29),
+    (True, 0): (128, 128, 1, 2.19, 3.10, (0.77,), 2.40, 0.21),
+    (True, 1): (256, 256, 1, 2.69, 6.13, (1.51,), 3.59, 0.15),
+    (True, 2): (128, 64, 2, 2.93, 1.25, (0.62, 1.11), 2.52, 0.25),
+    (True, 3): (128, 256, 1, 2.00, 3.82, (1.00,), 3.40, 0.16),
+}
+# The kernel that streams the weight, by the kind of the rows: us a launch; a workgroup alone, and for each macro-step of a wave; a macro-step where workgroups share a compute unit, and what four
+# rows add to that.
+_MX4_STREAM = {1: (2.20, 0.32, 0.20, 0.34, 0.11), 3: (0.05, 3.44, 0.49, 0.39, 0.32), 4: (2.76, 0.87, 0.01, 0.13, 0.09)}
+_MX4_SLICES = (1, 2, 3, 4, 6, 8, 12, 16)
+
+
+@functools.lru_cache(maxsize=8192)
+def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
+    macros = -(-k // 128)
+    best = (float("inf"), -1, 1)
     if m <= 64:
-        return 2, 8
-    return (1 if m > 128 and (m + 255) // 256 * ((n + 255) // 256) * 2 > TUNING.compute_units else 0), 1
+        tiles = 1 if m <= 16 else 2 if m <= 32 or kind == 3 else 4        # of 16 rows, together
+        fours = 4 * tiles if m > 16 or kind == 4 else 1 if m <= 4 else 2 if m <= 8 and kind == 1 else 4      # loads of four rows
+        per = -(-macros // 8) if kind == 4 else 2 * -(-macros // 16)
+        launch, alone, step, shared, rows = _MX4_STREAM[kind]
+        load = max(1.0, -(-n // 16) * -(-m // (16 * tiles)) / cu)
+        best = (launch + alone + per * step + load * per * (shared + rows * fours), -1, 1)
+    steps = -(-k // 256) if kind == 4 else 2 * macros if kind == 1 else 12 * -(-k // 256)
+    for (four, shape), (features, tokens, held, launch, each_wg, step, join, join_mb) in _MX4_TILES.items():
+        if four != (kind == 4):
+            continue
+        tiles = -(-n // features) * -(-m // tokens)
+        for slices in _MX4_SLICES:
+            if slices > 1 and (steps < 2 * slices or tiles * slices > 4 * held * cu):
+                break
+            each = -(-steps // slices)
+            real = -(-steps // each)
+            rounds, left = divmod(tiles * real, held * cu)
+            t = launch + rounds * (each_wg + each * step[held - 1])
+            if left:
+                t += each_wg + each * step[-(-left // cu) - 1]
+            if real > 1:
+                t += join + join_mb * real * m * n * 8 / 2 ** 20
+            best = min(best, (t, shape, slices))
+    return best[1:]
+
+
+def mx4_choice(m: int, n: int, k: int, kind: int) -> Tuple[int, int]:
+    """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: ``(-1, 1)`` the one that streams the weight (up to 64 rows), else the
+    shape of the tiles and into how many slices K is cut (mx4_tiles.hip): the one that takes least by the times above."""
+    return _mx4_choice(m, n, k, kind, TUNING.compute_units)
 
 
 def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, swiglu: bool = False) -> torch.Tensor:
@@ -2909,7 +2956,7 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         ld, scales, lds = rows.stride(0), None, 0
     if m == 1:                             # (the one row's stride says nothing)
         ld, lds = (128 * w.pairs, 8 * w.pairs) if four else (rows.shape[1], 0)
-    shape, slices = mx4_choice(m, w.n, k, kind, swiglu)
+    shape, slices = mx4_choice(m, w.n, k, kind)
     row_bytes = ld if four else 2 * ld
     most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
     if shape >= 0 and (most < 512 or (w.n + 528) * w.pairs * 128 >= 1 << 32):

@@ -117,7 +117,7 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
 
     ``temperature``, ``top_p``, ``top_k``: a sequence of one number a row, or (float32, float32, int32) tensors on the logits' device,
     whose numbers are not looked at: a temperature or top_p that is not positive, or a top_k below 1, then acts as a temperature of 0.
-    A call that is captured into a graph takes tensors."""
+    A call of more than 64 rows that is captured into a graph takes tensors."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise KernelError("token_probs: logits must be float32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
@@ -137,24 +137,33 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
         return out
     # whether some row is cut: known of sequences, taken as given of tensors
     cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or rows and (min(top_p) < 1 or min(top_k) < vocab)
-    given = [(i, array.array("i" if i == 2 else "f", [int(k) if k < vocab else vocab for k in v] if i == 2 else v)) for i, v in enumerate((temperature, top_p, top_k)) if not isinstance(v, torch.Tensor)]
-    if given:                                # the sequences go over together
-        if torch.cuda.is_current_stream_capturing():
-            raise KernelError("token_probs: a captured call takes its options as tensors on the device (a replay would read a sequence's memory again, which is gone by then)")
-        host = torch.empty(4 * rows * len(given), dtype=torch.uint8, pin_memory=True)
-        host.copy_(torch.frombuffer(bytearray(b"".join(v.tobytes() for _, v in given)), dtype=torch.uint8))
-        there = host.to(dev, non_blocking=True)
-    options = [v if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, top_k)]
-    at = [v.data_ptr() if v is not None else 0 for v in options]
-    for n, (i, _) in enumerate(given):
-        at[i] = there.data_ptr() + 4 * rows * n
+    sequences = [None if isinstance(v, torch.Tensor) else array.array("f" if i < 2 else "i", v if i < 2 else [int(k) if k < vocab else vocab for k in v])
+                 for i, v in enumerate((temperature, top_p, top_k))]
+    at = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, top_k)]
+    given = None
+    if any(v is not None for v in sequences):
+        data = bytearray(b"".join(v.tobytes() for v in sequences if v is not None))
+        if rows <= 64 and all(v is not None for v in sequences):
+            given = (ctypes.c_char * len(data)).from_buffer(data)             # in the launch itself
+        else:
+            if torch.cuda.is_current_stream_capturing():
+                raise KernelError("token_probs: a captured call of more than 64 rows, or with some options as tensors, takes all of them as tensors on the device "
+                                  "(a replay would read a sequence's memory again, which is gone by then)")
+            host = torch.empty(len(data), dtype=torch.uint8, pin_memory=True)
+            host.copy_(torch.frombuffer(data, dtype=torch.uint8))
+            there = host.to(dev, non_blocking=True)
+            place = there.data_ptr()
+            for i, v in enumerate(sequences):
+                if v is not None:
+                    at[i], place = place, place + 4 * rows
     # a long row is cut into parts of 4,096 logits at least, one workgroup each, up to about four workgroups a compute unit in all
     parts = max(1, min(32, 4 * ops.TUNING.compute_units // rows, vocab // 4096))
     size = build.load("token_probs").lcu_token_probs_scratch_bytes
     size.restype = ctypes.c_size_t
-    scratch = torch.empty(size(rows, parts, int(cuts)), dtype=torch.uint8, device=dev)
-    _check(ops.bind("token_probs", "lcu_token_probs", "pliippppiip")(logits.data_ptr(), logits.stride(0), rows, vocab, *at, out.data_ptr(), parts, int(cuts), scratch.data_ptr(),
-                                                                    ops.raw_stream()), "token_probs")
+    size = size(rows, vocab, parts, int(cuts))
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _check(ops.bind("token_probs", "lcu_token_probs", "pliipppppiip")(logits.data_ptr(), logits.stride(0), rows, vocab, *at, given, out.data_ptr(), parts, int(cuts),
+                                                                     None if scratch is None else scratch.data_ptr(), ops.raw_stream()), "token_probs")
     return out
 
 
@@ -205,12 +214,12 @@ def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tenso
     tokens = torch.empty((requests, int(max_drafts) + 1), dtype=torch.int32, device=dev)
     if requests == 0:
         return accepted, tokens
-    # the row at which a run ends is cut into parts of 2,048 tokens, one workgroup each: what a workgroup of the second launch takes at once
-    parts = min(64, -(-vocab // 2048))
-    sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev)
+    # the row at which a run ends is cut into parts of 2,048 tokens, one workgroup each: what a workgroup of the second launch takes at once; a workgroup a request does all of a short one
+    parts = 1 if vocab <= 8192 else min(64, -(-vocab // 2048))
+    sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev) if parts > 1 else None
     _check(ops.bind("verify", "lcu_verify_drafts", "plipipiplppiiippp")(
         probs.data_ptr(), probs.stride(0), rows, starts.data_ptr(), requests, drafts.data_ptr() if n else None, n, None if draft_probs is None else draft_probs.data_ptr(),
-        0 if draft_probs is None else draft_probs.stride(0), accept.data_ptr() if n else None, final.data_ptr(), vocab, int(max_drafts), parts, sums.data_ptr(), accepted.data_ptr(),
+        0 if draft_probs is None else draft_probs.stride(0), accept.data_ptr() if n else None, final.data_ptr(), vocab, int(max_drafts), parts, None if sums is None else sums.data_ptr(), accepted.data_ptr(),
         tokens.data_ptr(), ops.raw_stream()), "verify_drafts")
     return accepted, tokens
 

@@ -79,12 +79,16 @@ OPTIONS = [(1.0, 1.0, 10 ** 9), (0.7, 0.9, 10 ** 9), (1.0, 1.0, 40), (1.3, 0.95,
            (1.0, 1e-6, 10 ** 9), (1.0, 1 - 2.0 ** -20, 3), (0.8, 0.999, 2), (1e-30, 0.9, 20)]
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 3, 63, 257, 1000, 4096, 32003])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 63, 257, 1000, 1025, 4096, 4097, 8192, 8193, 32003])
 def test_options(vocab):
     n = len(OPTIONS)
     logits = rnd(n, vocab, seed=vocab, std=3.0)
     ts, ps, ks = ([o[i] for o in OPTIONS] for i in range(3))
     check(run(logits, ts, ps, ks), logits, ts, ps, ks, f"vocabulary {vocab}")
+    # more rows than a launch holds the options of
+    many = run(logits.repeat(6, 1), ts * 6, ps * 6, ks * 6)
+    assert torch.equal(many, run(logits, ts, ps, ks).repeat(6, 1)) or vocab > 8192          # (a long row's sums go by its parts, which are fewer of many rows)
+    check(many, logits.repeat(6, 1), ts * 6, ps * 6, ks * 6, "many")
     # each alone: in more parts a row, and rows without a cut on their own
     for i in range(n):
         check(run(logits[i:i + 1], ts[i:i + 1], ps[i:i + 1], ks[i:i + 1]), logits[i:i + 1], ts[i:i + 1], ps[i:i + 1], ks[i:i + 1], "alone")
@@ -180,9 +184,10 @@ def test_it_is_what_sample_rows_draws_from():
             assert reach[i] >= u - 1e-5 and (i == 0 or reach[i - 1] <= u + 1e-5)
 
 
-def test_captured():
+@pytest.mark.parametrize("v", [900, 9000, 40000])
+def test_captured(v):
     from llama_cu_amd import sampling
-    rows, v = 4, 9000
+    rows = 4
     options = [torch.tensor([0.7, 1.0, 0.0, 1.3]).cuda(), torch.tensor([0.9, 1.0, 1.0, 1.0]).cuda(), torch.tensor([v, v, v, 30], dtype=torch.int32).cuda()]
     logits = rnd(rows, v, seed=1, std=3.0).cuda()
     side = torch.cuda.Stream()
@@ -193,10 +198,13 @@ def test_captured():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         got = sampling.token_probs(logits, *options)
+        again = sampling.token_probs(logits, [0.7, 1.0, 0.0, 1.3], [0.9, 1.0, 1.0, 1.0], [v, v, v, 30])
         with pytest.raises(KernelError, match="as tensors"):
-            sampling.token_probs(logits, [1.0] * rows, [1.0] * rows, [v] * rows)
+            sampling.token_probs(logits, options[0], [1.0] * rows, [v] * rows)
+        with pytest.raises(KernelError, match="as tensors"):
+            sampling.token_probs(logits[:1].expand(65, v).contiguous(), [1.0] * 65, [1.0] * 65, [v] * 65)
     for seed in (2, 3, 4, 5):
         logits.copy_(rnd(rows, v, seed=seed, std=3.0))
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(got, sampling.token_probs(logits, *options))
+        assert torch.equal(got, sampling.token_probs(logits, *options)) and torch.equal(again, got)

@@ -80,7 +80,7 @@ def case(requests, most, vocab, seed, ragged=True, std=2.0, apart=0.7):
 
 
 @pytest.mark.parametrize("lookup", [False, True])
-@pytest.mark.parametrize("requests,most,vocab", [(1, 1, 2), (1, 4, 1), (3, 0, 50), (1, 5, 257), (9, 3, 1000), (17, 7, 4099), (40, 8, 131), (2, 4, 128259), (300, 2, 67)])
+@pytest.mark.parametrize("requests,most,vocab", [(1, 1, 2), (1, 4, 1), (3, 0, 50), (1, 5, 257), (9, 3, 1000), (17, 7, 4099), (40, 8, 131), (2, 4, 128259), (300, 2, 67), (5, 3, 1024), (5, 3, 1025), (4, 3, 8192), (4, 3, 8193), (6, 4, 20000), (2, 2, 300001)])
 def test_token_for_token(requests, most, vocab, lookup):
     for seed in range(3):
         probs, starts, drafts, accept, final, q = case(requests, most, vocab, seed, ragged=seed > 0)
@@ -101,9 +101,10 @@ def test_all_kinds_of_endings():
         agree(probs, starts, drafts, torch.full_like(accept, u), torch.full_like(final, u), 6)
 
 
-def test_greedy_rows():
+@pytest.mark.parametrize("v", [300, 10000])
+def test_greedy_rows(v):
     """One-hot distributions: a draft stands where it is the target's token, and that token comes out."""
-    v, n = 300, 5
+    n = 5
     want = torch.randint(0, v, (n + 1,), generator=torch.Generator().manual_seed(1))
     probs = torch.nn.functional.one_hot(want, v).float()
     drafts = want[:n].int().clone()
@@ -119,8 +120,8 @@ def test_greedy_rows():
             assert got[1][0].tolist() == want[:wrong + 1].tolist() + [-1] * (n - wrong)
 
 
-def test_rows_that_leave_nothing():
-    v = 100
+@pytest.mark.parametrize("v", [100, 9000])
+def test_rows_that_leave_nothing(v):
     probs, starts, drafts, accept, final, q = case(6, 3, v, 9, ragged=False)
     probs[starts[1]] = 0.0                              # a row without any probability
     probs[starts[2]] = q[3 * 2] * 0.5                   # less than the draft's everywhere: nothing is left but the target's own
@@ -139,9 +140,10 @@ def test_rows_that_leave_nothing():
     agree(lone, [0, 2], torch.tensor([7], dtype=torch.int32), torch.tensor([1.0]), torch.tensor([0.5]), 1)
 
 
-def test_starts_that_make_no_sense():
+@pytest.mark.parametrize("v", [64, 9000])
+def test_starts_that_make_no_sense(v):
     from llama_cu_amd import sampling
-    probs, starts, drafts, accept, final, q = case(4, 3, 64, 2, ragged=False)
+    probs, starts, drafts, accept, final, q = case(4, 3, v, 2, ragged=False)
     for bad in ([0, 4, 3, 12, 16], [0, -5, 8, 12, 16], [0, 4, 8, 12, 400], [2 ** 31 - 1, 4, 8, -2 ** 31, 16], [0, 16, 16, 16, 16], [1, 5, 9, 13, 17]):
         a, t = sampling.verify_drafts(probs.cuda(), torch.tensor(bad, dtype=torch.int64).int().cuda(), drafts.cuda(), accept.cuda(), final.cuda(), 3, q.cuda())
         good = sampling.verify_drafts(probs.cuda(), torch.tensor(starts, dtype=torch.int32).cuda(), drafts.cuda(), accept.cuda(), final.cuda(), 3, q.cuda())
