@@ -17,6 +17,8 @@ def _base(p: argparse.ArgumentParser) -> None:
                    "--random-weights a folder that holds config.json, or a config.json itself, is enough")
     p.add_argument("--max-steps", type=int, default=1000, help="most tokens to generate (default 1000)")
     p.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
+    p.add_argument("--weights", choices=["file", "mx4"], default="file",
+                   help="how matrices are held: as their file's, or attention's and the dense feed-forward's in microscaled 4-bit numbers")
     p.add_argument("--random-weights", type=int, default=None, metavar="SEED",
                    help="make the weights from SEED on the GPU instead of reading model.safetensors")
     p.add_argument("--temperature", type=float, default=0.0)
@@ -48,7 +50,7 @@ def _engine(args):
     from .config import load_config
     from .engine.engine import Engine
     from .sampling import SamplingParams, TOP_K_ALL
-    kw = dict(page_size=args.page_size, max_seqs=args.max_seqs)
+    kw = dict(page_size=args.page_size, max_seqs=args.max_seqs, weights=args.weights)
     if args.num_pages:
         kw["num_pages"] = args.num_pages
     elif args.max_tokens:

@@ -6,7 +6,8 @@
 // tile and pair of macro-steps (256 k)
 //   codes   2 KB: [macro-step][group g = 0 .. 3][row of the tile] 16 bytes, the block of 32 that begins at k = 128 macro + 32 g: a wave's
 //           load of 16 bytes a lane is one run of 1 KB and is an operand of the matrix instructions as it arrives;
-//   scales  128 bytes: [row][macro-step][group], a row's eight blocks together.
+//   scales  128 bytes: [row][odd][slice], a row's eight blocks together, block 2 slice + odd: the lane of a product of 32 x 32 x 64 that has the row's even or odd blocks finds its
+//           four side by side.
 #pragma once
 #include "common.h"
 
@@ -33,6 +34,9 @@ __device__ __forceinline__ mx4_u32x4 mx4_to_bf16(uint32_t codes, float scale) {
     v[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
     return v;
 }
+
+// Where the scale of block b (0 .. 7) of a row's pair stands.
+__device__ __forceinline__ int mx4_scale_place(int b) { return (b & 1) * 4 + (b >> 1); }
 
 // Where row `row` of a weight in the products' order begins in its tile's first pair: bytes.
 __device__ __forceinline__ size_t mx4_row_codes(int row, int pairs) { return (size_t)(row >> 4) * pairs * MX4_PAIR_CODES + (row & 15) * 16; }

@@ -28,7 +28,8 @@ __device__ __forceinline__ uint32_t magnitude(bf16_t x) { return (uint32_t)(x.bi
 // units: 8 numbers each, `row_units` to a row (a multiple of 32: rows are filled up to 256 numbers).
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(MX4_THREADS)
-mx4_quantize_kernel(const T *__restrict__ x, size_t ldx, int k, uint32_t units, uint32_t row_units, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+mx4_quantize_kernel(const T *__restrict__ x, size_t ldx, int k, uint32_t units, uint32_t row_units, uint32_t *__restrict__ codes, uint8_t *__restrict__ scales,
+                    uint8_t *__restrict__ by_pair, size_t rows) {
     const uint32_t u = blockIdx.x * MX4_THREADS + threadIdx.x;
     if (u >= units) return;                                        // (units are whole waves' halves: a block's four lanes go together)
     const uint32_t row = u / row_units, at = (u - row * row_units) * MX4_UNIT;
@@ -52,7 +53,11 @@ mx4_quantize_kernel(const T *__restrict__ x, size_t ldx, int k, uint32_t units, 
 #undef PAIR
     }
     codes[u] = e == 255 ? 0u : out;
-    if ((threadIdx.x & 3) == 0) scales[u >> 2] = (uint8_t)e;
+    if ((threadIdx.x & 3) == 0) {
+        scales[u >> 2] = (uint8_t)e;
+        const uint32_t block = at / MX4_BLOCK;
+        if (by_pair) by_pair[(block / 8 * rows + row) * 8 + mx4_scale_place(block % 8)] = (uint8_t)e;
+    }
 }
 
 template <class T, bool WIDE>
@@ -132,15 +137,16 @@ static uint32_t mx4_units(long long rows, long long row_units) {
     return units > 0 && units < 1ll << 31 ? (uint32_t)units : 0u;
 }
 
-// x: [rows, ldx] of `type`; codes: [rows][kp / 2], scales: [rows][kp / 32] with kp = k rounded up to 256, codes 4-byte aligned.
-LCU_API int lcu_mx4_quantize(const void *x, long long ldx, int type, long long rows, int k, void *codes, void *scales, hipStream_t stream) {
+// x: [rows, ldx] of `type`; codes: [rows][kp / 2], scales: [rows][kp / 32] with kp = k rounded up to 256, codes 4-byte aligned; by_pair: null, or the scales once more as the products in
+// tiles read them, [kp / 256][rows][8], a row's eight as in mx4.h.
+LCU_API int lcu_mx4_quantize(const void *x, long long ldx, int type, long long rows, int k, void *codes, void *scales, void *by_pair, hipStream_t stream) {
     if (rows <= 0 || k <= 0) return LCU_OK;
     const long long row_units = ((long long)k + MX4_PAIR - 1) / MX4_PAIR * (MX4_PAIR / MX4_UNIT);
     const uint32_t units = mx4_units(rows, row_units);
     if (!units || !x || !codes || !scales || (uintptr_t)codes % 4 || (rows > 1 && ldx < k) || (type != LCU_BF16 && type != LCU_F32)) return LCU_BAD_ARGUMENT;
     const dim3 grid((units + MX4_THREADS - 1) / MX4_THREADS), block(MX4_THREADS);
     const bool wide = mx4_wide(x, ldx, type);
-#define GO(T, WIDE) mx4_quantize_kernel<T, WIDE><<<grid, block, 0, stream>>>((const T *)x, (size_t)ldx, k, units, (uint32_t)row_units, (uint32_t *)codes, (uint8_t *)scales)
+#define GO(T, WIDE) mx4_quantize_kernel<T, WIDE><<<grid, block, 0, stream>>>((const T *)x, (size_t)ldx, k, units, (uint32_t)row_units, (uint32_t *)codes, (uint8_t *)scales, (uint8_t *)by_pair, (size_t)rows)
     if (type == LCU_BF16) { if (wide) GO(bf16_t, true); else GO(bf16_t, false); }
     else { if (wide) GO(float, true); else GO(float, false); }
 #undef GO

@@ -127,7 +127,7 @@ mx4_stream_kernel(const bf16_t *__restrict__ X, int ldx, int plane, Mx4Args a) {
         mx4_u32x4 w[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float sc = mx4_scale(((h ? scale[u][n].y : scale[u][n].x) >> 8 * g) & 255u);
+            const float sc = mx4_scale(((g & 1 ? scale[u][n].y : scale[u][n].x) >> 8 * (2 * h + (g >> 1))) & 255u);      // block 4 h + g
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[n][j] = mx4_to_bf16(code[u][n][h][j], sc);
         }
@@ -198,7 +198,7 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             w[u][n] = __builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)s * 1024));
-            wscale[u][n] = *(const uint32_t *)(ws[n] + (size_t)(s >> 1) * MX4_PAIR_SCALES + 4 * (s & 1));
+            wscale[u][n] = *(const uint32_t *)(ws[n] + (size_t)(s >> 1) * MX4_PAIR_SCALES + 4 * (g & 1)) >> 8 * (2 * (s & 1) + (g >> 1));      // block 4 (s & 1) + g
         }
     };
     auto fetch_x = [&](int u, int s) {
@@ -222,7 +222,7 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
-                    acc[n][m] = mx4_multiply_codes_16<0>(w[u][n], x[u % AHEAD_X][m], acc[n][m], wscale[u][n] >> 8 * g, xscale[u % AHEAD_X][m] >> 8 * g);
+                    acc[n][m] = mx4_multiply_codes_16<0>(w[u][n], x[u % AHEAD_X][m], acc[n][m], wscale[u][n], xscale[u % AHEAD_X][m] >> 8 * g);
 #pragma unroll
             for (int n = 0; n < NT; ++n) asm volatile("s_nop 7" : "+v"(acc[n][MT - 1]));      // (the last products' wait, which the compiler leaves short behind a branch)
             if (s + u + AHEAD_W < s1) fetch_w(u, s + u + AHEAD_W);

@@ -8,7 +8,8 @@
 //                      slices (32 x 32 x 16) out of it as they are needed; W takes a quarter of the LDS and of its bandwidth that bfloat16 would.
 //                      The waves stand four by features and two by tokens, since every wave converts its own features' codes.
 //   rows in float32    are bfloat16 rows of three times the k (planes one behind the other), with W gone through three times.
-//   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, eight bytes a row and step, come into registers.
+//   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, four bytes a lane and step, come into registers.  Steps of 128 k, which the rings hold more of,
+//                      took a tenth longer: half a line a row and load.
 #include <type_traits>
 #include "mx4.h"
 #include "mx4/matrix.h"
@@ -28,7 +29,7 @@ template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_> stru
     static constexpr int FT = FT_, TT = TT_, WF = WF_, WT = WT_, SF = SF_, ST = ST_, SLICES = 4;
     static constexpr int WAVES = WF * WT, THREADS = WAVES * WAVE, F = 32 * FT * WF, T = 32 * TT * WT;
     static constexpr int FP = FOUR ? 8 : 2, TP = 8;                    // pieces (16 bytes) of a row a stage
-    static constexpr int STEP_CODES = FOUR ? 2048 : 512;               // bytes of a tile of 16 features a step
+    static constexpr int STEP_CODES = 256 * FP;                        // bytes of a tile of 16 features a step
     static constexpr int LF = F * FP / WAVE / WAVES, LT = T * TP / WAVE / WAVES;       // loads of a wave a stage
     static constexpr int LS = FOUR ? FT + TT : FT;                     // and of scales, into registers
     static constexpr int LDS = SF * F * FP + ST * T * TP;              // pieces
@@ -36,10 +37,14 @@ template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_> stru
     static_assert(FT % 2 == 0 && F * FP % (WAVE * WAVES) == 0 && T * TP % (WAVE * WAVES) == 0 && SF >= ST && ST >= 2 && LDS * 16 <= 160 * 1024, "whole loads, and room for the stages");
 };
 
+// Where piece c of row r stands among the row's in LDS: sixteen neighbouring rows' pieces c lie in sixteen places that are read at once (c ^ (r & 7), in eight: four
+// cycles a read more).
+__device__ __forceinline__ int mt_place(int r, int c) { return c ^ (r >> 1 & 7); }
+
 template <class S> struct MtFrags { mx4_u32x4 f[S::FT], t[S::TT]; };
 
-// The scales of a step: FOUR: a row's eight bytes, moved so that the lane's own are bytes 0 and 2 of each half; else the lane's one byte of each tile.
-template <class S> struct MtScales { uint32_t f[S::FT][S::FOUR ? 2 : 1], t[S::FOUR ? S::TT : 1][2]; };
+// The scales of a step: FOUR: of the lane's row its four blocks', a byte a slice; else the byte of its one block.
+template <class S> struct MtScales { uint32_t f[S::FT], t[S::FOUR ? S::TT : 1]; };
 
 __device__ __forceinline__ void mt_read(mx4_u32x4 &to, const mx4_u32x4 *from) {
     to = *from;
@@ -54,26 +59,28 @@ __device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const 
                                         IssueF &&issue_f, const int (&at_f)[S::SLICES], const int (&at_t)[S::SLICES], MtFrags<S> (&op)[2], mx4_u32x4 (&codes)[S::FT],
                                         const MtScales<S> &before, const MtScales<S> &now, mx4_f32x16 (&acc)[S::FT][S::TT]) {
     auto slice = [&](auto number) {
-        constexpr int s = decltype(number)::value, PRODUCTS = S::FT * S::TT, used = (s + 3) % 4;         // the slice that is multiplied
+        constexpr int s = decltype(number)::value, PRODUCTS = S::FT * S::TT, used = (s + S::SLICES - 1) % S::SLICES;         // the slice that is multiplied
         MtFrags<S> &use = op[(s + 1) & 1], &get = op[s & 1];
 #pragma unroll
         for (int i = 0; i < PRODUCTS; ++i) {
             const int f = i / S::TT, t = i % S::TT;
             if constexpr (S::FOUR) {
                 const MtScales<S> &sc = s == 0 ? before : now;
-                acc[f][t] = mx4_multiply_codes_32<2 * (used & 1)>(use.f[f], use.t[t], acc[f][t], sc.f[f][used / 2], sc.t[t][used / 2]);
+                acc[f][t] = mx4_multiply_codes_32<used>(use.f[f], use.t[t], acc[f][t], sc.f[f], sc.t[t]);
             } else {
                 acc[f][t] = mx4_multiply_32(use.f[f], use.t[t], acc[f][t]);
             }
             __builtin_amdgcn_sched_barrier(0);
             {
-                constexpr int ALL = PRODUCTS * (S::SLICES - 1), L = S::LF + S::LT;
-                const int n = s * PRODUCTS + i, l0 = n * L / ALL, l1 = (n + 1) * L / ALL;
+                // the tokens' loads in the first slice where they are wanted in the next step, the features' behind them; else all spread over all slices but the last
+                constexpr int FIRST = S::ST == 2 ? PRODUCTS : PRODUCTS * (S::SLICES - 1) * S::LT / (S::LT + S::LF), REST = PRODUCTS * (S::SLICES - 1) - FIRST;
+                const int n = s * PRODUCTS + i;
+                if (n < FIRST) {
 #pragma unroll
-                for (int l = l0; l < l1; ++l) {
-                    if (l < S::LT) issue_t(dt, l);
-                    else if (l < L) issue_f(df, l - S::LT);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int l = n * S::LT / FIRST; l < (n + 1) * S::LT / FIRST; ++l) { issue_t(dt, l); __builtin_amdgcn_sched_barrier(0); }
+                } else if (n < FIRST + REST) {
+#pragma unroll
+                    for (int l = (n - FIRST) * S::LF / REST; l < (n - FIRST + 1) * S::LF / REST; ++l) { issue_f(df, l); __builtin_amdgcn_sched_barrier(0); }
                 }
             }
             if constexpr (S::FOUR) {
@@ -98,7 +105,7 @@ __device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const 
                     const int f0 = (i - HALF) * S::FT / (PRODUCTS - HALF), f1 = (i + 1 - HALF) * S::FT / (PRODUCTS - HALF);
 #pragma unroll
                     for (int x = f0; x < f1; ++x) {
-                        get.f[x] = mx4_to_bf16(codes[x][s], mx4_scale(now.f[x][0]));
+                        get.f[x] = mx4_to_bf16(codes[x][s], mx4_scale(now.f[x]));
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -113,7 +120,7 @@ __device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const 
 
 struct MtArgs {
     const void *x, *xs;             // rows (bfloat16, or codes) and the codes' scales
-    uint32_t ldx, lds, x_bytes, xs_bytes;     // bytes from row to row; of the whole
+    uint32_t ldx, lds, x_bytes, xs_bytes;     // bytes from row to row, and of the scales from a pair of macro-steps to the next (a row's are 8 bytes); of the whole
     const uint8_t *codes, *scales;
     uint32_t codes_bytes, scales_bytes;
     int pairs;
@@ -156,8 +163,8 @@ mx4_tiles_kernel(MtArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < S::LT; ++i) {
-        const int r = (i * S::WAVES + wave) * 8 + lane / 8;
-        from_t[i] = (uint32_t)(tt0 * S::T + r) * a.ldx + 16u * ((lane % 8) ^ (r & 7));
+        const int r = (i * S::WAVES + wave) * (WAVE / S::TP) + lane / S::TP;
+        from_t[i] = (uint32_t)(tt0 * S::T + r) * a.ldx + 16u * mt_place(r, lane % S::TP);
     }
     mx4_u32x4 *const lds_f = mt_lds, *const lds_t = mt_lds + S::SF * S::F * S::FP;
     // (a later step than there are: the last once more, which nobody reads)
@@ -168,52 +175,32 @@ mx4_tiles_kernel(MtArgs a) {
     };
     auto issue_t = [&](mx4_u32x4 *dst, int step, int i) {
         auto *to = (__attribute__((address_space(3))) void *)(dst + (i * S::WAVES + wave) * WAVE);
-        const uint32_t from = from_t[i] + (uint32_t)(first + min(step, steps - 1)) * 128u;
+        const uint32_t from = from_t[i] + (uint32_t)(first + min(step, steps - 1)) * (16u * S::TP);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(xb, to, 16, from, 0, 0, 0);
     };
     // ---- where the lane's operands stand in a stage
     int at_f[S::SLICES], at_t[S::SLICES];
 #pragma unroll
     for (int s = 0; s < S::SLICES; ++s) {
-        at_f[s] = FOUR ? l32 / 16 * 128 + (s * 2 + hi) * 16 + l32 % 16 : l32 / 16 * 32 + hi * 16 + l32 % 16;
-        at_t[s] = l32 * S::TP + ((FOUR ? 2 * s + hi : 4 * hi + s) ^ (l32 & 7));
+        at_f[s] = l32 / 16 * (16 * S::FP) + ((FOUR ? s * 2 : 0) + hi) * 16 + l32 % 16;
+        at_t[s] = l32 * S::TP + mt_place(l32, FOUR ? 2 * s + hi : 4 * hi + s);
     }
     const int of_f = wf * 32 * FT * S::FP, of_t = wt * 32 * TT * S::TP;
     uint32_t sf[FT], st[TT];
 #pragma unroll
-    for (int f = 0; f < FT; ++f) sf[f] = (uint32_t)mx4_row_scales(feature(wf * 32 * FT + 32 * f + l32), a.pairs) + (FOUR ? 0 : hi);
+    for (int f = 0; f < FT; ++f) sf[f] = (uint32_t)mx4_row_scales(feature(wf * 32 * FT + 32 * f + l32), a.pairs) + 4 * hi;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) st[t] = (uint32_t)(tt0 * S::T + wt * 32 * TT + 32 * t + l32) * a.lds;
+    for (int t = 0; t < TT; ++t) st[t] = (uint32_t)(tt0 * S::T + wt * 32 * TT + 32 * t + l32) * 8u + 4u * hi;
     auto fetch_scales = [&](MtScales<S> &to, int step, int w_step) {
         if constexpr (FOUR) {
-            typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 #pragma unroll
-            for (int f = 0; f < FT; ++f) {
-                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sb, sf[f] + (uint32_t)w_step * MX4_PAIR_SCALES, 0, 0));
-                to.f[f][0] = v[0]; to.f[f][1] = v[1];
-            }
+            for (int f = 0; f < FT; ++f) to.f[f] = __builtin_amdgcn_raw_buffer_load_b32(sb, sf[f] + (uint32_t)w_step * MX4_PAIR_SCALES, 0, 0);
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(xsb, st[t] + (uint32_t)step * 8u, 0, 0));
-                to.t[t][0] = v[0]; to.t[t][1] = v[1];
-            }
+            for (int t = 0; t < TT; ++t) to.t[t] = __builtin_amdgcn_raw_buffer_load_b32(xsb, st[t] + (uint32_t)step * a.lds, 0, 0);
         } else {
 #pragma unroll
-            for (int f = 0; f < FT; ++f) to.f[f][0] = __builtin_amdgcn_raw_buffer_load_b8(sb, sf[f] + (uint32_t)(w_step >> 2) * MX4_PAIR_SCALES + 2u * (w_step & 3), 0, 0);
+            for (int f = 0; f < FT; ++f) to.f[f] = __builtin_amdgcn_raw_buffer_load_b8(sb, sf[f] + (uint32_t)(w_step >> 2) * MX4_PAIR_SCALES + (w_step & 3), 0, 0);
         }
-    };
-    auto moved = [&](const MtScales<S> &v) {
-        MtScales<S> o = v;
-        if constexpr (FOUR) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int f = 0; f < FT; ++f) o.f[f][h] = v.f[f][h] >> 8 * hi;
-#pragma unroll
-                for (int t = 0; t < TT; ++t) o.t[t][h] = v.t[t][h] >> 8 * hi;
-            }
-        }
-        return o;
     };
     mx4_f32x16 acc[FT][TT];
 #pragma unroll
@@ -228,12 +215,12 @@ mx4_tiles_kernel(MtArgs a) {
 #pragma unroll
     for (int f = 0; f < FT; ++f) {
         op[1].f[f] = codes[f] = mx4_u32x4{0u, 0u, 0u, 0u};
-        before.f[f][0] = before.f[f][FOUR ? 1 : 0] = 0;
+        before.f[f] = 0;
     }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
         op[1].t[t] = mx4_u32x4{0u, 0u, 0u, 0u};
-        before.t[FOUR ? t : 0][0] = before.t[FOUR ? t : 0][1] = 0;
+        before.t[FOUR ? t : 0] = 0;
     }
     // W's step of the features' ring: one that goes round
     int wf_step = first % a.w_steps;
@@ -253,7 +240,7 @@ mx4_tiles_kernel(MtArgs a) {
     }
     int rf = 0, rt = 0, df = S::SF - 1, dt = S::ST - 1;
     for (int t = 0; t < steps; ++t) {
-        now = moved(next);
+        now = next;
         s_step = next_w(s_step);
         fetch_scales(next, first + min(t + 1, steps - 1), s_step);
         mt_wait_loads<S::LEFT>();                              // this step's stages are there
@@ -271,7 +258,7 @@ mx4_tiles_kernel(MtArgs a) {
 #pragma unroll
     for (int i = 0; i < FT * TT; ++i) {
         const int f = i / TT, t = i % TT;
-        if constexpr (FOUR) acc[f][t] = mx4_multiply_codes_32<2>(op[1].f[f], op[1].t[t], acc[f][t], before.f[f][1], before.t[t][1]);
+        if constexpr (FOUR) acc[f][t] = mx4_multiply_codes_32<3>(op[1].f[f], op[1].t[t], acc[f][t], before.f[f], before.t[t]);
         else acc[f][t] = mx4_multiply_32(op[1].f[f], op[1].t[t], acc[f][t]);
     }
     mt_wait_loads<0>();                                        // (the copies that nobody reads have landed before LDS is used otherwise)
@@ -376,7 +363,7 @@ static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
     return LCU_OK;
 }
 
-// Arguments as lcu_mx4_stream's; rows in 4 bits and their scales in whole pairs of macro-steps (256 k), bfloat16 rows in multiples of 64 k.  shape: 0: tiles of 128 x 128
+// Arguments as lcu_mx4_stream's, but that the scales of rows in 4 bits come by pairs of macro-steps (256 k): [pairs][lds bytes], 8 bytes a row; rows in 4 bits in whole pairs.  shape: 0: tiles of 128 x 128
 // (features x tokens), 1: 256 x 256, 2: 128 x 64.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats,
 // 16-byte aligned.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
 LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *xs, long long lds, const void *codes, const void *scales, int pairs, void *y, long long ldy,
@@ -388,7 +375,7 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
         ((uintptr_t)x | (uintptr_t)codes) % 16 || (uintptr_t)scales % 8 || row_bytes <= 0 || row_bytes % 16 || (M + 512ll) * row_bytes >= limit || (w_rows + 512) * pairs * 128 >= limit)
         return LCU_BAD_ARGUMENT;
     if (x_kind == 1 ? ldx < 128ll * macros : x_kind == 3 ? ldx % 768 || ldx < 3ll * macros * 128
-        : x_kind == 4 ? !xs || lds % 8 || (uintptr_t)xs % 8 || ldx < 128ll * ((macros + 1) / 2) || lds < 8ll * ((macros + 1) / 2) || (M + 512ll) * lds >= limit : true)
+        : x_kind == 4 ? !xs || lds % 8 || (uintptr_t)xs % 8 || ldx < 128ll * ((macros + 1) / 2) || lds < 8ll * M || (macros + 1) / 2 * lds + 4096 >= limit : true)
         return LCU_BAD_ARGUMENT;
     MtArgs a = {};
     a.x = x; a.xs = xs;
@@ -402,7 +389,7 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     a.steps = x_kind == 3 ? 3 * a.w_steps : a.w_steps;
     if (x_kind == 3 && a.w_steps > pairs * 4) return LCU_BAD_ARGUMENT;
     a.x_bytes = (uint32_t)((M - 1) * row_bytes + (long long)a.steps * 128);
-    a.xs_bytes = x_kind == 4 ? (uint32_t)((M - 1) * lds + two * 8ll) : 0u;
+    a.xs_bytes = x_kind == 4 ? (uint32_t)((two - 1) * lds + M * 8ll) : 0u;
     if (slices < 1 || slices > a.steps || (slices > 1 && (!planes || (uintptr_t)planes % 16))) return LCU_BAD_ARGUMENT;
     a.each = (a.steps + slices - 1) / slices;
     slices = (a.steps + a.each - 1) / a.each;                  // (as many as hold a step)
@@ -423,13 +410,14 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     int rc = LCU_BAD_ARGUMENT;
     if (x_kind == 4) {
         if (shape == 0) EPIS(true, 2, 2, 2, 2, 4, 4);
-        else if (shape == 1) EPIS(true, 4, 2, 2, 4, 3, 2);
+        else if (shape == 1) EPIS(true, 4, 4, 2, 2, 3, 2);
         else if (shape == 2) EPIS(true, 2, 1, 2, 2, 3, 3);
         else if (shape == 3) EPIS(true, 2, 2, 2, 4, 3, 3);
     } else {
         if (shape == 0) EPIS(false, 2, 2, 2, 2, 4, 4);
         else if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
         else if (shape == 2) EPIS(false, 2, 1, 2, 2, 4, 4);
+        else if (shape == 3) EPIS(false, 2, 4, 4, 1, 4, 3);
     }
 #undef EPIS
     if (rc != LCU_OK || slices == 1) return rc;

@@ -24,6 +24,7 @@ class EngineConfig:
     max_model_len: Optional[int] = None     # most tokens a request may hold (default, and at most: the model's positions)
     use_graphs: bool = True                 # replay decode steps from captured graphs
     pack_weights: Optional[bool] = None     # a second copy of the matrices in the decode kernels' order (default: if memory allows)
+    weights: str = "file"                   # "mx4": attention's and the dense feed-forward's matrices in microscaled 4-bit numbers, a quarter of bfloat16's bytes
     run_ahead: bool = True                  # launch a round before the round before has been read
     logprobs: bool = False                  # every sampled token comes with the log of the probability the model gave it
     poison_freed: bool = False              # debugging: fill pages that change hands with NaN
@@ -33,6 +34,8 @@ class EngineConfig:
             raise ValueError(f"engine configuration: {field} = {getattr(self, field)!r} {why}")
         if self.dtype not in ("bfloat16", "bf16", "float32", "f32", "fp32"):
             fail("dtype", "is neither bfloat16 nor float32")
+        if self.weights not in ("file", "mx4"):
+            fail("weights", "is neither file nor mx4")
         for f in ("page_size", "max_seqs", "max_batch_tokens"):
             if not isinstance(getattr(self, f), int) or getattr(self, f) <= 0:
                 fail(f, "must be a positive integer")
@@ -59,7 +62,7 @@ class EngineConfig:
     def runner_kwargs(self) -> Dict[str, Any]:
         """What ``ModelRunner`` takes (the scheduler's and the engine's own fields apart)."""
         kw = {k: getattr(self, k) for k in ("dtype", "device", "page_size", "max_seqs", "max_batch_tokens", "max_model_len",
-                                             "kv_fraction", "use_graphs", "pack_weights", "poison_freed")}
+                                             "kv_fraction", "use_graphs", "pack_weights", "weights", "poison_freed")}
         if self.num_pages is not None:
             kw["num_pages"] = self.num_pages
         if self.max_tokens is not None:

@@ -90,7 +90,7 @@ class ModelRunner:
                  page_size: int = 16, max_tokens: Optional[int] = None, num_pages: Optional[int] = None,
                  max_seqs: int = 8, max_batch_tokens: int = 2048, max_model_len: Optional[int] = None,
                  kv_fraction: float = 0.85, use_graphs: bool = True, pack_weights: Optional[bool] = None,
-                 poison_freed: bool = False):
+                 poison_freed: bool = False, weights: str = "file"):
         self.device = require_gpu(device)
         self.dtype = DTYPES[dtype]
         self.spec = spec
@@ -109,7 +109,7 @@ class ModelRunner:
             total = torch.cuda.mem_get_info(self.device)[1]
             pack_weights = self.dtype == torch.bfloat16 and free_bytes(self.device) - matrices >= 0.3 * total
         self.pack_weights = bool(pack_weights)
-        build = BuildContext(self.dtype, self.device, spec.max_positions, self.page_size, self.pack_weights)
+        build = BuildContext(self.dtype, self.device, spec.max_positions, self.page_size, self.pack_weights, weights)
         self.model.load(tensors, build)
 
         # cache groups: one per distinct pool that the layers' needs name (for keys and values in pages:

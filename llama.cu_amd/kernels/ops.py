@@ -2737,6 +2737,7 @@ class Mx4:
     scales: torch.Tensor
     k: int
     _filled: bool = False         # both are the front of memory that goes on, with zeros, to a multiple of 256 k
+    _by_pair: Optional[Tuple[torch.Tensor, int]] = None      # the scales as the products in tiles read them, [pairs of 128 k][rows][8], and the version of ``scales`` that they are of
 
     @property
     def shape(self):
@@ -2781,11 +2782,14 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     filled, blocks = -(-k // _MX4_PAIR) * _MX4_PAIR, -(-k // MX4_BLOCK)
     codes = torch.empty((m, filled // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((m, filled // MX4_BLOCK), dtype=torch.uint8, device=x.device)
+    # (rows for the product that streams the weight need no second copy; a weight's is not used, 1 / 136 of what is written)
+    by_pair = torch.empty((filled // _MX4_PAIR, m, 8), dtype=torch.uint8, device=x.device) if m > 16 else None
     if m and k:
-        _check(bind("mx4", "lcu_mx4_quantize", "plilipp")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], m, k, codes.data_ptr(), scales.data_ptr(), raw_stream()), "mx4_quantize")
-    if filled == k:
-        return Mx4(codes, scales, k, True)
-    return Mx4(codes[:, :16 * blocks], scales[:, :blocks], k, True)
+        _check(bind("mx4", "lcu_mx4_quantize", "plilippp")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], m, k, codes.data_ptr(), scales.data_ptr(),
+                                                           None if by_pair is None else by_pair.data_ptr(), raw_stream()), "mx4_quantize")
+    if filled != k:
+        codes, scales = codes[:, :16 * blocks], scales[:, :blocks]
+    return Mx4(codes, scales, k, True, None if by_pair is None else (by_pair, scales._version))
 
 
 def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -2804,6 +2808,8 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
 class PackedMx4:
     """A 4-bit weight ``[n, k]`` in the order in which the products read it (``pack_mx4``)."""
 
+    dtype, is_cuda = torch.uint8, True           # what whoever chooses among products asks of a matrix: none but ``gemm_mx4`` takes this one
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int):
         self.codes, self.scales, self.n, self.k = codes, scales, n, k
         self.pairs = -(-k // _MX4_PAIR)
@@ -2816,10 +2822,13 @@ class PackedMx4:
     def device(self):
         return self.codes.device
 
+    def dim(self) -> int:
+        return 2
+
 
 def pack_mx4(q: Mx4) -> PackedMx4:
     """A quantised weight ``[n, k]`` laid out for ``gemm_mx4``, once: features filled up to tiles of 16 and ``k`` to pairs of 128; a tile's codes of a pair in
-    ``[macro-step][block][feature][16 bytes]``, its scales in ``[feature][macro-step][block]``."""
+    ``[macro-step][block][feature][16 bytes]``, its scales in ``[feature][odd][even / 2]`` of its eight blocks."""
     n, blocks = _mx4_checked(q, "pack_mx4")
     if n < 1 or q.k < 1:
         raise KernelError(f"pack_mx4: a weight of {n} x {q.k} has nothing to multiply")
@@ -2830,7 +2839,7 @@ def pack_mx4(q: Mx4) -> PackedMx4:
     scales = torch.full((tiles * 16, pairs * 8), 127, dtype=torch.uint8, device=q.codes.device)
     scales[:n, :blocks] = q.scales
     codes = codes.view(tiles, 16, pairs, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous().view(-1)
-    scales = scales.view(tiles, 16, pairs, 8).permute(0, 2, 1, 3).contiguous().view(-1)
+    scales = scales.view(tiles, 16, pairs, 4, 2).permute(0, 2, 1, 4, 3).contiguous().view(-1)
     return PackedMx4(codes, scales, n, int(q.k))
 
 
@@ -2911,6 +2920,17 @@ def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
     return best[1:]
 
 
+def _mx4_by_pair(q: Mx4, blocks: int) -> torch.Tensor:
+    """The scales of rows in 4 bits as the products in tiles read them: a step's of all rows together (a row's own lie a line apart, and a load of 32 rows' looked up as
+    many lines as the step's codes did)."""
+    if q._by_pair is not None and q._by_pair[1] == q.scales._version:           # (not where the scales were changed since)
+        return q._by_pair[0]
+    rows, pairs = q.scales.shape[0], -(-blocks // 8)
+    out = torch.zeros((rows, 8 * pairs), dtype=torch.uint8, device=q.scales.device)
+    out[:, :blocks] = q.scales
+    return out.view(rows, pairs, 4, 2).permute(1, 0, 3, 2).contiguous()
+
+
 def mx4_choice(m: int, n: int, k: int, kind: int) -> Tuple[int, int]:
     """Which kernel multiplies ``m`` rows (``kind``: as in mx4_stream.hip) with a 4-bit weight ``[n, k]``: ``(-1, 1)`` the one that streams the weight (up to 64 rows), else the
     shape of the tiles and into how many slices K is cut (mx4_tiles.hip): the one that takes least by the times above."""
@@ -2971,8 +2991,11 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
     steps = w.pairs if four else (-(-k // 128) * 2 if kind == 1 else 12 * w.pairs)
     slices = max(1, min(slices, steps))
     planes = torch.empty(slices * min(m, most) * w.n, dtype=torch.float32, device=device) if slices > 1 else None
+    if four:
+        scales = _mx4_by_pair(x, blocks)
+        xs, lds = scales.data_ptr(), 8 * m
     f = bind("mx4_tiles", "lcu_mx4_tiles", "pliplppipliiiiiip")
     for r in range(0, m, most):
-        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + r * lds if four else None, lds, *weight, out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r),
+        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + 8 * r if four else None, lds, *weight, out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r),
                  w.n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), raw_stream()), "gemm_mx4")
     return out

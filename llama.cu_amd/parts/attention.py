@@ -171,7 +171,7 @@ class Attention(Part):
 
     def _load_general(self, tensors, build: BuildContext) -> None:
         nm, nh, nkv, dh, dv = self.names, self.heads, self.kv_heads, self.head_dim, self.value_dim
-        self.w_in = Weight(fused_rows([tensors[nm[k]] for k in self._in_keys()]), build)
+        self.w_in = Weight(fused_rows([tensors[nm[k]] for k in self._in_keys()]), build, four_bits=True)
         # (values that are the keys are read from the keys' columns of the product: the same numbers, before the norm)
         self.offsets = (0, nh * dh, nh * dh if self.values_are_keys else (nh + nkv) * dh)
         self.g_off = (nh + nkv) * dh + (0 if self.values_are_keys else nkv * dv)
@@ -208,7 +208,7 @@ class Attention(Part):
             else:
                 ops.say_once(f"attention with {nh} heads of {dh} (values {dv}) in {nkv} groups runs on the generic kernel, not on the matrix cores")
         self.output_matrix, self.output_width = w_o.contiguous(), nh * self.stored_value_dim
-        self.w_o = Weight(self.output_matrix, build) if self.own_output else None
+        self.w_o = Weight(self.output_matrix, build, four_bits=True) if self.own_output else None
         self.position.load({}, build)
         if type(self.position).apply is not Part.apply:
             raise ValueError("attention: the general path takes a rotation, a bias inside the scores or no position encoding")
@@ -267,14 +267,14 @@ class Attention(Part):
         if self.padded_dim != self.head_dim and self.position.rotary_tables() is not None:
             raise ValueError(f"attention: head_dim {self.head_dim} is no multiple of 8, which the kernels take only without a rotation")
         if self.shares_kv:
-            self.w_qkv = Weight(self._pad_heads(tensors[nm["q"]], self.heads), build)
+            self.w_qkv = Weight(self._pad_heads(tensors[nm["q"]], self.heads), build, four_bits=True)
         elif self.padded_dim != self.head_dim:
             self.w_qkv = Weight(torch.cat([self._pad_heads(tensors[nm["q"]], self.heads),
-                                           self._pad_heads(tensors[nm["k"]], self.kv_heads), tensors[nm["v"]]]).contiguous(), build)
+                                           self._pad_heads(tensors[nm["k"]], self.kv_heads), tensors[nm["v"]]]).contiguous(), build, four_bits=True)
         else:
             # one matrix with the rows of q, then k, then v: in place where the loader laid them out so
-            self.w_qkv = Weight(fused_rows([tensors[nm["q"]], tensors[nm["k"]], tensors[nm["v"]]]), build)
-        self.w_o = Weight(tensors[nm["o"]], build)
+            self.w_qkv = Weight(fused_rows([tensors[nm["q"]], tensors[nm["k"]], tensors[nm["v"]]]), build, four_bits=True)
+        self.w_o = Weight(tensors[nm["o"]], build, four_bits=True)
         if self.norm_eps is not None:            # the kernel takes the norms' weights in 32-bit
             self.q_norm = self._pad_heads(tensors[nm["q_norm"]].float(), self.heads).contiguous()
             self.k_norm = None if self.shares_kv else self._pad_heads(tensors[nm["k_norm"]].float(), self.kv_heads).contiguous()

@@ -208,6 +208,7 @@ class BuildContext:
     page_size: int
     pack_weights: bool = True        # keep a second copy of bfloat16 matrices in the order the decode kernel streams them (of experts, of both types,
                                      # in the experts' kernels' order; of a bfloat16 shared expert a third, in theirs)
+    weights: str = "file"            # "mx4": matrices that can be are held in microscaled 4-bit numbers (attention's and the dense feed-forward's)
 
 
 @dataclass

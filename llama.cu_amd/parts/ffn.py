@@ -64,16 +64,19 @@ class SwiGLU(Part):
     def load(self, tensors, build: BuildContext) -> None:
         g, u = tensors[self.names["gate"]], tensors[self.names["up"]]
         rows = self.intermediate_size
-        if build.dtype == torch.bfloat16 and g.dtype == u.dtype == torch.bfloat16 and g.is_cuda:
+        four = build.weights == "mx4" and g.is_cuda
+        if not four and build.dtype == torch.bfloat16 and g.dtype == u.dtype == torch.bfloat16 and g.is_cuda:
             rows = self._padded_rows(build.dtype, g.device)
         if rows != self.intermediate_size:
             # the plain copy, which the library multiplies, has rows of zeros behind each half; the
             # copy that the decode kernels stream does not
             plain = fused_rows([g, u], pad_rows_to=rows)
             self.w_gate_up = Weight(plain, build, packed_from=torch.cat([g, u], dim=0) if build.pack_weights else None, halves=True)
+        elif four:
+            self.w_gate_up = Weight(torch.cat([g, u], dim=0), build, four_bits=True)
         else:
             self.w_gate_up = Weight(fused_rows([g, u]), build, halves=True)
-        self.w_down = Weight(tensors[self.names["down"]], build)
+        self.w_down = Weight(tensors[self.names["down"]], build, four_bits=True)
         self.dtype = build.dtype
 
     def takes_scaled_rows(self, n_rows: int) -> bool:
@@ -108,6 +111,11 @@ class SwiGLU(Part):
             if isinstance(h, ScaledRows):
                 raise ops.KernelError("feed-forward: rows that wait for their normalisation go with an activation in the product's epilogue only")
             act = ops.swiglu(linear(h, self.w_gate_up, out_dtype=self.dtype), activation=self.activation)
+        elif self.w_gate_up.four_bits:
+            if self.activation == "silu":
+                act = ops.gemm_mx4(h, self.w_gate_up.plain, out_dtype=self.dtype, swiglu=True)
+            else:
+                act = ops.swiglu(linear(h, self.w_gate_up, out_dtype=self.dtype), activation=self.activation, alpha=self.alpha, limit=self.limit)
         elif isinstance(h, ScaledRows) and mid_swiglu_takes(h.rows.shape[0], self.w_gate_up) and ops.mid_supported(h.rows, self.w_gate_up.plain):
             act = linear_swiglu_mid(h, self.w_gate_up, **self.act)
         elif self.dtype == torch.float32 and (isinstance(h, ScaledRows) or ops.skinny_f32_supported(h, self.w_gate_up.plain, self.dtype)):

@@ -7,6 +7,8 @@ Which routine multiplies is decided here and nowhere else:
   (``ops.tiles_choice``), else to the library's matrix product (hipBLASLt through
   torch, with bfloat16 or, for logits, float32 output), as the reference's engine calls
   its vendor library (llama.cu/src/op/linear.rs:91-118);
+* a matrix that the engine holds in 4 bits (``EngineConfig.weights`` "mx4"): the hand-written products with such a weight, whatever
+  the rows (``ops.gemm_mx4``);
 * all float32 (the true 32-bit path): the hand-written weight-streaming kernel on the
   32-bit matrix instruction, for any number of rows;
 * everything else (mixed types: a weight that its file stores in 32-bit beside
@@ -32,11 +34,17 @@ class Weight:
     (measured on the Llama-3-8B shapes).  The copy doubles the memory of the matrices;
     ``BuildContext.pack_weights`` switches it off."""
 
-    def __init__(self, tensor: torch.Tensor, build=None, packed_from: Optional[torch.Tensor] = None, halves: bool = False):
+    def __init__(self, tensor: torch.Tensor, build=None, packed_from: Optional[torch.Tensor] = None, halves: bool = False, four_bits: bool = False):
         """``packed_from``: the matrix to pack if it is not ``tensor`` (a gate/up matrix whose plain copy
         has rows of zeros for the library's sake, see ``library_friendly_rows``, is packed without them).
         ``halves``: the matrix is two matrices one above the other (gate and up) whose rows a kernel pairs:
-        it is packed only if each half is whole blocks of 16 rows."""
+        it is packed only if each half is whole blocks of 16 rows.
+        ``four_bits``: the matrix may be held in 4 bits if the engine is asked for that (``BuildContext.weights``); ``plain`` is then
+        an ``ops.PackedMx4``, and there is nothing else of it."""
+        self.four_bits = four_bits and getattr(build, "weights", "file") == "mx4" and tensor.is_cuda
+        if self.four_bits:
+            self.plain, self.packed = ops.pack_mx4(ops.mx4_quantize(tensor)), None
+            return
         self.plain = tensor.contiguous()
         want = build is None or getattr(build, "pack_weights", True)
         src = self.plain if packed_from is None else packed_from.contiguous()
@@ -80,6 +88,10 @@ def linear(x: torch.Tensor, weight: Union[torch.Tensor, Weight], out_dtype: Opti
         raise ops.KernelError("linear: operands must be on the GPU (there is no CPU path)")
     weight, packed = _split(weight)
     out_dtype = out.dtype if out is not None else (out_dtype or x.dtype)
+    if isinstance(weight, ops.PackedMx4):
+        if accumulate:
+            return ops.scaled_sum(out, ops.gemm_mx4(x, weight, out_dtype=torch.float32), 1.0)
+        return ops.gemm_mx4(x, weight, out=out, out_dtype=out_dtype)
     all_bf16 = x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16
     if (all_bf16 and packed is not None and packed.shape == weight.shape and not accumulate and x.dim() == 2 and wavek_takes(x, packed)
             and out_dtype in (torch.bfloat16, torch.float32) and (out is None or _plain_rows(out))

@@ -29,9 +29,15 @@ def _splitmix64(x: int) -> int:
     return z ^ (z >> 31)
 
 
-def uniform(seed: int, request: int, index: int) -> float:
-    """A number in [0, 1) with 24 random bits, a pure function of its three keys."""
+# what a number is drawn for: a token; whether a draft stands; the token after the drafts that do
+DRAW, JUDGE, FINAL = 0, 1, 2
+
+
+def uniform(seed: int, request: int, index: int, purpose: int = DRAW) -> float:
+    """A number in [0, 1) with 24 random bits, a pure function of its keys."""
     h = _splitmix64(seed & _MASK)
+    if purpose:
+        h = _splitmix64(h ^ purpose)
     h = _splitmix64(h ^ (request & _MASK))
     h = _splitmix64(h ^ (index & _MASK))
     return (h >> 40) / float(1 << 24)
@@ -225,6 +231,39 @@ def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tenso
 
 
 class Sampler:
+    def probs(self, logits: torch.Tensor, params: Sequence[SamplingParams]) -> torch.Tensor:
+        """Every row's distribution under its options (``token_probs``): what ``sample_device`` draws the row's token from."""
+        if len(params) != logits.shape[0]:
+            raise KernelError(f"probs: {logits.shape[0]} rows with options for {len(params)}")
+        return token_probs(logits, [0.0 if p.is_argmax else p.temperature for p in params], [p.top_p for p in params], [p.top_k for p in params])
+
+    def verify(self, logits: torch.Tensor, drafts: Sequence[Sequence[int]], params: Sequence[SamplingParams], keys: Sequence[Tuple[int, int]],
+               draft_probs: Optional[torch.Tensor] = None) -> List[List[int]]:
+        """The tokens that drafted ones turn into: of request ``i`` its drafts that stand and the token after them, distributed as tokens drawn one
+        after the other from the model's own logits.  ``logits`` (float32): for every request a row for each of its drafts and one more, the
+        requests one after the other; ``draft_probs``: what the drafts were drawn from, a row each (``probs`` of the drafting model's logits;
+        None: they were certain, found in the text or greedy); ``keys[i] = (request id, index of its first drafted token)``.  Whether drafts stand
+        is judged by numbers of their own, not by those that ``sample`` draws tokens with."""
+        if not (len(drafts) == len(params) == len(keys)):
+            raise KernelError("verify: drafts, options and keys, one of each a request")
+        counts = [len(d) for d in drafts]
+        if logits.dim() != 2 or logits.shape[0] != sum(counts) + len(drafts):
+            raise KernelError(f"verify: {sum(counts)} drafts of {len(drafts)} requests need {sum(counts) + len(drafts)} rows of logits, got {tuple(logits.shape)}")
+        if not drafts:
+            return []
+        probs = self.probs(logits, [p for p, c in zip(params, counts) for _ in range(c + 1)])
+        starts, flat, judge, final = [0], [], [], []
+        for d, p, (request, index) in zip(drafts, params, keys):
+            starts.append(starts[-1] + len(d) + 1)
+            flat += [int(t) for t in d]
+            judge += [uniform(p.seed, request, index + j, JUDGE) for j in range(len(d))]
+            final.append(uniform(p.seed, request, index, FINAL))
+        dev = logits.device
+        ints, floats = _to_device(starts + flat, torch.int32, dev), _to_device(judge + final, torch.float32, dev)
+        accepted, tokens = verify_drafts(probs, ints[:len(starts)], ints[len(starts):], floats[:len(flat)], floats[len(flat):], max(counts), draft_probs)
+        both = torch.cat([accepted.unsqueeze(1), tokens], dim=1).tolist()
+        return [row[1:row[0] + 2] for row in both]
+
     def sample_device(self, logits: torch.Tensor, params: Sequence[SamplingParams],
                       keys: Sequence[Tuple[int, int]]) -> torch.Tensor:
         """A token for every row, left on the device (int32)."""

@@ -241,6 +241,21 @@ def test_rows_in_4_bits_of_other_memory():
     assert torch.equal(again.codes, there.codes) and torch.equal(again.scales, there.scales)
 
 
+def test_rows_in_4_bits_that_were_changed():
+    """What the scales are when the product is called counts, however many rows there are."""
+    from llama_cu_amd.kernels import ops
+    n, k = 64, 288
+    w, exact = weight(n, k)
+    for m in (4, 40, 200):
+        q = ops.mx4_quantize(rnd(m, k, seed=m).bfloat16().cuda())
+        before = ops.gemm_mx4(q, w, out_dtype=torch.float32)
+        q.scales.add_(1)
+        assert torch.equal(ops.gemm_mx4(q, w, out_dtype=torch.float32), 2 * before)
+        q.scales[m // 2] = 255
+        after = ops.gemm_mx4(q, w, out_dtype=torch.float32)
+        assert torch.isnan(after[m // 2]).all() and torch.equal(after[:m // 2], 2 * before[:m // 2]) and torch.equal(after[m // 2 + 1:], 2 * before[m // 2 + 1:])
+
+
 def test_infinities_of_32_bit_rows():
     from llama_cu_amd.kernels import ops
     w, exact = weight(32, 128)
