@@ -98,11 +98,11 @@ mx4_stream_kernel(const bf16_t *__restrict__ X, int ldx, int plane, Mx4Args a) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[n][m] = mx4_f32x4{0.f, 0.f, 0.f, 0.f};
     mx4_u32x4 code[AHEAD][NT][2], b[MT * PLANES][LOADS];
-    uint2 scale[AHEAD][NT];
+    uint32_t scale[AHEAD][NT];                       // of the lane's odd or even blocks
     auto fetch_w = [&](int u, int p) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            scale[u][n] = *(const uint2 *)(ws[n] + (size_t)p * MX4_PAIR_SCALES);
+            scale[u][n] = *(const uint32_t *)(ws[n] + (size_t)p * MX4_PAIR_SCALES + 4 * (g & 1));
 #pragma unroll
             for (int h = 0; h < 2; ++h) code[u][n][h] = __builtin_nontemporal_load((const mx4_u32x4 *)(wc[n] + (size_t)p * MX4_PAIR_CODES + 1024 * h));
         }
@@ -127,7 +127,7 @@ mx4_stream_kernel(const bf16_t *__restrict__ X, int ldx, int plane, Mx4Args a) {
         mx4_u32x4 w[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float sc = mx4_scale(((g & 1 ? scale[u][n].y : scale[u][n].x) >> 8 * (2 * h + (g >> 1))) & 255u);      // block 4 h + g
+            const float sc = mx4_scale((scale[u][n] >> 8 * (2 * h + (g >> 1))) & 255u);      // block 4 h + g
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[n][j] = mx4_to_bf16(code[u][n][h][j], sc);
         }
@@ -252,6 +252,9 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
     const Mx4Args a = {(const uint8_t *)codes, (const uint8_t *)scales, pairs, macros, y, ldy, M, N, ((uintptr_t)y | (uintptr_t)(ldy * elem)) % (4 * elem) == 0};
     const int tiles = (cols + 15) / 16, waves = min(MX4_WAVES, x_kind == 4 ? macros : (macros + 1) / 2);
     const dim3 block(waves * WAVE);
+    // two tiles of features a workgroup where there are many, and more than four rows are read for them (us, one tile / two: 16384 x 2048 16 rows 10.8 / 9.5, 28672 x 4096 16 rows 26.1 / 24.9,
+    // 128256 x 4096 8 rows 70.6 / 65.1; one row 58.9 / 59.7; 4096 x 14336 8 rows 13.1 / 15.6)
+    const bool pairs_of = x_kind == 1 && M > 4 && M <= 16 && N > 8192 && epi < MX4_EPI_SWIGLU;
     auto grid = [&](int nt, int mt) { return dim3(epi >= MX4_EPI_SWIGLU ? tiles : (tiles + nt - 1) / nt, (M + 16 * mt - 1) / (16 * mt)); };
     if ((M + 15) / 16 > 65535) return LCU_BAD_ARGUMENT;
 #define GO(NT, MT, PLANES, EPI, LOADS) mx4_stream_kernel<NT, MT, PLANES, EPI, LOADS><<<grid(NT, MT), block, 0, stream>>>((const bf16_t *)x, (int)ldx, (int)(PLANES == 3 ? ldx / 3 : 0), a)
@@ -265,7 +268,7 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
         } else if (x_kind == 3) {                          \
             if (M <= 4) GO(NT, 1, 3, EPI, 1);              \
             else if (M <= 16) GO(NT, 1, 3, EPI, 4);        \
-            else GO(NT, 2, 3, EPI, 4);                     \
+            else GO(NT, NT == 1 ? 2 : 1, 3, EPI, 4);       \
         } else {                                           \
             if (M <= 4) GO(NT, 1, 1, EPI, 1);              \
             else if (M <= 8) GO(NT, 1, 1, EPI, 2);         \
@@ -276,6 +279,7 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
     } while (0)
     if (epi == MX4_EPI_SWIGLU) ROWS(2, MX4_EPI_SWIGLU);
     else if (epi == MX4_EPI_SWIGLU_F32) ROWS(2, MX4_EPI_SWIGLU_F32);
+    else if (pairs_of) { if (epi == MX4_EPI_BF16) ROWS(2, MX4_EPI_BF16); else ROWS(2, MX4_EPI_F32); }
     else if (epi == MX4_EPI_BF16) ROWS(1, MX4_EPI_BF16);
     else ROWS(1, MX4_EPI_F32);
 #undef GO

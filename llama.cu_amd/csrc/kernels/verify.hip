@@ -98,12 +98,35 @@ vf_sum_kernel(const float *__restrict__ p, size_t ldp, int rows, const int *__re
     const VfLeft left = vf_left(run, p, ldp, drafts, q, ldq);
     const int each = (vocab + parts - 1) / parts, part0 = blockIdx.y * PARTS;
     double mine[PARTS], own[PARTS];
+    if (each <= 4 * VF_THREADS) {                      // all of a workgroup's loads on their way at once; what they bring is not wanted again, but for one part
+        float pv[PARTS][4], qv[PARTS][4];
 #pragma unroll
-    for (int n = 0; n < PARTS; ++n) {
-        const int lo = min(vocab, (part0 + n) * each), hi = part0 + n < parts ? min(vocab, lo + each) : lo;
-        mine[n] = own[n] = 0.0;
+        for (int n = 0; n < PARTS; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int lo = min(vocab, (part0 + n) * each), hi = part0 + n < parts ? min(vocab, lo + each) : lo, i = lo + j * VF_THREADS + (int)threadIdx.x;
+                pv[n][j] = i < hi ? __builtin_nontemporal_load(left.p + i) : 0.f;
+                qv[n][j] = i < hi && left.q ? __builtin_nontemporal_load(left.q + i) : 0.f;
+            }
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
+            mine[n] = own[n] = 0.0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int lo = min(vocab, (part0 + n) * each), i = lo + j * VF_THREADS + (int)threadIdx.x;
+                const double v = vf_clean(pv[n][j]);
+                own[n] += v;
+                if (i != left.without) mine[n] += fmax(v - (double)vf_clean(qv[n][j]), 0.0);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < PARTS; ++n) {
+            const int lo = min(vocab, (part0 + n) * each), hi = part0 + n < parts ? min(vocab, lo + each) : lo;
+            mine[n] = own[n] = 0.0;
 #pragma unroll 4
-        for (int i = lo + threadIdx.x; i < hi; i += VF_THREADS) { mine[n] += left(i); own[n] += vf_clean(left.p[i]); }
+            for (int i = lo + threadIdx.x; i < hi; i += VF_THREADS) { mine[n] += left(i); own[n] += vf_clean(left.p[i]); }
+        }
     }
 #pragma unroll
     for (int n = 0; n < PARTS; ++n) {

@@ -2875,13 +2875,14 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
 # Tiles (features, tokens) by whether the rows are in 4 bits and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three workgroups
 # on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
 _MX4_TILES = {
-    (False, 0): (128, 128, 2, 3.56, 2.33, (0.45, 0.71, 0.95), 2.54, 0.24),
-    (False, 1): (256, 256, 1, 4.07, 5.26, (1.09,), 3.05, 0.17),
-    (False, 2): (128, 64, 3, 4.71, 0.01, (0.40, 0.54, 0.65), 2.44, 0.29),
-    (True, 0): (128, 128, 1, 2.19, 3.10, (0.77,), 2.40, 0.21),
-    (True, 1): (256, 256, 1, 2.69, 6.13, (1.51,), 3.59, 0.15),
-    (True, 2): (128, 64, 2, 2.93, 1.25, (0.62, 1.11), 2.52, 0.25),
-    (True, 3): (128, 256, 1, 2.00, 3.82, (1.00,), 3.40, 0.16),
+    (False, 0): (128, 128, 2, 4.78, 1.66, (0.43, 0.74), 2.47, 0.21),
+    (False, 1): (256, 256, 1, 2.10, 6.99, (1.09,), 3.54, 0.15),
+    (False, 2): (128, 64, 3, 4.43, 0.45, (0.38, 0.53, 0.69), 2.78, 0.26),
+    (False, 3): (256, 128, 2, 5.14, 3.31, (0.64, 1.34), 4.49, 0.14),
+    (True, 0): (128, 128, 1, 1.62, 3.72, (0.70,), 2.72, 0.17),
+    (True, 1): (256, 256, 1, 2.32, 10.59, (1.25,), 3.44, 0.12),
+    (True, 2): (128, 64, 2, 2.60, 1.82, (0.56, 1.01), 2.62, 0.22),
+    (True, 3): (128, 256, 1, 1.37, 4.71, (0.88,), 3.37, 0.15),
 }
 # The kernel that streams the weight, by the kind of the rows: us a launch; a workgroup alone, and for each macro-step of a wave; a macro-step where workgroups share a compute unit, and what four
 # rows add to that.
