@@ -137,6 +137,40 @@ static uint32_t mx4_units(long long rows, long long row_units) {
     return units > 0 && units < 1ll << 31 ? (uint32_t)units : 0u;
 }
 
+// Scales [rows, lds], whole pairs of macro-steps, as the products in tiles read them: [pairs][rows][8].
+__global__ void __launch_bounds__(MX4_THREADS)
+mx4_by_pair_kernel(const uint8_t *__restrict__ scales, size_t lds, size_t rows, int pairs, uint8_t *__restrict__ out) {
+    const size_t row = (size_t)blockIdx.x * MX4_THREADS + threadIdx.x;
+    if (row >= rows) return;
+    for (int p = blockIdx.y; p < pairs; p += gridDim.y) {
+        uint8_t s[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) s[mx4_scale_place(b)] = scales[row * lds + 8 * p + b];
+        uint64_t all = 0;
+#pragma unroll
+        for (int b = 0; b < 8; ++b) all |= (uint64_t)s[b] << 8 * b;
+        *(uint64_t *)(out + ((size_t)p * rows + row) * 8) = all;
+    }
+}
+
+// The number of the capture into a graph that a stream is in, 0: none.
+LCU_API int lcu_capture_id(hipStream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (stream && hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) (void)hipGetLastError();
+    return status == hipStreamCaptureStatusNone ? 0 : (int)(id % 0x7fffffff) + 1;
+}
+
+// scales: [rows, lds] bytes, 8 pairs of them in every row; out: [pairs][rows][8], 8-byte aligned.
+LCU_API int lcu_mx4_by_pair(const void *scales, long long lds, long long rows, int pairs, void *out, hipStream_t stream) {
+    if (rows <= 0 || pairs <= 0) return LCU_OK;
+    const long long groups = (rows + MX4_THREADS - 1) / MX4_THREADS;
+    if (!scales || !out || (uintptr_t)out % 8 || (rows > 1 && lds < 8 * (long long)pairs) || groups > 0x7fffffff) return LCU_BAD_ARGUMENT;
+    mx4_by_pair_kernel<<<dim3((unsigned)groups, (unsigned)min(pairs, 256)), dim3(MX4_THREADS), 0, stream>>>((const uint8_t *)scales, (size_t)lds, (size_t)rows, pairs, (uint8_t *)out);
+    LCU_LAUNCH_CHECK();
+    return LCU_OK;
+}
+
 // x: [rows, ldx] of `type`; codes: [rows][kp / 2], scales: [rows][kp / 32] with kp = k rounded up to 256, codes 4-byte aligned; by_pair: null, or the scales once more as the products in
 // tiles read them, [kp / 256][rows][8], a row's eight as in mx4.h.
 LCU_API int lcu_mx4_quantize(const void *x, long long ldx, int type, long long rows, int k, void *codes, void *scales, void *by_pair, hipStream_t stream) {

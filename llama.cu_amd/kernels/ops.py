@@ -69,6 +69,28 @@ def on_current_device(device: torch.device, what: str) -> None:
         raise KernelError(f"{what}: the operands are on {device}, the current device is cuda:{current}")
 
 
+def here(what: str, first: torch.Tensor, *more: Optional[torch.Tensor]) -> None:
+    """Refuses operands that are not all on the current device."""
+    at = first.get_device()
+    for t in more:
+        if t is not None and t.get_device() != at:
+            break
+    else:
+        if at >= 0 and at == torch._C._cuda_getDevice():
+            return
+    _gpu(first, *more)
+    on_current_device(first.device, what)
+
+
+def apart(what: str, out: torch.Tensor, *read: Optional[torch.Tensor]) -> None:
+    """Refuses a result over what is still read for it (rows, or vectors: from the first byte of each to its last)."""
+    lo = out.data_ptr()
+    hi = lo + ((out.shape[0] - 1) * out.stride(0) + out.shape[-1]) * out.element_size()
+    for t in read:
+        if t is not None and t.data_ptr() < hi and lo < t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[-1]) * t.element_size() and t.numel():
+            raise KernelError(f"{what}: out lies over an operand")
+
+
 _LETTERS = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int}
 _bound: Dict = {}
 
@@ -2728,39 +2750,51 @@ MX4_BLOCK = 32            # numbers along k that share a scale
 _MX4_PAIR = 256           # k that the products' order is filled up to
 
 
-@dataclass
 class Mx4:
     """Rows of microscaled 4-bit numbers (the MXFP4 format): ``codes`` (uint8 ``[rows, 16 * blocks]``, two a byte, the first in the low half: a sign
     and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6) times ``2 ** (scales - 127)`` (uint8 ``[rows, blocks]``, 255: not a number), 32 neighbours of the
-    ``k`` numbers of a row to a block; codes behind ``k`` are zero."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    k: int
-    _filled: bool = False         # both are the front of memory that goes on, with zeros, to a multiple of 256 k
-    _by_pair: Optional[Tuple[torch.Tensor, int]] = None      # the scales as the products in tiles read them, [pairs of 128 k][rows][8], and the version of ``scales`` that they are of
+    ``k`` numbers of a row to a block; codes behind ``k`` are zero.  The tensors may be written to, not replaced."""
+
+    __slots__ = ("_codes", "_scales", "_k", "_filled", "_by_pair", "_of")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
+        self._codes, self._scales, self._k = codes, scales, int(k)
+        self._filled = False              # (mx4_quantize:) both are the front of memory that goes on, with zeros, to a multiple of 256 k
+        self._by_pair = self._of = None   # the scales as the products in tiles read them, and the state of `scales` that they are of
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    k = property(lambda self: self._k)
 
     @property
     def shape(self):
-        return torch.Size((self.codes.shape[0], self.k))
+        return torch.Size((self._codes.shape[0], self._k))
+
+    def __repr__(self):
+        return f"Mx4({self._codes.shape[0]} x {self._k}, {self._codes.device})"
+
+    def __getstate__(self):               # (a copy's memory may end with its rows)
+        return self._codes, self._scales, self._k
+
+    def __setstate__(self, state):
+        self.__init__(*state)
 
 
 def _mx4_checked(q: Mx4, what: str) -> Tuple[int, int]:
     """``(rows, blocks)`` of a well-formed Mx4."""
     if not isinstance(q, Mx4):
         raise KernelError(f"{what}: need an Mx4 (mx4_quantize), got {type(q).__name__}")
-    blocks = -(-int(q.k) // MX4_BLOCK)
-    if q.k < 0 or q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or q.codes.dim() != 2 or q.scales.dim() != 2 \
-            or q.codes.shape[1] != 16 * blocks or q.scales.shape != (q.codes.shape[0], blocks):
-        raise KernelError(f"{what}: codes {q.codes.dtype} {tuple(q.codes.shape)} and scales {q.scales.dtype} {tuple(q.scales.shape)} are not those of rows of {q.k} numbers")
-    for t, name in ((q.codes, "codes"), (q.scales, "scales")):
+    codes, scales, k = q._codes, q._scales, q._k
+    blocks = -(-k // MX4_BLOCK)
+    if q._filled:                         # (made so)
+        return codes.shape[0], blocks
+    if k < 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 \
+            or codes.shape[1] != 16 * blocks or scales.shape != (codes.shape[0], blocks):
+        raise KernelError(f"{what}: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not those of rows of {k} numbers")
+    for t, name in ((codes, "codes"), (scales, "scales")):
         if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
             raise KernelError(f"{what}: the {name}' rows must be contiguous and apart, got strides {t.stride()}")
-    return q.codes.shape[0], blocks
-
-
-def _mx4_here(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    _gpu(*tensors)
-    on_current_device(next(t for t in tensors if t is not None).device, what)
+    return codes.shape[0], blocks
 
 
 def _mx4_source(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -2768,10 +2802,18 @@ def _mx4_source(x: torch.Tensor, what: str) -> torch.Tensor:
     _type(x, what)
     if x.dim() != 2:
         raise KernelError(f"{what}: need rows [m, k], got shape {tuple(x.shape)}")
-    _mx4_here(what, x)
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    here(what, x)
+    if x.stride(1) != 1 and x.shape[1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()
     return x
+
+
+def _mx4_state(scales: torch.Tensor, stream: int) -> Optional[Tuple[int, int]]:
+    """What tells whether scales were written to since, or are to be in the replays of a graph: the tensor's version and the number of the capture that is under way
+    (None: the tensor counts no versions)."""
+    if scales.is_inference():
+        return None
+    return scales._version, bind("mx4", "lcu_capture_id", "")(stream)
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4:
@@ -2779,17 +2821,21 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     number goes to the nearest code, ties to the even one, and beyond 6 scales to 6.  A block that holds an infinity or a NaN becomes NaN."""
     x = _mx4_source(x, "mx4_quantize")
     m, k = x.shape
-    filled, blocks = -(-k // _MX4_PAIR) * _MX4_PAIR, -(-k // MX4_BLOCK)
-    codes = torch.empty((m, filled // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((m, filled // MX4_BLOCK), dtype=torch.uint8, device=x.device)
+    pairs, blocks, device, stream = -(-k // _MX4_PAIR), -(-k // MX4_BLOCK), x.device, raw_stream()
+    codes = torch.empty_strided((m, 128 * pairs), (128 * pairs, 1), dtype=torch.uint8, device=device)
+    scales = torch.empty_strided((m, 8 * pairs), (8 * pairs, 1), dtype=torch.uint8, device=device)
     # (rows for the product that streams the weight need no second copy; a weight's is not used, 1 / 136 of what is written)
-    by_pair = torch.empty((filled // _MX4_PAIR, m, 8), dtype=torch.uint8, device=x.device) if m > 16 else None
+    by_pair = torch.empty_strided((pairs, m, 8), (8 * m, 8, 1), dtype=torch.uint8, device=device) if m > 16 and not scales.is_inference() else None
     if m and k:
         _check(bind("mx4", "lcu_mx4_quantize", "plilippp")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], m, k, codes.data_ptr(), scales.data_ptr(),
-                                                           None if by_pair is None else by_pair.data_ptr(), raw_stream()), "mx4_quantize")
-    if filled != k:
-        codes, scales = codes[:, :16 * blocks], scales[:, :blocks]
-    return Mx4(codes, scales, k, True, None if by_pair is None else (by_pair, scales._version))
+                                                           None if by_pair is None else by_pair.data_ptr(), stream), "mx4_quantize")
+    if blocks % 8:
+        codes, scales = codes.as_strided((m, 16 * blocks), (128 * pairs, 1)), scales.as_strided((m, blocks), (8 * pairs, 1))
+    q = Mx4(codes, scales, k)
+    q._filled = True
+    if by_pair is not None:
+        q._by_pair, q._of = by_pair, _mx4_state(scales, stream)
+    return q
 
 
 def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -2797,10 +2843,11 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     m, _ = _mx4_checked(q, "mx4_values")
     if out_dtype not in _TYPE:
         raise KernelError(f"mx4_values: type {out_dtype} is not supported (float32 or bfloat16)")
-    _mx4_here("mx4_values", q.codes, q.scales)
-    out = torch.empty((m, q.k), dtype=out_dtype, device=q.codes.device)
-    if m and q.k:
-        _check(bind("mx4", "lcu_mx4_values", "plpllipli")(q.codes.data_ptr(), q.codes.stride(0), q.scales.data_ptr(), q.scales.stride(0), m, q.k, out.data_ptr(), q.k,
+    codes, scales, k = q._codes, q._scales, q._k
+    here("mx4_values", codes, scales)
+    out = torch.empty_strided((m, k), (k, 1), dtype=out_dtype, device=codes.device)
+    if m and k:
+        _check(bind("mx4", "lcu_mx4_values", "plpllipli")(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), m, k, out.data_ptr(), k,
                                                           _TYPE[out_dtype], raw_stream()), "mx4_values")
     return out
 
@@ -2813,6 +2860,10 @@ class PackedMx4:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int):
         self.codes, self.scales, self.n, self.k = codes, scales, n, k
         self.pairs = -(-k // _MX4_PAIR)
+        size = -(-n // 16) * self.pairs * 2048
+        if n < 1 or k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.shape != (size,) or scales.shape != (size // 16,) \
+                or not codes.is_contiguous() or not scales.is_contiguous():
+            raise KernelError(f"PackedMx4: a weight of {n} x {k} has {size} bytes of codes and {size // 16} scales, got {codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
 
     @property
     def shape(self):
@@ -2832,10 +2883,13 @@ def pack_mx4(q: Mx4) -> PackedMx4:
     n, blocks = _mx4_checked(q, "pack_mx4")
     if n < 1 or q.k < 1:
         raise KernelError(f"pack_mx4: a weight of {n} x {q.k} has nothing to multiply")
-    _mx4_here("pack_mx4", q.codes, q.scales)
+    here("pack_mx4", q.codes, q.scales)
     tiles, pairs = -(-n // 16), -(-q.k // _MX4_PAIR)
     codes = torch.zeros((tiles * 16, pairs * 128), dtype=torch.uint8, device=q.codes.device)
     codes[:n, :16 * blocks] = q.codes
+    codes[:, (q.k + 1) // 2:] = 0              # (whatever they came with: zeros behind k make the rows' own numbers there not matter)
+    if q.k % 2:
+        codes[:, q.k // 2] &= 15
     scales = torch.full((tiles * 16, pairs * 8), 127, dtype=torch.uint8, device=q.codes.device)
     scales[:n, :blocks] = q.scales
     codes = codes.view(tiles, 16, pairs, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous().view(-1)
@@ -2858,7 +2912,9 @@ def _mx4_rows(x: torch.Tensor, k: int) -> Tuple[torch.Tensor, int]:
 
 def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     """Rows in 4 bits as the products read them: whole pairs of macro-steps, rows on 16 bytes, scales on 8."""
-    fits = (q._filled or blocks % 8 == 0) and q.codes.data_ptr() % 16 == 0 and q.scales.data_ptr() % 8 == 0 \
+    if q._filled and q._codes.stride(0) < 1 << 24:
+        return q
+    fits = blocks % 8 == 0 and q.codes.data_ptr() % 16 == 0 and q.scales.data_ptr() % 8 == 0 \
         and (q.codes.shape[0] == 1 or (q.codes.stride(0) % 16 == 0 and q.codes.stride(0) < 1 << 24 and q.scales.stride(0) % 8 == 0 and q.scales.stride(0) < 1 << 24))
     if fits:
         return q
@@ -2867,7 +2923,7 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     scales = torch.zeros((q.codes.shape[0], whole), dtype=torch.uint8, device=q.codes.device)
     codes[:, :16 * blocks] = q.codes
     scales[:, :blocks] = q.scales
-    return Mx4(codes[:, :16 * blocks], scales[:, :blocks], q.k, True)
+    return Mx4(codes, scales, 32 * whole)
 
 
 # What the kernels of the 4-bit products take, us, fitted to 12,000 timed products of 12 to 3,200 rows and 9,500 of 1 to 96 (64 to 128,256 features, K 128 to 28,672;
@@ -2921,15 +2977,16 @@ def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
     return best[1:]
 
 
-def _mx4_by_pair(q: Mx4, blocks: int) -> torch.Tensor:
-    """The scales of rows in 4 bits as the products in tiles read them: a step's of all rows together (a row's own lie a line apart, and a load of 32 rows' looked up as
-    many lines as the step's codes did)."""
-    if q._by_pair is not None and q._by_pair[1] == q.scales._version:           # (not where the scales were changed since)
-        return q._by_pair[0]
-    rows, pairs = q.scales.shape[0], -(-blocks // 8)
-    out = torch.zeros((rows, 8 * pairs), dtype=torch.uint8, device=q.scales.device)
-    out[:, :blocks] = q.scales
-    return out.view(rows, pairs, 4, 2).permute(1, 0, 3, 2).contiguous()
+def _mx4_by_pair(q: Mx4, blocks: int, stream: int) -> torch.Tensor:
+    """The scales of rows in 4 bits (``_mx4_whole``) as the products in tiles read them: a pair of macro-steps' of all rows together (a row's own lie a line apart, and a load
+    of 32 rows' looked up as many lines as the step's codes did)."""
+    scales = q._scales
+    if q._by_pair is not None and q._of == _mx4_state(scales, stream):
+        return q._by_pair
+    rows, pairs = scales.shape[0], -(-blocks // 8)
+    out = torch.empty_strided((pairs, rows, 8), (8 * rows, 8, 1), dtype=torch.uint8, device=scales.device)
+    _check(bind("mx4", "lcu_mx4_by_pair", "pllip")(scales.data_ptr(), scales.stride(0), rows, pairs, out.data_ptr(), stream), "gemm_mx4 scales")
+    return out
 
 
 def mx4_choice(m: int, n: int, k: int, kind: int) -> Tuple[int, int]:
@@ -2948,55 +3005,61 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
     four = isinstance(x, Mx4)
     if four:
         m, blocks = _mx4_checked(x, "gemm_mx4 x")
-        k, device = x.k, x.codes.device
+        k, first, of_rows = x._k, x._codes, x._scales
     else:
         _type(x, "gemm_mx4 x")
         if x.dim() != 2:
             raise KernelError(f"gemm_mx4: need rows [m, k], got shape {tuple(x.shape)}")
-        (m, k), device = x.shape, x.device
+        (m, k), first, of_rows = x.shape, x, None
+    n = w.n
     if k != w.k:
         raise KernelError(f"gemm_mx4: rows of {k} numbers with a weight of {w.k}")
-    if swiglu and w.n % 2:
-        raise KernelError(f"gemm_mx4: {w.n} features are not as many gate as up rows")
-    cols = w.n // 2 if swiglu else w.n
+    if swiglu and n % 2:
+        raise KernelError(f"gemm_mx4: {n} features are not as many gate as up rows")
+    cols = n // 2 if swiglu else n
     dtype = out.dtype if out is not None else out_dtype or (torch.bfloat16 if four else x.dtype)
     if dtype not in _TYPE or (out is not None and out_dtype not in (None, dtype)):
         raise KernelError(f"gemm_mx4 out: type {dtype} is not supported (float32 or bfloat16, that of out)")
-    _mx4_here("gemm_mx4", x.codes if four else x, x.scales if four else None, w.codes, out)
+    here("gemm_mx4", first, w.codes, of_rows, out)
+    device = first.device
     if out is None:
-        out = torch.empty((m, cols), dtype=dtype, device=device)
-    elif out.shape != (m, cols) or (cols > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < cols):
-        raise KernelError(f"gemm_mx4 out: need {(m, cols)} with contiguous rows apart, got {tuple(out.shape)} with strides {out.stride()}")
+        out = torch.empty_strided((m, cols), (cols, 1), dtype=dtype, device=device)
+    else:
+        if out.shape != (m, cols) or (cols > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < cols):
+            raise KernelError(f"gemm_mx4 out: need {(m, cols)} with contiguous rows apart, got {tuple(out.shape)} with strides {out.stride()}")
+        apart("gemm_mx4", out, first, of_rows)
     if m == 0:
         return out
+    stream = raw_stream()
     if four:
         q = _mx4_whole(x, blocks)
-        rows, kind, ld, scales, lds = q.codes, 4, q.codes.stride(0), q.scales, q.scales.stride(0)
+        rows, kind, scales = q._codes, 4, q._scales
+        ld, lds, xs = rows.stride(0), scales.stride(0), scales.data_ptr()
+        if m == 1:                         # (the one row's stride says nothing)
+            ld, lds = 128 * w.pairs, 8 * w.pairs
+        row_bytes = ld
     else:
         rows, kind = _mx4_rows(x, k)
-        ld, scales, lds = rows.stride(0), None, 0
-    if m == 1:                             # (the one row's stride says nothing)
-        ld, lds = (128 * w.pairs, 8 * w.pairs) if four else (rows.shape[1], 0)
-    shape, slices = mx4_choice(m, w.n, k, kind)
-    row_bytes = ld if four else 2 * ld
+        ld, lds, xs = rows.stride(0) if m > 1 else rows.shape[1], 0, None
+        row_bytes = 2 * ld
+    shape, slices = _mx4_choice(m, n, k, kind, TUNING.compute_units)
     most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
-    if shape >= 0 and (most < 512 or (w.n + 528) * w.pairs * 128 >= 1 << 32):
+    if shape >= 0 and (most < 512 or (n + 528) * w.pairs * 128 >= 1 << 32):
         shape = -1
     of_out = out.stride(0) if m > 1 else cols
     epilogue = (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0)
-    xs = scales.data_ptr() if four else None
-    weight = (w.codes.data_ptr(), w.scales.data_ptr(), w.pairs)
     if shape < 0:
-        _check(bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")(rows.data_ptr(), ld, kind, xs, lds, *weight, out.data_ptr(), of_out, m, w.n, k, epilogue, raw_stream()), "gemm_mx4")
+        _check(bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")(rows.data_ptr(), ld, kind, xs, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs, out.data_ptr(), of_out, m, n, k,
+                                                                      epilogue, stream), "gemm_mx4")
         return out
     steps = w.pairs if four else (-(-k // 128) * 2 if kind == 1 else 12 * w.pairs)
     slices = max(1, min(slices, steps))
-    planes = torch.empty(slices * min(m, most) * w.n, dtype=torch.float32, device=device) if slices > 1 else None
+    planes = torch.empty_strided((slices * min(m, most) * n,), (1,), dtype=torch.float32, device=device) if slices > 1 else None
     if four:
-        scales = _mx4_by_pair(x, blocks)
+        scales = _mx4_by_pair(q, blocks, stream)
         xs, lds = scales.data_ptr(), 8 * m
     f = bind("mx4_tiles", "lcu_mx4_tiles", "pliplppipliiiiiip")
     for r in range(0, m, most):
-        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + 8 * r if four else None, lds, *weight, out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r),
-                 w.n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), raw_stream()), "gemm_mx4")
+        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + 8 * r if four else None, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs,
+                 out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r), n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), stream), "gemm_mx4")
     return out

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -115,6 +116,13 @@ def _options(values, dtype: torch.dtype, rows: int, device, what: str, fine, why
     return values
 
 
+@functools.lru_cache(maxsize=1024)
+def _probs_scratch(rows: int, vocab: int, parts: int, cuts: bool) -> int:
+    size = build.load("token_probs").lcu_token_probs_scratch_bytes
+    size.restype = ctypes.c_size_t
+    return size(rows, vocab, parts, int(cuts))
+
+
 def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The distribution that ``sample_rows`` draws each row's token from, float32 ``[rows, vocab]``: with the logits in descending order
     (equal ones by index), weights ``w_i = exp((l_i - l_0) / T)`` and sums ``c`` of them, entry ``i`` has the share
@@ -134,15 +142,16 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda low, high, total: low > 0 and total == total, "> 0")
     top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, high, total: low >= 1, ">= 1")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
-    elif out.shape != (rows, vocab) or out.dtype != torch.float32 or not out.is_contiguous():
-        raise KernelError(f"token_probs out: must be contiguous float32 {(rows, vocab)}, got {out.dtype} {tuple(out.shape)}")
-    _gpu(logits, out)
-    ops.on_current_device(dev, "token_probs")
+        out = torch.empty_strided((rows, vocab), (vocab, 1), dtype=torch.float32, device=dev)
+    else:
+        if out.shape != (rows, vocab) or out.dtype != torch.float32 or not out.is_contiguous():
+            raise KernelError(f"token_probs out: must be contiguous float32 {(rows, vocab)}, got {out.dtype} {tuple(out.shape)}")
+        ops.apart("token_probs", out, logits, *[v for v in (temperature, top_p, top_k) if isinstance(v, torch.Tensor)])
+    ops.here("token_probs", logits, out)
     if rows == 0:
         return out
     # whether some row is cut: known of sequences, taken as given of tensors
-    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or rows and (min(top_p) < 1 or min(top_k) < vocab)
+    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or min(top_p) < 1 or min(top_k) < vocab
     sequences = [None if isinstance(v, torch.Tensor) else array.array("f" if i < 2 else "i", v if i < 2 else [int(k) if k < vocab else vocab for k in v])
                  for i, v in enumerate((temperature, top_p, top_k))]
     at = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, top_k)]
@@ -164,10 +173,8 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
                     at[i], place = place, place + 4 * rows
     # a long row is cut into parts of 4,096 logits at least, one workgroup each, up to about four workgroups a compute unit in all
     parts = max(1, min(32, 4 * ops.TUNING.compute_units // rows, vocab // 4096))
-    size = build.load("token_probs").lcu_token_probs_scratch_bytes
-    size.restype = ctypes.c_size_t
-    size = size(rows, vocab, parts, int(cuts))
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    size = _probs_scratch(rows, vocab, parts, cuts)
+    scratch = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=dev) if size else None
     _check(ops.bind("token_probs", "lcu_token_probs", "pliipppppiip")(logits.data_ptr(), logits.stride(0), rows, vocab, *at, given, out.data_ptr(), parts, int(cuts),
                                                                      None if scratch is None else scratch.data_ptr(), ops.raw_stream()), "token_probs")
     return out
@@ -213,16 +220,15 @@ def verify_drafts(probs: torch.Tensor, starts: torch.Tensor, drafts: torch.Tenso
         raise KernelError(f"verify_drafts: max_drafts {max_drafts} is not supported (0 to {MAX_DRAFTS})")
     if not 0 < vocab <= MAX_VOCAB:
         raise KernelError(f"verify_drafts: a vocabulary of {vocab} is not supported (1 to {MAX_VOCAB})")
-    _gpu(probs, starts, drafts, accept, final, draft_probs)
-    dev = probs.device
-    ops.on_current_device(dev, "verify_drafts")
-    accepted = torch.empty(requests, dtype=torch.int32, device=dev)
-    tokens = torch.empty((requests, int(max_drafts) + 1), dtype=torch.int32, device=dev)
+    ops.here("verify_drafts", probs, starts, drafts, accept, final, draft_probs)
+    dev, width = probs.device, int(max_drafts) + 1
+    accepted = torch.empty_strided((requests,), (1,), dtype=torch.int32, device=dev)
+    tokens = torch.empty_strided((requests, width), (width, 1), dtype=torch.int32, device=dev)
     if requests == 0:
         return accepted, tokens
     # the row at which a run ends is cut into parts of 2,048 tokens, one workgroup each: what a workgroup of the second launch takes at once; a workgroup a request does all of a short one
     parts = 1 if vocab <= 8192 else min(64, -(-vocab // 2048))
-    sums = torch.empty(requests * parts * 2, dtype=torch.float64, device=dev) if parts > 1 else None
+    sums = torch.empty_strided((requests * parts * 2,), (1,), dtype=torch.float64, device=dev) if parts > 1 else None
     _check(ops.bind("verify", "lcu_verify_drafts", "plipipiplppiiippp")(
         probs.data_ptr(), probs.stride(0), rows, starts.data_ptr(), requests, drafts.data_ptr() if n else None, n, None if draft_probs is None else draft_probs.data_ptr(),
         0 if draft_probs is None else draft_probs.stride(0), accept.data_ptr() if n else None, final.data_ptr(), vocab, int(max_drafts), parts, None if sums is None else sums.data_ptr(), accepted.data_ptr(),

@@ -256,6 +256,84 @@ def test_rows_in_4_bits_that_were_changed():
         assert torch.isnan(after[m // 2]).all() and torch.equal(after[:m // 2], 2 * before[:m // 2]) and torch.equal(after[m // 2 + 1:], 2 * before[m // 2 + 1:])
 
 
+def test_rows_in_4_bits_that_are_changed_between_replays():
+    """A captured product reads the scales that stand there when it is replayed, whether the rows were quantised before the capture, in another one or in its own."""
+    from llama_cu_amd.kernels import ops
+    n, k, m = 64, 288, 200
+    w, _ = weight(n, k)
+    x = rnd(m, k, seed=1).bfloat16().cuda()
+    q = ops.mx4_quantize(x)
+    ops.gemm_mx4(q, w), ops.gemm_mx4(ops.mx4_quantize(x), w)
+    torch.cuda.synchronize()
+    first, second, third = (torch.cuda.CUDAGraph() for _ in range(3))
+    with torch.cuda.graph(first):
+        of_eager = ops.gemm_mx4(q, w, out_dtype=torch.float32)
+    with torch.cuda.graph(second):
+        captured = ops.mx4_quantize(x)
+        of_own = ops.gemm_mx4(captured, w, out_dtype=torch.float32)
+    with torch.cuda.graph(third):
+        of_other = ops.gemm_mx4(captured, w, out_dtype=torch.float32)
+    for seed in (2, 3, 4):
+        now = ops.mx4_quantize(rnd(m, k, seed=seed).bfloat16().cuda())
+        q.codes.copy_(now.codes), q.scales.copy_(now.scales)
+        first.replay()
+        x.copy_(rnd(m, k, seed=seed + 10))
+        second.replay()
+        captured.scales.add_(1)
+        third.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(of_eager, ops.gemm_mx4(now, w, out_dtype=torch.float32))
+        assert torch.equal(of_own, ops.gemm_mx4(ops.mx4_quantize(x), w, out_dtype=torch.float32))
+        assert torch.equal(of_other, 2 * of_own) and torch.equal(ops.gemm_mx4(captured, w, out_dtype=torch.float32), of_other)
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_in_inference_mode(m):
+    from llama_cu_amd.kernels import ops
+    w, _ = weight(64, 288)
+    x = rnd(m, 288).bfloat16().cuda()
+    want = ops.gemm_mx4(ops.mx4_quantize(x), w, out_dtype=torch.float32)
+    outside = ops.mx4_quantize(x)
+    with torch.inference_mode():
+        inside = ops.mx4_quantize(x)
+        for q in (inside, outside):
+            assert torch.equal(ops.gemm_mx4(q, w, out_dtype=torch.float32), want)
+            q.scales.add_(1)
+            assert torch.equal(ops.gemm_mx4(q, w, out_dtype=torch.float32), 2 * want)
+    assert torch.equal(ops.gemm_mx4(outside, w, out_dtype=torch.float32), 2 * want)
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 200])
+@pytest.mark.parametrize("k", [70, 257, 300])
+def test_whatever_lies_behind_k(m, k):
+    """Codes behind the last number, which a file may hold anything in, are not numbers of a row."""
+    from llama_cu_amd.kernels import ops
+    blocks = -(-k // 32)
+
+    def filled(q):
+        codes = q.codes.clone()
+        codes[:, (k + 1) // 2:] = 0x77
+        if k % 2:
+            codes[:, k // 2] |= 0x70
+        return ops.Mx4(codes, q.scales.clone(), k)
+
+    source, rows = ops.mx4_quantize(rnd(48, k, seed=1).bfloat16().cuda()), ops.mx4_quantize(rnd(m, k, seed=2).bfloat16().cuda())
+    assert source.codes.shape == (48, 16 * blocks)
+    want = ops.gemm_mx4(rows, ops.pack_mx4(source))
+    assert torch.equal(ops.gemm_mx4(filled(rows), ops.pack_mx4(filled(source))), want)
+    assert torch.equal(ops.mx4_values(filled(rows)), ops.mx4_values(rows))
+
+
+def test_copies_of_rows_in_4_bits():
+    import copy
+    from llama_cu_amd.kernels import ops
+    w, _ = weight(64, 300)
+    q = ops.mx4_quantize(rnd(40, 300).bfloat16().cuda())
+    want = ops.gemm_mx4(q, w)
+    for other in (copy.copy(q), copy.deepcopy(q), ops.Mx4(q.codes.cpu().cuda(), q.scales.cpu().cuda(), 300)):
+        assert torch.equal(ops.gemm_mx4(other, w), want)
+
+
 def test_infinities_of_32_bit_rows():
     from llama_cu_amd.kernels import ops
     w, exact = weight(32, 128)

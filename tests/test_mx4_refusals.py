@@ -13,7 +13,8 @@ def four(m=4, k=64):
 
 
 def weight(n=32, k=64):
-    return ops.PackedMx4(torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8), n, k)
+    size = -(-n // 16) * -(-k // 256) * 2048
+    return ops.PackedMx4(torch.zeros(size, dtype=torch.uint8), torch.zeros(size // 16, dtype=torch.uint8), n, k)
 
 
 def refused(what, f, *args, **kw):
@@ -52,6 +53,26 @@ def test_products():
     refused("on the GPU", ops.gemm_mx4, four(3), weight())
 
 
+def test_what_is_fixed():
+    """Rows' tensors are not replaced, and a packed weight has the bytes that its sizes ask for: the kernels read all of them."""
+    q = four()
+    for name in ("codes", "scales", "k"):
+        with pytest.raises(AttributeError):
+            setattr(q, name, getattr(q, name))
+    w = weight(40, 300)
+    for codes, scales, n, k in ((w.codes[:-1], w.scales, 40, 300), (w.codes, w.scales[1:], 40, 300), (w.codes, w.scales, 49, 300), (w.codes, w.scales, 40, 513), (w.codes.int(), w.scales, 40, 300),
+                                (w.codes.view(2, -1), w.scales, 40, 300), (w.codes[:0], w.scales[:0], 0, 300)):
+        refused("bytes of codes", ops.PackedMx4, codes, scales, n, k)
+
+
+def test_copies_hold_what_they_were():
+    import copy
+    import pickle
+    q = four(3, 40)
+    for other in (copy.copy(q), copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+        assert torch.equal(other.codes, q.codes) and torch.equal(other.scales, q.scales) and other.shape == q.shape
+
+
 @pytest.mark.gpu
 def test_outputs():
     w = ops.pack_mx4(ops.Mx4(four(32).codes.cuda(), four(32).scales.cuda(), 64))
@@ -61,3 +82,7 @@ def test_outputs():
         refused("contiguous rows apart", ops.gemm_mx4, x, w, out=there)
     refused("contiguous rows apart", ops.gemm_mx4, x, w, out=torch.zeros(3, 32).cuda(), swiglu=True)
     refused("on the GPU", ops.gemm_mx4, x, w, out=torch.zeros(3, 32))
+    wide = torch.zeros(3, 128).cuda()
+    refused("over an operand", ops.gemm_mx4, wide[:, :64], w, out=wide[:, 32:64])
+    refused("over an operand", ops.gemm_mx4, wide[:, :64], w, out=wide[:, 96:])       # between the rows: refused too
+    assert ops.gemm_mx4(wide[:1, :64], w, out=wide[:1, 96:]).shape == (1, 32)

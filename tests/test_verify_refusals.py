@@ -54,3 +54,10 @@ def test_verify_drafts():
         refused("max_drafts", call, most=most)
     refused("drafts must be", call, probs=torch.zeros(1, 8))
     refused("vocabulary of 0", call, probs=torch.zeros(5, 0), draft_probs=torch.zeros(3, 0))
+
+
+def test_a_distribution_does_not_go_over_its_logits():
+    logits = torch.zeros(4, 40)
+    for out in (logits, logits.view(-1)[20:100].view(2, 40)):
+        with pytest.raises(KernelError, match="over an operand"):
+            token_probs(logits[:out.shape[0]], [1.0] * len(out), [0.9] * len(out), [5] * len(out), out=out)
