@@ -7,7 +7,8 @@
 //   rows in bfloat16   a step is 64 k.  A lane reads a block of 32 codes of a feature at once, a step's worth, and makes the operands of the four
 //                      slices (32 x 32 x 16) out of it as they are needed; W takes a quarter of the LDS and of its bandwidth that bfloat16 would.
 //                      The waves stand four by features and two by tokens, since every wave converts its own features' codes.
-//   rows in float32    are bfloat16 rows of three times the k (planes one behind the other), with W gone through three times.
+//   rows in float32    come as three planes of bfloat16 whose sum they are, and a step takes all three: the features' operands are made once for them.  (As rows of three times the
+//                      k, with W gone through three times: 37 x 4104 x 11008 31.3 us, so 26.4; 1600 x 6144 x 4096 223 us, so 211.)
 //   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, four bytes a lane and step, come into registers.  Steps of 128 k, which the rings hold more of,
 //                      took a tenth longer: half a line a row and load.
 #include <type_traits>
@@ -23,25 +24,25 @@ __device__ __forceinline__ void mt_wait_loads() {
     __builtin_amdgcn_s_waitcnt((LEFT & 15) | ((LEFT >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
-// FOUR: rows in 4 bits.  SF, ST: steps of features and of tokens that the rings hold.
-template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_> struct MtShape {
+// FOUR: rows in 4 bits.  SF, ST: steps of features and of tokens that the rings hold.  P: planes of a row that a step takes, one product each with the same features.
+template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_, int P_ = 1> struct MtShape {
     static constexpr bool FOUR = FOUR_;
-    static constexpr int FT = FT_, TT = TT_, WF = WF_, WT = WT_, SF = SF_, ST = ST_, SLICES = 4;
+    static constexpr int FT = FT_, TT = TT_, WF = WF_, WT = WT_, SF = SF_, ST = ST_, P = P_, TOKENS = TT * P, SLICES = 4;
     static constexpr int WAVES = WF * WT, THREADS = WAVES * WAVE, F = 32 * FT * WF, T = 32 * TT * WT;
     static constexpr int FP = FOUR ? 8 : 2, TP = 8;                    // pieces (16 bytes) of a row a stage
     static constexpr int STEP_CODES = 256 * FP;                        // bytes of a tile of 16 features a step
-    static constexpr int LF = F * FP / WAVE / WAVES, LT = T * TP / WAVE / WAVES;       // loads of a wave a stage
+    static constexpr int LF = F * FP / WAVE / WAVES, LT = P * T * TP / WAVE / WAVES;       // loads of a wave a stage
     static constexpr int LS = FOUR ? FT + TT : FT;                     // and of scales, into registers
-    static constexpr int LDS = SF * F * FP + ST * T * TP;              // pieces
+    static constexpr int LDS = SF * F * FP + ST * P * T * TP;              // pieces
     static constexpr int LEFT = (SF > ST ? LF : 0) + (ST - 2) * (LF + LT + LS);        // loads that may be on their way when a step begins
-    static_assert(FT % 2 == 0 && F * FP % (WAVE * WAVES) == 0 && T * TP % (WAVE * WAVES) == 0 && SF >= ST && ST >= 2 && LDS * 16 <= 160 * 1024, "whole loads, and room for the stages");
+    static_assert(FT % 2 == 0 && F * FP % (WAVE * WAVES) == 0 && T * P * TP % (WAVE * WAVES) == 0 && (P == 1 || !FOUR) && SF >= ST && ST >= 2 && LDS * 16 <= 160 * 1024, "whole loads, and room for the stages");
 };
 
 // Where piece c of row r stands among the row's in LDS: sixteen neighbouring rows' pieces c lie in sixteen places that are read at once (c ^ (r & 7), in eight: four
 // cycles a read more).
 __device__ __forceinline__ int mt_place(int r, int c) { return c ^ (r >> 1 & 7); }
 
-template <class S> struct MtFrags { mx4_u32x4 f[S::FT], t[S::TT]; };
+template <class S> struct MtFrags { mx4_u32x4 f[S::FT], t[S::TOKENS]; };
 
 // The scales of a step: FOUR: of the lane's row its four blocks', a byte a slice; else the byte of its one block.
 template <class S> struct MtScales { uint32_t f[S::FT], t[S::FOUR ? S::TT : 1]; };
@@ -59,16 +60,16 @@ __device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const 
                                         IssueF &&issue_f, const int (&at_f)[S::SLICES], const int (&at_t)[S::SLICES], MtFrags<S> (&op)[2], mx4_u32x4 (&codes)[S::FT],
                                         const MtScales<S> &before, const MtScales<S> &now, mx4_f32x16 (&acc)[S::FT][S::TT]) {
     auto slice = [&](auto number) {
-        constexpr int s = decltype(number)::value, PRODUCTS = S::FT * S::TT, used = (s + S::SLICES - 1) % S::SLICES;         // the slice that is multiplied
+        constexpr int s = decltype(number)::value, PRODUCTS = S::FT * S::TOKENS, used = (s + S::SLICES - 1) % S::SLICES;         // the slice that is multiplied
         MtFrags<S> &use = op[(s + 1) & 1], &get = op[s & 1];
 #pragma unroll
         for (int i = 0; i < PRODUCTS; ++i) {
-            const int f = i / S::TT, t = i % S::TT;
+            const int f = i / S::TT % S::FT, t = i % S::TT, p = i / (S::FT * S::TT);
             if constexpr (S::FOUR) {
                 const MtScales<S> &sc = s == 0 ? before : now;
                 acc[f][t] = mx4_multiply_codes_32<used>(use.f[f], use.t[t], acc[f][t], sc.f[f], sc.t[t]);
             } else {
-                acc[f][t] = mx4_multiply_32(use.f[f], use.t[t], acc[f][t]);
+                acc[f][t] = mx4_multiply_32(use.f[f], use.t[p * S::TT + t], acc[f][t]);
             }
             __builtin_amdgcn_sched_barrier(0);
             {
@@ -92,12 +93,15 @@ __device__ __forceinline__ void mt_turn(const mx4_u32x4 *__restrict__ nf, const 
                     else mt_read(get.f[r - S::TT], nf + at_f[s] + 32 * S::FP * (r - S::TT));
                 }
             } else {
-                constexpr int READS = S::TT + (s == 0 ? S::FT : 0);
+                constexpr int READS = S::TOKENS + (s == 0 ? S::FT : 0);
                 const int r0 = i * READS / PRODUCTS, r1 = (i + 1) * READS / PRODUCTS;
 #pragma unroll
                 for (int r = r0; r < r1; ++r) {
                     if (s == 0 && r < S::FT) mt_read(codes[r], nf + at_f[0] + 32 * S::FP * r);
-                    else mt_read(get.t[r - (s == 0 ? S::FT : 0)], nt + at_t[s] + 32 * S::TP * (r - (s == 0 ? S::FT : 0)));
+                    else {
+                        const int x = r - (s == 0 ? S::FT : 0);
+                        mt_read(get.t[x], nt + at_t[s] + (x / S::TT * S::T + 32 * (x % S::TT)) * S::TP);
+                    }
                 }
                 // the next slice's features, in the second half of this one's products
                 constexpr int HALF = PRODUCTS / 2;
@@ -126,7 +130,7 @@ struct MtArgs {
     int pairs;
     void *y;
     long long ldy;
-    int M, N, steps, w_steps;       // steps of X; of W, which begins anew where it ends
+    int M, N, steps, slices;
     int wide_out;
     int each;                       // steps of a slice of K; slice i's sums go to the i-th plane of y
     long long plane;
@@ -140,12 +144,13 @@ mx4_tiles_kernel(MtArgs a) {
     constexpr bool FOUR = S::FOUR, SWIGLU = EPI >= MT_EPI_SWIGLU, OUT32 = EPI == MT_EPI_F32 || EPI == MT_EPI_SWIGLU_F32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, hi = lane >> 5;
     const int wf = wave % S::WF, wt = wave / S::WF;
-    // ---- which tile: workgroups go to the eight dies in turn; a die takes a run of tiles, those of a few feature tiles side by side
-    const int first = blockIdx.y * a.each, steps = min(a.steps - first, a.each);
-    const int t_tiles = (a.M + S::T - 1) / S::T, f_tiles = (a.N + S::F - 1) / S::F, tiles = t_tiles * f_tiles;
-    const int each = (tiles + 7) / 8, item = blockIdx.x % 8 * each + blockIdx.x / 8;
-    if ((int)blockIdx.x / 8 >= each || item >= tiles) return;
-    const int ft0 = item / t_tiles, tt0 = item - ft0 * t_tiles, half_n = a.N / 2;
+    // ---- which tile and slice: workgroups go to the eight dies in turn; a die takes a run of a slice's tiles, those of a few feature tiles side by side (17 tiles in 12 slices
+    // by tiles alone, 3 a die and none for the last two: 41 us, so 35)
+    const int t_tiles = (a.M + S::T - 1) / S::T, f_tiles = (a.N + S::F - 1) / S::F, tiles = t_tiles * f_tiles, items = tiles * a.slices;
+    const int run = (items + 7) / 8, item = blockIdx.x % 8 * run + blockIdx.x / 8;
+    if ((int)blockIdx.x / 8 >= run || item >= items) return;
+    const int slice_k = item / tiles, of_slice = item - slice_k * tiles, ft0 = of_slice / t_tiles, tt0 = of_slice - ft0 * t_tiles, half_n = a.N / 2;
+    const int first = slice_k * a.each, steps = min(a.steps - first, a.each);
     // row r of the tile's features in W (SwiGLU: in turns 32 gate rows and the up rows that meet them)
     auto feature = [&](int r) { return SWIGLU ? (r / 32 & 1) * half_n + ft0 * (S::F / 2) + r / 64 * 32 + r % 32 : ft0 * S::F + r; };
     const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.codes), 0, a.codes_bytes, 0x00020000);
@@ -164,7 +169,7 @@ mx4_tiles_kernel(MtArgs a) {
 #pragma unroll
     for (int i = 0; i < S::LT; ++i) {
         const int r = (i * S::WAVES + wave) * (WAVE / S::TP) + lane / S::TP;
-        from_t[i] = (uint32_t)(tt0 * S::T + r) * a.ldx + 16u * mt_place(r, lane % S::TP);
+        from_t[i] = (uint32_t)(tt0 * S::T + r % S::T) * a.ldx + (S::P > 1 ? (uint32_t)(r / S::T) * (a.ldx / S::P) : 0u) + 16u * mt_place(r, lane % S::TP);
     }
     mx4_u32x4 *const lds_f = mt_lds, *const lds_t = mt_lds + S::SF * S::F * S::FP;
     // (a later step than there are: the last once more, which nobody reads)
@@ -218,13 +223,13 @@ mx4_tiles_kernel(MtArgs a) {
         before.f[f] = 0;
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
+    for (int t = 0; t < S::TOKENS; ++t) {
         op[1].t[t] = mx4_u32x4{0u, 0u, 0u, 0u};
         before.t[FOUR ? t : 0] = 0;
     }
-    // W's step of the features' ring: one that goes round
-    int wf_step = first % a.w_steps;
-    auto next_w = [&](int s) { return s + 1 == a.w_steps ? 0 : s + 1; };
+    // the features' ring's step (behind the last one: the first, which nobody reads)
+    int wf_step = first;
+    auto next_w = [&](int s) { return s + 1 == a.steps ? 0 : s + 1; };
     // what SF - 1 turns before the first would have asked for
     int s_step = wf_step;
     fetch_scales(next, first, s_step);
@@ -232,7 +237,7 @@ mx4_tiles_kernel(MtArgs a) {
     for (int j = 1 - S::SF; j < 0; ++j) {
         if (j + S::ST - 1 >= 0) {
 #pragma unroll
-            for (int i = 0; i < S::LT; ++i) issue_t(lds_t + (j + S::ST - 1) * S::T * S::TP, j + S::ST - 1, i);
+            for (int i = 0; i < S::LT; ++i) issue_t(lds_t + (j + S::ST - 1) * S::P * S::T * S::TP, j + S::ST - 1, i);
         }
 #pragma unroll
         for (int i = 0; i < S::LF; ++i) issue_f(lds_f + (j + S::SF - 1) * S::F * S::FP, wf_step, i);
@@ -245,7 +250,7 @@ mx4_tiles_kernel(MtArgs a) {
         fetch_scales(next, first + min(t + 1, steps - 1), s_step);
         mt_wait_loads<S::LEFT>();                              // this step's stages are there
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        mt_turn<S>(lds_f + rf * S::F * S::FP + of_f, lds_t + rt * S::T * S::TP + of_t, lds_f + df * S::F * S::FP, lds_t + dt * S::T * S::TP,
+        mt_turn<S>(lds_f + rf * S::F * S::FP + of_f, lds_t + rt * S::P * S::T * S::TP + of_t, lds_f + df * S::F * S::FP, lds_t + dt * S::P * S::T * S::TP,
                    [&](mx4_u32x4 *dst, int i) { issue_t(dst, t + S::ST - 1, i); }, [&](mx4_u32x4 *dst, int i) { issue_f(dst, wf_step, i); }, at_f, at_t, op, codes, before, now, acc);
         before = now;
         wf_step = next_w(wf_step);
@@ -256,17 +261,17 @@ mx4_tiles_kernel(MtArgs a) {
     }
     // the last slice
 #pragma unroll
-    for (int i = 0; i < FT * TT; ++i) {
-        const int f = i / TT, t = i % TT;
+    for (int i = 0; i < FT * S::TOKENS; ++i) {
+        const int f = i / TT % FT, t = i % TT, p = i / (FT * TT);
         if constexpr (FOUR) acc[f][t] = mx4_multiply_codes_32<3>(op[1].f[f], op[1].t[t], acc[f][t], before.f[f], before.t[t]);
-        else acc[f][t] = mx4_multiply_32(op[1].f[f], op[1].t[t], acc[f][t]);
+        else acc[f][t] = mx4_multiply_32(op[1].f[f], op[1].t[p * TT + t], acc[f][t]);
     }
     mt_wait_loads<0>();                                        // (the copies that nobody reads have landed before LDS is used otherwise)
     __syncthreads();
     // ---- out: a wave turns 32 tokens at a time through LDS of its own, and stores whole rows of its features
     constexpr int OUT_F = SWIGLU ? 16 * FT : 32 * FT, ELEM = OUT32 ? 4 : 2, PITCH = OUT_F * ELEM + 16, CH = OUT_F * ELEM / 16;
     static_assert(S::WAVES * 32 * PITCH <= S::LDS * 16, "room for the waves' rows");
-    char *mine = (char *)mt_lds + wave * 32 * PITCH, *const y = (char *)a.y + (size_t)blockIdx.y * a.plane * ELEM;
+    char *mine = (char *)mt_lds + wave * 32 * PITCH, *const y = (char *)a.y + (size_t)slice_k * a.plane * ELEM;
     const int out_n = SWIGLU ? half_n : a.N, f0 = (SWIGLU ? ft0 * (S::F / 2) : ft0 * S::F) + wf * OUT_F;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -350,7 +355,8 @@ mx4_join_kernel(const float *__restrict__ planes, int slices, long long plane, i
 
 template <class S, int EPI>
 static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
-    const int tiles = ((a.M + S::T - 1) / S::T) * ((a.N + S::F - 1) / S::F);
+    const long long items = (long long)((a.M + S::T - 1) / S::T) * ((a.N + S::F - 1) / S::F) * slices;
+    if (items > 0x7ffffff0) return LCU_BAD_ARGUMENT;
     constexpr int bytes = S::LDS * 16;
     static bool asked = false;
     if (!asked && bytes > 64 * 1024) {                         // more LDS than a launch gets unasked
@@ -358,13 +364,13 @@ static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
         if (e != hipSuccess) return (int)e;
         asked = true;
     }
-    mx4_tiles_kernel<S, EPI><<<dim3((tiles + 7) / 8 * 8, slices), dim3(S::THREADS), bytes, stream>>>(a);
+    mx4_tiles_kernel<S, EPI><<<dim3((unsigned)((items + 7) / 8 * 8)), dim3(S::THREADS), bytes, stream>>>(a);
     LCU_LAUNCH_CHECK();
     return LCU_OK;
 }
 
-// Arguments as lcu_mx4_stream's, but that the scales of rows in 4 bits come by pairs of macro-steps (256 k): [pairs][lds bytes], 8 bytes a row; rows in 4 bits in whole pairs.  shape: 0: tiles of 128 x 128
-// (features x tokens), 1: 256 x 256, 2: 128 x 64.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats,
+// Arguments as lcu_mx4_stream's, but that the scales of rows in 4 bits come by pairs of macro-steps (256 k): [pairs][lds bytes], 8 bytes a row; rows in 4 bits in whole pairs.  shape: by x_kind, tiles of features x tokens:
+// 1: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 256 x 128; 3: 0 128 x 64, 1 256 x 64, 2 256 x 32; 4: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 128 x 256.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats,
 // 16-byte aligned.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
 LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *xs, long long lds, const void *codes, const void *scales, int pairs, void *y, long long ldy,
                           int M, int N, int K, int epi, int shape, int slices, void *planes, hipStream_t stream) {
@@ -383,16 +389,14 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     a.codes = (const uint8_t *)codes; a.scales = (const uint8_t *)scales;
     a.codes_bytes = (uint32_t)(w_rows * pairs * 128); a.scales_bytes = (uint32_t)(w_rows * pairs * 8);
     a.pairs = pairs; a.y = y; a.ldy = ldy; a.M = M; a.N = N;
-    // steps: 256 k in 4 bits, else 64; three planes one behind the other are rows of three times as many, filled up to whole pairs
+    // steps: 256 k in 4 bits, else 64
     const int two = (macros + 1) / 2;
-    a.w_steps = x_kind == 4 ? two : x_kind == 3 ? (int)(ldx / 3 / 64) : macros * 2;
-    a.steps = x_kind == 3 ? 3 * a.w_steps : a.w_steps;
-    if (x_kind == 3 && a.w_steps > pairs * 4) return LCU_BAD_ARGUMENT;
-    a.x_bytes = (uint32_t)((M - 1) * row_bytes + (long long)a.steps * 128);
+    a.steps = x_kind == 4 ? two : macros * 2;
+    a.x_bytes = (uint32_t)((M - 1) * row_bytes + (x_kind == 3 ? row_bytes : (long long)a.steps * 128));
     a.xs_bytes = x_kind == 4 ? (uint32_t)((two - 1) * lds + M * 8ll) : 0u;
     if (slices < 1 || slices > a.steps || (slices > 1 && (!planes || (uintptr_t)planes % 16))) return LCU_BAD_ARGUMENT;
     a.each = (a.steps + slices - 1) / slices;
-    slices = (a.steps + a.each - 1) / a.each;                  // (as many as hold a step)
+    a.slices = slices = (a.steps + a.each - 1) / a.each;       // (as many as hold a step)
     const bool wide = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % 16 == 0;
     a.wide_out = wide;
     if (slices > 1) {
@@ -413,6 +417,10 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
         else if (shape == 1) EPIS(true, 4, 4, 2, 2, 3, 2);
         else if (shape == 2) EPIS(true, 2, 1, 2, 2, 3, 3);
         else if (shape == 3) EPIS(true, 2, 2, 2, 4, 3, 3);
+    } else if (x_kind == 3) {
+        if (shape == 0) EPIS(false, 2, 1, 2, 2, 4, 3, 3);
+        else if (shape == 1) EPIS(false, 2, 1, 4, 2, 4, 4, 3);
+        else if (shape == 2) EPIS(false, 2, 1, 4, 1, 4, 4, 3);
     } else {
         if (shape == 0) EPIS(false, 2, 2, 2, 2, 4, 4);
         else if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);

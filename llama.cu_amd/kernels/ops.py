@@ -2926,24 +2926,27 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     return Mx4(codes, scales, 32 * whole)
 
 
-# What the kernels of the 4-bit products take, us, fitted to 12,000 timed products of 12 to 3,200 rows and 9,500 of 1 to 96 (64 to 128,256 features, K 128 to 28,672;
-# weights out of memory): the choice by these numbers takes 1.01 (many rows) to 1.05 (few) times what the best choice takes, geometric mean.
-# Tiles (features, tokens) by whether the rows are in 4 bits and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three workgroups
+# What the kernels of the 4-bit products take, us, fitted to 171,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory): the choice by
+# these numbers takes 1.023 times what the best choice takes, geometric mean; 1.01 of many rows, 1.05 where the streaming kernel and the tiles meet.
+# Tiles (features, tokens) by the kind of the rows and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three workgroups
 # on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
 _MX4_TILES = {
-    (False, 0): (128, 128, 2, 4.78, 1.66, (0.43, 0.74), 2.47, 0.21),
-    (False, 1): (256, 256, 1, 2.10, 6.99, (1.09,), 3.54, 0.15),
-    (False, 2): (128, 64, 3, 4.43, 0.45, (0.38, 0.53, 0.69), 2.78, 0.26),
-    (False, 3): (256, 128, 2, 5.14, 3.31, (0.64, 1.34), 4.49, 0.14),
-    (True, 0): (128, 128, 1, 1.62, 3.72, (0.70,), 2.72, 0.17),
-    (True, 1): (256, 256, 1, 2.32, 10.59, (1.25,), 3.44, 0.12),
-    (True, 2): (128, 64, 2, 2.60, 1.82, (0.56, 1.01), 2.62, 0.22),
-    (True, 3): (128, 256, 1, 1.37, 4.71, (0.88,), 3.37, 0.15),
+    1: ((128, 128, 2, 3.37, 2.44, (0.41, 0.72), 2.63, 0.20),
+        (256, 256, 1, 3.03, 5.22, (1.01,), 3.86, 0.16),
+        (128, 64, 3, 3.22, 0.96, (0.37, 0.55, 0.72), 2.63, 0.26),
+        (256, 128, 2, 4.42, 3.22, (0.59, 1.22), 3.29, 0.16)),
+    3: ((128, 64, 1, 5.38, 1.83, (0.55,), 2.50, 0.34),
+        (256, 64, 1, 5.84, 1.81, (0.83,), 2.61, 0.31),
+        (256, 32, 2, 6.87, 0.00, (0.52, 1.02), 2.79, 0.32)),
+    4: ((128, 128, 1, 3.92, 3.57, (0.71,), 2.93, 0.16),
+        (256, 256, 1, 3.24, 11.13, (1.25,), 4.21, 0.12),
+        (128, 64, 2, 3.17, 2.97, (0.59, 1.12), 2.98, 0.18),
+        (128, 256, 1, 3.76, 4.24, (0.90,), 3.43, 0.15)),
 }
 # The kernel that streams the weight, by the kind of the rows: us a launch; a workgroup alone, and for each macro-step of a wave; a macro-step where workgroups share a compute unit, and what four
 # rows add to that.
-_MX4_STREAM = {1: (2.20, 0.32, 0.20, 0.34, 0.11), 3: (0.05, 3.44, 0.49, 0.39, 0.32), 4: (2.76, 0.87, 0.01, 0.13, 0.09)}
-_MX4_SLICES = (1, 2, 3, 4, 6, 8, 12, 16)
+_MX4_STREAM = {1: (0.05, 2.25, 0.34, 0.29, 0.11), 3: (0.45, 2.46, 0.70, 0.34, 0.33), 4: (1.37, 1.95, 0.20, 0.23, 0.09)}
+_MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
 
 
 @functools.lru_cache(maxsize=8192)
@@ -2957,10 +2960,8 @@ def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
         launch, alone, step, shared, rows = _MX4_STREAM[kind]
         load = max(1.0, -(-n // 16) * -(-m // (16 * tiles)) / cu)
         best = (launch + alone + per * step + load * per * (shared + rows * fours), -1, 1)
-    steps = -(-k // 256) if kind == 4 else 2 * macros if kind == 1 else 12 * -(-k // 256)
-    for (four, shape), (features, tokens, held, launch, each_wg, step, join, join_mb) in _MX4_TILES.items():
-        if four != (kind == 4):
-            continue
+    steps = -(-k // 256) if kind == 4 else 2 * macros
+    for shape, (features, tokens, held, launch, each_wg, step, join, join_mb) in enumerate(_MX4_TILES[kind]):
         tiles = -(-n // features) * -(-m // tokens)
         for slices in _MX4_SLICES:
             if slices > 1 and (steps < 2 * slices or tiles * slices > 4 * held * cu):
@@ -3052,7 +3053,7 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         _check(bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")(rows.data_ptr(), ld, kind, xs, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs, out.data_ptr(), of_out, m, n, k,
                                                                       epilogue, stream), "gemm_mx4")
         return out
-    steps = w.pairs if four else (-(-k // 128) * 2 if kind == 1 else 12 * w.pairs)
+    steps = w.pairs if four else -(-k // 128) * 2
     slices = max(1, min(slices, steps))
     planes = torch.empty_strided((slices * min(m, most) * n,), (1,), dtype=torch.float32, device=device) if slices > 1 else None
     if four:
