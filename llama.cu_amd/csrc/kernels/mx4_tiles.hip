@@ -358,11 +358,12 @@ static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
     const long long items = (long long)((a.M + S::T - 1) / S::T) * ((a.N + S::F - 1) / S::F) * slices;
     if (items > 0x7ffffff0) return LCU_BAD_ARGUMENT;
     constexpr int bytes = S::LDS * 16;
-    static bool asked = false;
-    if (!asked && bytes > 64 * 1024) {                         // more LDS than a launch gets unasked
+    static unsigned long long asked = 0;                       // a bit a device
+    int device = 0;
+    if (bytes > 64 * 1024 && hipGetDevice(&device) == hipSuccess && !(asked >> (device & 63) & 1)) {      // more LDS than a launch gets unasked
         const hipError_t e = hipFuncSetAttribute((const void *)mx4_tiles_kernel<S, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return (int)e;
-        asked = true;
+        asked |= 1ull << (device & 63);
     }
     mx4_tiles_kernel<S, EPI><<<dim3((unsigned)((items + 7) / 8 * 8)), dim3(S::THREADS), bytes, stream>>>(a);
     LCU_LAUNCH_CHECK();

@@ -140,7 +140,7 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     dev = logits.device
     temperature = _options(temperature, torch.float32, rows, dev, "temperature", lambda low, high, total: low >= 0 and high < float("inf") and total == total, ">= 0")
     top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda low, high, total: low > 0 and total == total, "> 0")
-    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, high, total: low >= 1, ">= 1")
+    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, high, total: low >= 1 and total == total, ">= 1")
     if out is None:
         out = torch.empty_strided((rows, vocab), (vocab, 1), dtype=torch.float32, device=dev)
     else:

@@ -149,3 +149,43 @@ def test_verify_refusals():
     with pytest.raises(KernelError, match="probs"):
         s.probs(logits, [p])
     assert [len(t) for t in s.verify(logits, [[], [], []], [p] * 3, [(i, 0) for i in range(3)])] == [1, 1, 1]
+
+
+@pytest.mark.parametrize("name", ["A", "B"])
+@pytest.mark.parametrize("family", ["divasun", "lozezen", "ralepel", "mufotar", "gefudra", "lapunex"])
+def test_other_designs_compute_with_the_rounded_matrices(family, name, monkeypatch):
+    """As the Llama model above, by logits: a prompt as a whole, and then two requests' tokens one by one."""
+    import importlib
+    from llama_cu_amd.engine.runner import ModelRunner
+    from llama_cu_amd.kernels import ops
+    from llama_cu_amd.parts import ffn, linear
+    C, T = importlib.import_module(f"{family}_common"), importlib.import_module(f"test_gpu_{family}")
+    cfg = getattr(C, f"CFG_{name}")
+    args = (cfg, getattr(C, f"RANKS_{name}"), 5) if family == "divasun" else (cfg, 5)
+    folder = C.make_folder(cfg, C.random_weights(*args))
+    a, b = C.tokens_of(cfg["vocab"], 60, 1), C.tokens_of(cfg["vocab"], 9, 2)
+
+    def logits(**kw):
+        r = ModelRunner.from_folder(folder, dtype="float32", page_size=16, max_tokens=1024, max_seqs=4, max_batch_tokens=1024, **kw)
+        held = sum(isinstance(v, ops.PackedMx4) for v in seen)
+        out = [r.step([0], [a[:50]], [list(range(50))]).clone(), r.step([1, 0], [b[:8], a[50:51]], [list(range(8)), [0]]).clone()]
+        for i in range(51, 54):
+            out.append(r.step([0], [a[i:i + 1]], [[0]]).clone())
+        r.end(0); r.end(1)
+        r.cache.check()
+        return torch.cat(out).double().cpu(), held
+
+    seen, plain = [], linear.Weight.__init__
+
+    def watched(self, tensor, build=None, packed_from=None, halves=False, four_bits=False):
+        if watched.round and (four_bits or halves):                  # (gate and up, which the feed-forward alone says are halves)
+            tensor = ops.mx4_values(ops.mx4_quantize(tensor), torch.float32).to(tensor.dtype)
+            packed_from = None
+        plain(self, tensor, build, packed_from, halves, four_bits)
+        seen.append(self.plain)
+    monkeypatch.setattr(linear.Weight, "__init__", watched)
+    watched.round = False
+    got, held = logits(weights="mx4")
+    watched.round = True
+    want, _ = logits()
+    assert_close(got, want, T.REL["float32"], f"{family} {name}: {held} matrices in 4 bits")

@@ -26,7 +26,7 @@ def test_token_probs():
         refused("temperature must be 2 numbers >= 0", token_probs, x, t, fine[1], fine[2])
     for p in ([1.0], [1.0, 0.0], [1.0, float("nan")]):
         refused("top_p must be 2 numbers > 0", token_probs, x, fine[0], p, fine[2])
-    for k in ([1], [0, 8], [8, -1]):
+    for k in ([1], [0, 8], [8, -1], [8, float("nan")], [float("nan"), 8]):
         refused("top_k must be 2 numbers >= 1", token_probs, x, fine[0], fine[1], k)
     for out in (torch.zeros(2, 9), torch.zeros(2, 8).double(), torch.zeros(2, 16)[:, :8], torch.zeros(1, 8)):
         refused("out: must be contiguous float32", token_probs, x, *fine, out=out)
