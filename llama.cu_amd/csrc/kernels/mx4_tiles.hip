@@ -310,17 +310,17 @@ mx4_tiles_kernel(MtArgs a) {
 // The planes of the slices' sums, added up, and the epilogue: four columns a thread.
 template <int EPI>
 __global__ void __launch_bounds__(256)
-mx4_join_kernel(const float *__restrict__ planes, int slices, long long plane, int N, int M, void *__restrict__ y, long long ldy, int wide_out) {
+mx4_join_kernel(const float *__restrict__ planes, int slices, long long plane, int N, int M, long long ldp, void *__restrict__ y, long long ldy, int wide_out) {
     constexpr bool SWIGLU = EPI >= MT_EPI_SWIGLU, OUT32 = EPI == MT_EPI_F32 || EPI == MT_EPI_SWIGLU_F32;
     const int cols = SWIGLU ? N / 2 : N, fours = (cols + 3) / 4;
     const long long at = blockIdx.x * 256ll + threadIdx.x;
     if (at >= (long long)M * fours) return;
     const int row = (int)(at / fours), col = (int)(at - (long long)row * fours) * 4, n = min(4, cols - col);
     auto sum = [&](int c, float (&v)[4]) {
-        const float *from = planes + (size_t)row * N + c;
+        const float *from = planes + row * ldp + c;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = 0.f;
-        if (N % 4 == 0 && c % 4 == 0) {
+        if (c % 4 == 0) {
 #pragma unroll 4
             for (int s = 0; s < slices; ++s) {
                 const mx4_f32x4 p = *(const mx4_f32x4 *)(from + s * plane);
@@ -371,7 +371,8 @@ static int mt_go(const MtArgs &a, int slices, hipStream_t stream) {
 }
 
 // Arguments as lcu_mx4_stream's, but that the scales of rows in 4 bits come by pairs of macro-steps (256 k): [pairs][lds bytes], 8 bytes a row; rows in 4 bits in whole pairs.  shape: by x_kind, tiles of features x tokens:
-// 1: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 256 x 128; 3: 0 128 x 64, 1 256 x 64, 2 256 x 32; 4: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 128 x 256.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats,
+// 1: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 256 x 128, 4 256 x 32; 3: 0 128 x 64, 1 256 x 64, 2 256 x 32; 4: 0 128 x 128, 1 256 x 256, 2 128 x 64, 3 128 x 256.  slices: of K, each of which has workgroups of its own; with more than one, planes has room for slices x M x N floats (N
+// rounded up to four),
 // 16-byte aligned.  A load's place is 32 bits: a call takes rows and weights of less than 4 GiB each (the rows of the last tile beyond their end too).
 LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *xs, long long lds, const void *codes, const void *scales, int pairs, void *y, long long ldy,
                           int M, int N, int K, int epi, int shape, int slices, void *planes, hipStream_t stream) {
@@ -401,8 +402,8 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
     const bool wide = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % 16 == 0;
     a.wide_out = wide;
     if (slices > 1) {
-        a.y = planes; a.ldy = N; a.plane = (long long)M * N;
-        a.wide_out = N % 4 == 0;
+        a.y = planes; a.ldy = (N + 3) / 4 * 4; a.plane = M * a.ldy;             // (rows of whole fours, with 13 columns or 929: else each number went alone, twice the time)
+        a.wide_out = true;
     }
 #define EPIS(...)                                                                    \
     do {                                                                             \
@@ -427,13 +428,14 @@ LCU_API int lcu_mx4_tiles(const void *x, long long ldx, int x_kind, const void *
         else if (shape == 1) EPIS(false, 2, 4, 4, 2, 4, 3);
         else if (shape == 2) EPIS(false, 2, 1, 2, 2, 4, 4);
         else if (shape == 3) EPIS(false, 2, 4, 4, 1, 4, 3);
+        else if (shape == 4) EPIS(false, 2, 1, 4, 1, 3, 3);
     }
 #undef EPIS
     if (rc != LCU_OK || slices == 1) return rc;
     const long long threads = (long long)M * ((cols + 3) / 4);
     const int out_wide = ((uintptr_t)y | (uintptr_t)(ldy * elem) | (uintptr_t)(cols * elem)) % (4 * elem) == 0;
     const dim3 grid((unsigned int)((threads + 255) / 256)), block(256);
-#define JOIN(EPI) mx4_join_kernel<EPI><<<grid, block, 0, stream>>>((const float *)planes, slices, a.plane, N, M, y, ldy, out_wide)
+#define JOIN(EPI) mx4_join_kernel<EPI><<<grid, block, 0, stream>>>((const float *)planes, slices, a.plane, N, M, a.ldy, y, ldy, out_wide)
     if (epi == MT_EPI_BF16) JOIN(MT_EPI_BF16);
     else if (epi == MT_EPI_F32) JOIN(MT_EPI_F32);
     else if (epi == MT_EPI_SWIGLU) JOIN(MT_EPI_SWIGLU);

@@ -2926,26 +2926,28 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     return Mx4(codes, scales, 32 * whole)
 
 
-# What the kernels of the 4-bit products take, us, fitted to 171,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory): the choice by
-# these numbers takes 1.023 times what the best choice takes, geometric mean; 1.01 of many rows, 1.05 where the streaming kernel and the tiles meet.
-# Tiles (features, tokens) by the kind of the rows and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three workgroups
+# What the kernels of the 4-bit products take, us, fitted to 193,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory): the choice by
+# these numbers takes 1.02 times what the best choice takes, geometric mean; 1.01 of many rows, 1.06 where the streaming kernel and the tiles meet (48 and 64 rows).  Up to 8 rows (4 in
+# float32) the streaming kernel takes 1.01 to 1.03 times the best without being asked; at 16 it would be 1.09, 1.42 and 1.06.
+# Tiles (features, tokens) by the kind of the rows and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three, four workgroups
 # on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
 _MX4_TILES = {
-    1: ((128, 128, 2, 3.37, 2.44, (0.41, 0.72), 2.63, 0.20),
-        (256, 256, 1, 3.03, 5.22, (1.01,), 3.86, 0.16),
-        (128, 64, 3, 3.22, 0.96, (0.37, 0.55, 0.72), 2.63, 0.26),
-        (256, 128, 2, 4.42, 3.22, (0.59, 1.22), 3.29, 0.16)),
-    3: ((128, 64, 1, 5.38, 1.83, (0.55,), 2.50, 0.34),
-        (256, 64, 1, 5.84, 1.81, (0.83,), 2.61, 0.31),
-        (256, 32, 2, 6.87, 0.00, (0.52, 1.02), 2.79, 0.32)),
-    4: ((128, 128, 1, 3.92, 3.57, (0.71,), 2.93, 0.16),
-        (256, 256, 1, 3.24, 11.13, (1.25,), 4.21, 0.12),
-        (128, 64, 2, 3.17, 2.97, (0.59, 1.12), 2.98, 0.18),
-        (128, 256, 1, 3.76, 4.24, (0.90,), 3.43, 0.15)),
+    1: ((128, 128, 2, 4.52, 1.32, (0.42, 0.71), 1.64, 0.20),
+        (256, 256, 1, 6.23, 2.04, (0.99,), 1.99, 0.17),
+        (128, 64, 3, 3.93, 0.32, (0.37, 0.53, 0.69), 1.98, 0.26),
+        (256, 128, 2, 7.00, 0.78, (0.58, 1.18), 1.77, 0.17),
+        (256, 32, 4, 4.11, 0.00, (0.39, 0.56, 0.69, 0.94), 2.03, 0.26)),
+    3: ((128, 64, 1, 5.76, 1.84, (0.57,), 2.18, 0.22),
+        (256, 64, 1, 6.35, 1.85, (0.90,), 2.80, 0.20),
+        (256, 32, 2, 6.92, 0.00, (0.53, 1.02), 2.16, 0.28)),
+    4: ((128, 128, 1, 4.82, 2.84, (0.71,), 1.97, 0.18),
+        (256, 256, 1, 7.54, 7.07, (1.25,), 0.58, 0.14),
+        (128, 64, 2, 3.77, 2.50, (0.60, 1.10), 2.60, 0.19),
+        (128, 256, 1, 4.89, 3.13, (0.89,), 2.32, 0.16)),
 }
 # The kernel that streams the weight, by the kind of the rows: us a launch; a workgroup alone, and for each macro-step of a wave; a macro-step where workgroups share a compute unit, and what four
 # rows add to that.
-_MX4_STREAM = {1: (0.05, 2.25, 0.34, 0.29, 0.11), 3: (0.45, 2.46, 0.70, 0.34, 0.33), 4: (1.37, 1.95, 0.20, 0.23, 0.09)}
+_MX4_STREAM = {1: (1.45, 0.87, 0.33, 0.29, 0.12), 3: (0.91, 1.87, 0.77, 0.35, 0.33), 4: (0.92, 2.56, 0.19, 0.22, 0.09)}
 _MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
 
 
@@ -2953,9 +2955,11 @@ _MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
 def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
     macros = -(-k // 128)
     best = (float("inf"), -1, 1)
+    if m <= (4 if kind == 3 else 8):
+        return -1, 1
     if m <= 64:
         tiles = 1 if m <= 16 else 2 if m <= 32 or kind == 3 else 4        # of 16 rows, together
-        fours = 4 * tiles if m > 16 or kind == 4 else 1 if m <= 4 else 2 if m <= 8 and kind == 1 else 4      # loads of four rows
+        fours = 4 * tiles                                                 # loads of four rows
         per = -(-macros // 8) if kind == 4 else 2 * -(-macros // 16)
         launch, alone, step, shared, rows = _MX4_STREAM[kind]
         load = max(1.0, -(-n // 16) * -(-m // (16 * tiles)) / cu)
@@ -3055,7 +3059,7 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         return out
     steps = w.pairs if four else -(-k // 128) * 2
     slices = max(1, min(slices, steps))
-    planes = torch.empty_strided((slices * min(m, most) * n,), (1,), dtype=torch.float32, device=device) if slices > 1 else None
+    planes = torch.empty_strided((slices * min(m, most) * (n + 3 & -4),), (1,), dtype=torch.float32, device=device) if slices > 1 else None
     if four:
         scales = _mx4_by_pair(q, blocks, stream)
         xs, lds = scales.data_ptr(), 8 * m
