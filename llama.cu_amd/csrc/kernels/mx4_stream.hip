@@ -5,6 +5,10 @@
 // in registers, exactly and with their scale, two a conversion, in the order in which the matrix instruction of 16 x 16 x 32 wants its operand.  Rows of
 // float32 come as three planes of bfloat16 whose sum they are, each multiplied with the same codes.  Rows in 4 bits: the scaled instruction of 16 x 16 x 128
 // takes both sides' codes and scales as they are.
+//
+// Bound by memory where the weight is large, by the latency of a wave's chain of loads where it is not (a wave has K / 8, of which two pairs of macro-steps are on their way; K is
+// split over the waves of one workgroup and no further, so that no second launch adds the parts).  One row: 6144 x 4096 5.2 us (2.6 TB/s), 128256 x 4096 59 (4.7 TB/s); 8 rows: 28672 x
+// 4096 with the activation 15.1 us (4.1 TB/s), 57344 x 8192 54 (4.6).  Beyond 8 rows every workgroup's reading of all rows out of the L2 caches weighs more and the products in tiles take over.
 #include "mx4.h"
 #include "mx4/matrix.h"
 #include "gate_act.h"

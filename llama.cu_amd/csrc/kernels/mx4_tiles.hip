@@ -11,6 +11,12 @@
 //                      k, with W gone through three times: 37 x 4104 x 11008 31.3 us, so 26.4; 1600 x 6144 x 4096 223 us, so 211.)
 //   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, four bytes a lane and step, come into registers.  Steps of 128 k, which the rings hold more of,
 //                      took a tenth longer: half a line a row and load.
+//
+// Which tile: the largest that fills the card, and where none does slices of K beside each other, whose sums a second launch adds (the rule and its figures stand where the kernel is
+// chosen).  Rows in 4 bits have waves of 128 x 128 and one a SIMD, which read half of what waves of 64 x 128 do out of LDS a product (8192 x 28672 with 4,096 rows 480 us, so 430).
+// Bound by the matrix cores and, with many rows, the power that they draw: 28672 x 4096 with the activation, 2,048 rows in bfloat16 360 to 390 us (1.23 to 1.34 PFLOP/s; the library's
+// bfloat16 product alone 354 to 399); 8192 x 28672, 4,096 rows in 4 bits 420 to 430 us (4.5 PFLOP/s).  With few rows by latency: 28672 x 4096, 24 rows 22 us; 4096 x 14336, 64 rows in 4
+// bits 11.2 us and 3.8 for the slices' sums; 4104 x 11008, 37 rows in float32 20.5 us and 3.9.
 #include <type_traits>
 #include "mx4.h"
 #include "mx4/matrix.h"

@@ -15,6 +15,9 @@
 //   store   writes the whole row.
 // Where even those near the cut are too many (tens of thousands of equal logits) `cut` searches the row itself.
 //
+// Bound by memory where there are many rows, and each launch's latency where there are few: 320 rows of 128,256 with cuts of every kind 197 us (max 55, the logits' one trip from
+// memory; count 28, out of the last cache; bracket 12; write 62, at a copy's rate; cut 20 to 24; store 15), 5 rows 34 (5.6, 6.2, 6.3, 6.2, 9.4, 2 and the gaps between them).
+//
 // A NaN counts as -inf, which has no share; a row of nothing else becomes zeros.  Infinities of the one sign share alike.  A temperature
 // that is not positive leaves the first of the largest logits.
 #include "common.h"
