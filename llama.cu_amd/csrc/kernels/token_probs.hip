@@ -2,12 +2,11 @@
 //
 // With the logits in descending order (equal ones by index), weights w_i = exp((l_i - l_0) / T) and prefix sums c, a draw takes the first
 // entry with c_i >= u L, L = min(top_p c_n, c_k): entry i has the share (min(c_i, L) - min(c_{i-1}, L)) / L, so the entry at the cut
-// keeps the part of its weight that lies within.  Nothing is sorted.  Rows of up to 8,192 entries: one launch, a row in a workgroup's registers.  Longer ones: six launches, a row cut into parts in those that read or write it:
+// keeps the part of its weight that lies within.  Nothing is sorted.  Rows of up to 8,192 entries: one launch, a row in a workgroup's registers.  Longer ones: five launches (four of few rows), a row cut into parts in those that read or write it:
 //   max     the largest logit, where it stands, and the sum of all weights, in one pass with a running maximum;
 //   count   a histogram of the distances (l_0 - l) / T, counts alone;
-//   bracket a bin's weights are known to within its width, so the bins in which the cut can lie are known from the counts, and which entries are kept in
-//           full;
-//   write   rows without a cut are written.  Of the others what is not kept becomes zero; entries that are, or may be, are gathered;
+//   write   a bin's weights are known to within its width, so the bins in which the cut can lie are known from the counts, and which entries are kept in full.  Rows
+//           without a cut are written.  Of the others what is not kept becomes zero; entries that are, or may be, are gathered;
 //   cut     one workgroup a row finds the cut among the gathered entries, eight bits of their order at a time, on sums of 64-bit fixed-point
 //           weights (w 2^44: no order of additions changes them), and writes their shares.
 // Where more entries are kept than are gathered (a flat row) only those near the cut are, with the exact sum of what lies above, and the
@@ -15,8 +14,8 @@
 //   store   writes the whole row.
 // Where even those near the cut are too many (tens of thousands of equal logits) `cut` searches the row itself.
 //
-// Bound by memory where there are many rows, and each launch's latency where there are few: 320 rows of 128,256 with cuts of every kind 197 us (max 55, the logits' one trip from
-// memory; count 28, out of the last cache; bracket 12; write 62, at a copy's rate; cut 20 to 24; store 15), 5 rows 34 (5.6, 6.2, 6.3, 6.2, 9.4, 2 and the gaps between them).
+// Bound by memory where there are many rows, and each launch's latency where there are few: 320 rows of 128,256 with cuts of every kind 185 us out of memory (max 55, the logits' one
+// trip; count 28, out of the last cache; write 62, at a copy's rate; cut 18 to 23; store 14), 5 rows 30 (5.7, 5.9, 10, 9 and the gaps between them).
 //
 // A NaN counts as -inf, which has no share; a row of nothing else becomes zeros.  Infinities of the one sign share alike.  A temperature
 // that is not positive leaves the first of the largest logits.
@@ -35,8 +34,7 @@ struct TpPart {                                      // of a part of a row: its 
 struct TpRow {
     unsigned long long mass_above;                   // of entries kept in full that are not gathered
     unsigned int gathered;
-    int bin_lo, bin_hi;                              // the bins in which the cut can lie
-    unsigned int before, upto;                       // how many entries lie in the bins before them, and up to the last of them
+    unsigned int before, upto;                       // how many entries lie in the bins before those in which the cut can lie, and up to the last of them
     // the cut: which key, which of the equal ones is the last that is kept, and the part that it has, the scale of what is kept whole
     unsigned int border;
     int last, store;                                 // store: the row is yet to be written
@@ -229,83 +227,94 @@ tp_count_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
         if (count[b]) atomicAdd(&hist[(size_t)r * TP_BINS + b], count[b]);
 }
 
-// The bins in which the cut can lie.
-__global__ void __launch_bounds__(TP_CUT_THREADS)
-tp_bracket_kernel(int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k, const TpPart *__restrict__ part, int parts,
-                  TpRow *__restrict__ rows, const unsigned int *__restrict__ hists) {
-    constexpr int EACH = TP_BINS / TP_CUT_THREADS, WAVES = TP_CUT_THREADS / WAVE;
-    const int r = blockIdx.x;
-    const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
-    if (c.empty || c.greedy || !c.cuts) return;
-    const unsigned int *__restrict__ hist = hists + (size_t)r * TP_BINS;
+// The bins in which the cut can lie, lo to hi, and how many entries lie before and up to them.  Every thread of the workgroup (TP_THREADS) calls it and gets the answer; held: room for
+// the counts.
+struct TpBracket { int lo, hi; unsigned int before, upto; };
+__device__ __forceinline__ TpBracket tp_bracket(const TpCut &c, const unsigned int *__restrict__ hist, uint4 *__restrict__ held) {
+    constexpr int FOURS = TP_BINS / TP_THREADS / 4, WAVES = TP_THREADS / WAVE;
     __shared__ unsigned int wave_n[WAVES];
-    __shared__ double wave_lo[WAVES], wave_hi[WAVES];
-    __shared__ int found_k, found_lo, found_hi;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) { found_k = found_lo = found_hi = TP_BINS - 1; }
-    // a bin's weights lie between its borders': with room for the roundings of the distances and of the weights
+    __shared__ float wave_lo[WAVES], wave_hi[WAVES];
+    __shared__ int over[3];                            // the first thread whose bins reach: k entries; top_p of the sum at most, and at least
+    __shared__ int bin[3];
+    __shared__ unsigned int before[3], upto[3];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, me = (int)threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < FOURS; ++i) held[i * TP_THREADS + threadIdx.x] = ((const uint4 *)hist)[i * TP_THREADS + threadIdx.x];
+    if (threadIdx.x < 3) over[threadIdx.x] = TP_THREADS - 1;
+    __syncthreads();
+    // a bin's weights lie between its borders'.  A ten-thousandth either way is room for the roundings of distances and weights, and for sums in 32 bits: forty additions deep, 2^-24 each
     const float wide = c.per_bin > 0.f ? 1.0f / c.per_bin : 0.f;
-    unsigned int n[EACH], n_mine = 0;
-    double least[EACH], least_mine = 0.0, most[EACH], most_mine = 0.0;
+    auto walk = [&](unsigned int n_at, float most_at, float least_at, auto f) {
+        float most = 0.f, least = 0.f, edge = tp_weight((float)(me * FOURS * 4) * wide);
+#pragma unroll 1                                       // (with all of it unrolled: 75 registers, and three workgroups a compute unit instead of four)
+        for (int i = 0; i < FOURS; ++i) {
+            const uint4 four = held[me * FOURS + i];
+            const unsigned int n[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) n[e] = hist[threadIdx.x * EACH + e];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int b = (int)threadIdx.x * EACH + e;
-        most[e] = (double)n[e] * (double)(tp_weight((float)b * wide) * 1.0001f);
-        least[e] = (double)n[e] * (double)(tp_weight((float)(b + 1) * wide) * 0.9999f);
-        n_mine += n[e]; most_mine += most[e]; least_mine += least[e];
-    }
-    unsigned int n_scan = n_mine;
-    double most_scan = most_mine, least_scan = least_mine;
+            for (int e = 0; e < 4; ++e) {
+                const int b = (me * FOURS + i) * 4 + e;
+                const float next = tp_weight((float)(b + 1) * wide);
+                most += (float)n[e] * edge;
+                least += (float)n[e] * next;
+                edge = next;
+                n_at += n[e];
+                f(b, n[e], n_at, most_at + most * 1.0001f, least_at + least * 0.9999f);
+            }
+        }
+    };
+    unsigned int n_mine = 0, n_scan;
+    float most_mine = 0.f, least_mine = 0.f;
+    walk(0u, 0.f, 0.f, [&](int, unsigned int, unsigned int n, float most, float least) { n_mine = n; most_mine = most; least_mine = least; });
+    n_scan = n_mine;
+    float most_scan = most_mine, least_scan = least_mine;
 #pragma unroll
     for (int off = 1; off < WAVE; off <<= 1) {
         const unsigned int a = __shfl_up(n_scan, off, WAVE);
-        const double b = __shfl_up(most_scan, off, WAVE), d = __shfl_up(least_scan, off, WAVE);
+        const float b = __shfl_up(most_scan, off, WAVE), d = __shfl_up(least_scan, off, WAVE);
         if (lane >= off) { n_scan += a; most_scan += b; least_scan += d; }
     }
     if (lane == WAVE - 1) { wave_n[wave] = n_scan; wave_hi[wave] = most_scan; wave_lo[wave] = least_scan; }
+    // (what lies before a thread is the thread before's sum: its own sum less its own part would lose what is small beside that)
+    unsigned int n_at = __shfl_up(n_scan, 1, WAVE);
+    float most_at = __shfl_up(most_scan, 1, WAVE), least_at = __shfl_up(least_scan, 1, WAVE);
+    if (lane == 0) { n_at = 0; most_at = least_at = 0.f; }
     __syncthreads();
-    unsigned int n_at = n_scan - n_mine;
-    double most_at = most_scan - most_mine, least_at = least_scan - least_mine;
     for (int w = 0; w < wave; ++w) { n_at += wave_n[w]; most_at += wave_hi[w]; least_at += wave_lo[w]; }
-    const unsigned int n_first = n_at;
-    int first_k = TP_BINS, first_lo = TP_BINS, first_hi = TP_BINS;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int b = (int)threadIdx.x * EACH + e;
-        n_at += n[e]; most_at += most[e]; least_at += least[e];
-        if (first_k == TP_BINS && n_at >= (unsigned int)c.k) first_k = b;
-        if (first_lo == TP_BINS && most_at >= c.limit_p) first_lo = b;
-        if (first_hi == TP_BINS && least_at >= c.limit_p) first_hi = b;
-    }
-    // (a wave's first lane that is over has the wave's first bin; all lanes behind it are over too, and their minima would be taken one after the other)
-    auto first_of = [&](int mine, int *to) {
-        const unsigned long long over = __ballot(mine < TP_BINS);
-        if (over && lane == __ffsll(over) - 1) atomicMin(to, mine);
+    // (a wave's first lane that is over has the wave's first; all lanes behind it are over too, and their minima would be taken one after the other)
+    auto first_of = [&](bool is_over, int *to) {
+        const unsigned long long mask = __ballot(is_over);
+        if (mask && lane == __ffsll(mask) - 1) atomicMin(to, me);
     };
-    first_of(first_k, &found_k);
-    first_of(first_lo, &found_lo);
-    first_of(first_hi, &found_hi);
+    first_of(n_at + n_mine >= (unsigned int)c.k, &over[0]);
+    first_of((double)(most_at + most_mine) >= c.limit_p, &over[1]);
+    first_of((double)(least_at + least_mine) >= c.limit_p, &over[2]);
     __syncthreads();
-    const int lo = min(found_k, found_lo), hi = min(found_k, found_hi);
-    n_at = n_first;
+    // that thread's bin; its last if there is none at all
+    if (me == over[0] || me == over[1] || me == over[2]) {
+        int at[3] = {-1, -1, -1};
+        unsigned int n_before[3], n_upto[3];
+        walk(n_at, most_at, least_at, [&](int b, unsigned int n, unsigned int with, float most, float least) {
+            const bool is_over[3] = {with >= (unsigned int)c.k, (double)most >= c.limit_p, (double)least >= c.limit_p}, last = b % (FOURS * 4) == FOURS * 4 - 1;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-        const int b = (int)threadIdx.x * EACH + e;
-        if (b == lo) { rows[r].bin_lo = lo; rows[r].before = n_at; }
-        n_at += n[e];
-        if (b == hi) { rows[r].bin_hi = hi; rows[r].upto = n_at; }
+            for (int i = 0; i < 3; ++i)
+                if (at[i] < 0 && (is_over[i] || last)) { at[i] = b; n_before[i] = with - n; n_upto[i] = with; }
+        });
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (me == over[i]) { bin[i] = at[i]; before[i] = n_before[i]; upto[i] = n_upto[i]; }
     }
+    __syncthreads();
+    const int lo = bin[1] < bin[0] ? 1 : 0, hi = bin[2] < bin[0] ? 2 : 0;
+    return {bin[lo], bin[hi], before[lo], upto[hi]};
 }
 
 enum { TP_ALL = 0, TP_NEAR = 1, TP_SEARCH = 2 };      // what of a row is gathered: all that is kept, what is near the cut, nothing
-__device__ __forceinline__ int tp_how(const TpRow &b) { return b.upto <= TP_GATHER ? TP_ALL : b.upto - b.before <= TP_GATHER ? TP_NEAR : TP_SEARCH; }
+template <class B> __device__ __forceinline__ int tp_how(const B &b) { return b.upto <= TP_GATHER ? TP_ALL : b.upto - b.before <= TP_GATHER ? TP_NEAR : TP_SEARCH; }
 
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_THREADS)
 tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
-                const TpPart *__restrict__ part, TpRow *__restrict__ rows, TpEntry *__restrict__ entries, float *__restrict__ out) {
+                const TpPart *__restrict__ part, const unsigned int *__restrict__ hist, TpRow *__restrict__ rows, TpEntry *__restrict__ entries, float *__restrict__ out) {
     const int r = blockIdx.x, parts = gridDim.y;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
     int lo, hi;
@@ -321,14 +330,17 @@ tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
         tp_store_shares<WIDE>(row, lo, hi, to, [&](int, float l) { return tp_weight(tp_distance(c, l)) * inv; });
         return;
     }
-    const TpRow b = rows[r];
+    // every workgroup of a row finds the bins by itself: a launch for them alone took 6 us of 5 rows' 34 and 12 of 320 rows' 163
+    __shared__ __attribute__((aligned(16))) TpEntry mine[TP_GATHER / 2];
+    static_assert(sizeof(mine) >= TP_BINS * sizeof(unsigned int), "the counts, and then the entries");
+    const TpBracket b = tp_bracket(c, hist + (size_t)r * TP_BINS, (uint4 *)mine);
+    if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].before = b.before; rows[r].upto = b.upto; }
     const int how = tp_how(b);
     if (how == TP_SEARCH) return;
-    const int from = how == TP_ALL ? 0 : b.bin_lo;
+    const int from = how == TP_ALL ? 0 : b.lo;
     unsigned long long above = 0;
     // a workgroup's entries come together in LDS first: one place of them all in the row's list (an atomic addition a wave and four entries took 25 us of
     // 31 parts' 39)
-    __shared__ TpEntry mine[TP_GATHER / 2];
     __shared__ unsigned int mine_n, place;
     if (threadIdx.x == 0) mine_n = 0;
     __syncthreads();
@@ -346,7 +358,7 @@ tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
     auto entry = [&](int i, float l) {
         const float d = tp_distance(c, l);
         const int bin = d <= TP_NOTHING ? tp_bin(c, d) : TP_BINS;
-        if (bin >= from && bin <= b.bin_hi) mine[atomicAdd(&mine_n, 1u)] = {tp_key(l), i};
+        if (bin >= from && bin <= b.hi) mine[atomicAdd(&mine_n, 1u)] = {tp_key(l), i};
         if (bin < from) above += tp_fixed(tp_weight(d));
     };
     // as much of the stretch at a time as fits whatever is kept of it
@@ -505,16 +517,28 @@ __device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum a
     return t;
 }
 
+// A workgroup's part of a row's shares.
+template <bool WIDE>
+__device__ __forceinline__ void tp_store_row(const float *__restrict__ row, int vocab, const TpCut &c, const TpRow &t, float *__restrict__ to) {
+    int lo, hi;
+    tp_stretch(vocab, blockIdx.y, gridDim.y, lo, hi);
+    tp_store_shares<WIDE>(row, lo, hi, to, [&](int i, float l) {
+        const float d = tp_distance(c, l);
+        return d <= TP_NOTHING ? tp_share(t, tp_key(l), i, tp_weight(d)) : 0.f;
+    });
+}
+
 template <bool WIDE>
 __global__ void __launch_bounds__(TP_CUT_THREADS)
 tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const float *__restrict__ temperature, const float *__restrict__ top_p, const int *__restrict__ top_k,
               const TpPart *__restrict__ part, int parts, TpRow *__restrict__ rows, const TpEntry *__restrict__ entries, float *__restrict__ out) {
+    // gridDim.y workgroups a row, which all find its cut: with more than one each writes its part of a row that is yet to be written
     __shared__ TpShared sh;
     __shared__ unsigned int key_lo, key_hi;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
     if (c.empty || c.greedy || !c.cuts) {
-        if (threadIdx.x == 0) rows[r].store = 0;
+        if (threadIdx.x == 0 && gridDim.y == 1) rows[r].store = 0;
         return;
     }
     const TpRow b = rows[r];
@@ -560,9 +584,14 @@ tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
     TpRow t = tp_search(c, sh, how == TP_NEAR ? TpSum{b.mass_above, b.before} : TpSum{0, 0}, base, span, each);
     t.store = how != TP_ALL;
     if (how == TP_ALL) {
+        if (blockIdx.y > 0) return;
 #pragma unroll
         for (int e = 0; e < TP_EACH; ++e)
             if (e * TP_CUT_THREADS + threadIdx.x < gathered) to[at[e]] = tp_share(t, key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
+    }
+    if (gridDim.y > 1) {
+        if (t.store) tp_store_row<WIDE>(row, vocab, c, t, to);
+        return;
     }
     if (threadIdx.x == 0) {
         rows[r].border = t.border; rows[r].last = t.last; rows[r].store = t.store;
@@ -578,15 +607,7 @@ tp_store_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
     const TpRow t = rows[r];
     if (!t.store) return;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
-    int lo, hi;
-    tp_stretch(vocab, blockIdx.y, parts, lo, hi);
-    const float *row = logits + r * ld;
-    float *to = out + (size_t)r * vocab;
-    auto share = [&](int i, float l) {
-        const float d = tp_distance(c, l);
-        return d <= TP_NOTHING ? tp_share(t, tp_key(l), i, tp_weight(d)) : 0.f;
-    };
-    tp_store_shares<WIDE>(row, lo, hi, to, share);
+    tp_store_row<WIDE>(logits + r * ld, vocab, c, t, out + (size_t)r * vocab);
 }
 
 // A row of up to 1,024 EACH entries as a whole, in registers: one launch for everything.
@@ -682,12 +703,12 @@ LCU_API size_t lcu_token_probs_scratch_bytes(int rows, int vocab, int parts, int
 }
 
 // logits: [rows, ld] float32; temperature, top_p, top_k: [rows], on the device, or null and `given` holds the three one after the other on the host (up to 64 rows); out: [rows,
-// vocab] float32; parts: workgroups a row, 1 to 32; cuts: 0 if no row has top_k < vocab or top_p < 1; scratch: lcu_token_probs_scratch_bytes bytes, 8-byte aligned.
+// vocab] float32; parts: workgroups a row, 1 to 32; cuts: 0 if no row has top_k < vocab or top_p < 1; scratch: lcu_token_probs_scratch_bytes bytes, 16-byte aligned.
 LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int vocab, const float *temperature, const float *top_p, const int *top_k, const float *given, float *out,
                             int parts, int cuts, void *scratch, hipStream_t stream) {
     if (rows <= 0) return LCU_OK;
     const bool small = vocab <= TP_SMALL;
-    if (vocab <= 0 || vocab > TP_MAX_VOCAB || (rows > 1 && ld < vocab) || parts < 1 || parts > TP_MAX_PARTS || !logits || !out || (!small && (!scratch || (uintptr_t)scratch % 8)) ||
+    if (vocab <= 0 || vocab > TP_MAX_VOCAB || (rows > 1 && ld < vocab) || parts < 1 || parts > TP_MAX_PARTS || !logits || !out || (!small && (!scratch || (uintptr_t)scratch % 16)) ||
         (given ? rows > TP_GIVEN : !temperature || !top_p || !top_k))
         return LCU_BAD_ARGUMENT;
     TpOptions options;
@@ -710,11 +731,11 @@ LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int voc
         return LCU_OK;
     }
     char *at = (char *)scratch;
+    unsigned int *hist = cuts ? (unsigned int *)at : nullptr;
+    at += cuts ? (size_t)rows * TP_BINS * sizeof(unsigned int) : 0;
     TpPart *part = (TpPart *)at;             at += (size_t)rows * parts * sizeof(TpPart);
     TpRow *state = (TpRow *)at;              at += cuts ? (size_t)rows * sizeof(TpRow) : 0;
     TpEntry *entries = (TpEntry *)at;        at += cuts ? (size_t)rows * TP_GATHER * sizeof(TpEntry) : 0;
-    unsigned int *hist = cuts ? (unsigned int *)at : nullptr;
-    at += cuts ? (size_t)rows * TP_BINS * sizeof(unsigned int) : 0;
     float *copied = given ? (float *)at : nullptr;
     if (given) {
         temperature = copied;
@@ -723,6 +744,7 @@ LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int voc
     }
     const bool wide = (uintptr_t)logits % 16 == 0 && ld % 4 == 0 && vocab % 4 == 0 && (uintptr_t)out % 16 == 0;
     const dim3 cut(rows, parts), block(TP_THREADS);
+    const bool together = parts > 1 && (long long)rows * parts <= 256;            // a compute unit a workgroup: each finds its row's cut by itself, which saves a launch (5 rows)
 #define GO(WIDE)                                                                                                                                    \
     do {                                                                                                                                            \
         tp_max_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, options, temperature, copied, part, state, hist);                  \
@@ -730,15 +752,13 @@ LCU_API int lcu_token_probs(const float *logits, long long ld, int rows, int voc
         if (cuts) {                                                                                                                                 \
             tp_count_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, hist);                      \
             LCU_LAUNCH_CHECK();                                                                                                                     \
-            tp_bracket_kernel<<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(vocab, temperature, top_p, top_k, part, parts, state, hist);          \
-            LCU_LAUNCH_CHECK();                                                                                                                     \
         }                                                                                                                                           \
-        tp_write_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, entries, out);           \
+        tp_write_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, hist, state, entries, out);     \
         LCU_LAUNCH_CHECK();                                                                                                                         \
         if (cuts) {                                                                                                                                 \
-            tp_cut_kernel<WIDE><<<dim3(rows), dim3(TP_CUT_THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, parts, state, entries, out); \
+            tp_cut_kernel<WIDE><<<dim3(rows, together ? parts : 1), dim3(TP_CUT_THREADS), 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, parts, state, entries, out); \
             LCU_LAUNCH_CHECK();                                                                                                                     \
-            tp_store_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, out);               \
+            if (!together) tp_store_kernel<WIDE><<<cut, block, 0, stream>>>(logits, (size_t)ld, vocab, temperature, top_p, top_k, part, state, out);               \
             LCU_LAUNCH_CHECK();                                                                                                                     \
         }                                                                                                                                           \
     } while (0)

@@ -122,6 +122,24 @@ def test_equal_logits(vocab):
                 assert torch.equal(kept_here, kept_here.sort(descending=True, stable=True)[0])
 
 
+@pytest.mark.parametrize("vocab", [20000, 20001])
+@pytest.mark.parametrize("times", [1, 14])
+def test_rows_of_every_kind_together(vocab, times):
+    """A row whose kept entries are gathered, one of which only those near the cut are, one that is searched, one without a cut, a greedy and an empty one: beside each other, in
+    few rows (whose last launch does more) and in many."""
+    logits = rnd(6, vocab, seed=vocab, std=3.0)
+    logits[1] /= 3
+    logits[2] = 0
+    logits[5] = -float("inf")
+    ts, ps, ks = [0.8, 1.0, 1.0, 1.2, 0.0, 1.0], [0.95, 0.97, 0.6, 1.0, 1.0, 0.9], [10 ** 9, 15000, 10 ** 9, 10 ** 9, 3, 50]
+    got = run(logits.repeat(times, 1), ts * times, ps * times, ks * times).cpu()
+    assert torch.equal(got, got[:6].repeat(times, 1))
+    check(got[:5], logits[:5], ts[:5], ps[:5], ks[:5])
+    assert (got[5] == 0).all()
+    want, _, _ = exact(logits[2], 1.0, 0.6, 10 ** 9)
+    assert (got[2].double() - want).abs().max() <= 4e-6 and torch.equal(got[2] > 0, want > 0)
+
+
 def test_masked_logits():
     inf, low = float("inf"), torch.finfo(torch.float32).min
     v = 5000
