@@ -103,17 +103,28 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _options(values, dtype: torch.dtype, rows: int, device, what: str, fine, why: str) -> torch.Tensor:
-    """A number a row, on the device: a sequence, which is looked at here, or a tensor that is there already, which is not."""
+def _options(values, dtype: torch.dtype, rows: int, device, what: str, fine, why: str):
+    """A number a row, and the least of them: a sequence, which is looked at here, or a tensor that is on the device already, which is not (its least: None)."""
     if isinstance(values, torch.Tensor) and values.is_cuda:
         if values.device != device or values.dtype != dtype or values.shape != (rows,) or not values.is_contiguous():
             raise KernelError(f"token_probs: {what} on the device must be contiguous {dtype} [{rows}], got {values.dtype} {tuple(values.shape)}")
-        return values
+        return values, None
     values = values.tolist() if isinstance(values, torch.Tensor) else list(values)
-    # (the least, the largest and the sum, in which a NaN shows)
-    if len(values) != rows or (rows and not fine(min(values), max(values), sum(values))):
+    low = min(values, default=1)
+    total = sum(values)                # (in which a NaN shows)
+    if len(values) != rows or (rows and not (total == total and fine(low, values))):
         raise KernelError(f"token_probs: {what} must be {rows} numbers {why}")
-    return values
+    return values, low
+
+
+def _packed(kind: str, values, most: int):
+    """A sequence's numbers as the kernels have them; counts that no 32 bits hold are the vocabulary's."""
+    if kind == "i":
+        try:
+            return array.array("i", values)
+        except (OverflowError, TypeError):
+            values = [int(k) if k < most else most for k in values]
+    return array.array(kind, values)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -138,9 +149,9 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     if not 0 < vocab <= MAX_VOCAB:
         raise KernelError(f"token_probs: a vocabulary of {vocab} is not supported (1 to {MAX_VOCAB})")
     dev = logits.device
-    temperature = _options(temperature, torch.float32, rows, dev, "temperature", lambda low, high, total: low >= 0 and high < float("inf") and total == total, ">= 0")
-    top_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda low, high, total: low > 0 and total == total, "> 0")
-    top_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, high, total: low >= 1 and total == total, ">= 1")
+    temperature, _ = _options(temperature, torch.float32, rows, dev, "temperature", lambda low, v: low >= 0 and max(v) < float("inf"), ">= 0")
+    top_p, least_p = _options(top_p, torch.float32, rows, dev, "top_p", lambda low, _: low > 0, "> 0")
+    top_k, least_k = _options(top_k, torch.int32, rows, dev, "top_k", lambda low, _: low >= 1, ">= 1")
     if out is None:
         out = torch.empty_strided((rows, vocab), (vocab, 1), dtype=torch.float32, device=dev)
     else:
@@ -151,9 +162,8 @@ def token_probs(logits: torch.Tensor, temperature, top_p, top_k, out: Optional[t
     if rows == 0:
         return out
     # whether some row is cut: known of sequences, taken as given of tensors
-    cuts = isinstance(top_p, torch.Tensor) or isinstance(top_k, torch.Tensor) or min(top_p) < 1 or min(top_k) < vocab
-    sequences = [None if isinstance(v, torch.Tensor) else array.array("f" if i < 2 else "i", v if i < 2 else [int(k) if k < vocab else vocab for k in v])
-                 for i, v in enumerate((temperature, top_p, top_k))]
+    cuts = least_p is None or least_k is None or least_p < 1 or least_k < vocab
+    sequences = [None if isinstance(v, torch.Tensor) else _packed("f" if i < 2 else "i", v, vocab) for i, v in enumerate((temperature, top_p, top_k))]
     at = [v.data_ptr() if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, top_k)]
     given = None
     if any(v is not None for v in sequences):
