@@ -406,12 +406,13 @@ __device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum a
     int open = span ? 32 - __clz(span) : 1;            // bits that are not decided yet
     while (open > 0) {
         const int shift = max(0, open - 8);
+        const unsigned int digits = 1u << (open - shift);       // (the last ones may be fewer than 256: a key above them has been counted)
         __syncthreads();
         if (threadIdx.x < 256) { sh.mass[threadIdx.x] = 0; sh.count[threadIdx.x] = 0; }
         __syncthreads();
         each([&](unsigned int k, int, float w) {
             const unsigned int digit = ((k - base) >> shift) - (border >> shift);       // (border's undecided bits are zeros)
-            if (digit < 256u && k - base >= border) {
+            if (digit < digits && k - base >= border) {
                 atomicAdd(&sh.count[digit], 1u);
                 atomicAdd(&sh.mass[digit], tp_fixed(w));
             }

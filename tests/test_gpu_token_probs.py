@@ -140,6 +140,33 @@ def test_rows_of_every_kind_together(vocab, times):
     assert (got[2].double() - want).abs().max() <= 4e-6 and torch.equal(got[2] > 0, want > 0)
 
 
+@pytest.mark.parametrize("vocab", [300, 6000, 30000])
+@pytest.mark.parametrize("apart", [1, 3, 40])
+def test_logits_a_few_steps_apart_at_the_cut(vocab, apart):
+    """Logits whose last places alone tell them apart, the cut at each of them in turn, and a smallest one that makes the keys differ in any number of bits."""
+    near = 1.0 + torch.arange(60).flip(0) * apart * 2.0 ** -23
+    rows, ts, ps, ks = [], [], [], []
+    for i in range(60):
+        row = torch.full((vocab,), -float("inf"))
+        at = torch.randperm(vocab, generator=torch.Generator().manual_seed(i))
+        row[at[:60]] = near
+        row[at[60:160]] = near[-1] - 2.0 ** (i % 24 - 22) * (1 + torch.arange(100) / 100)
+        rows.append(row)
+        ts.append(1.0)
+        ps.append(1.0 if i % 3 else 0.5)
+        ks.append(i + 1 if i % 3 else vocab)
+    logits = torch.stack(rows)
+    got = run(logits, ts, ps, ks)
+    cut = [i for i in range(60) if i % 3 == 0]
+    check(got[cut], logits[cut], [1.0] * 20, [0.5] * 20, [vocab] * 20, f"{apart} steps apart")
+    for i in range(60):
+        if i % 3:                       # as many entries as were asked for, and the first of them (`check` would take the oracle's 1e-17 behind them for an entry)
+            kept = logits[i] >= near[i]
+            assert int(kept.sum()) == i + 1 and torch.equal((got[i] > 0).cpu(), kept)
+            want = torch.softmax(logits[i][kept].double(), 0)
+            assert ((got[i].cpu()[kept] / want - 1).abs() <= 5.2e-6).all()
+
+
 def test_masked_logits():
     inf, low = float("inf"), torch.finfo(torch.float32).min
     v = 5000
