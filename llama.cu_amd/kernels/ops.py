@@ -2808,12 +2808,12 @@ def _mx4_source(x: torch.Tensor, what: str) -> torch.Tensor:
     return x
 
 
-def _mx4_state(scales: torch.Tensor, stream: int) -> Optional[Tuple[int, int]]:
+def _mx4_state(scales: torch.Tensor, stream: int) -> Optional[Tuple[int, int, int]]:
     """What tells whether scales were written to since, or are to be in the replays of a graph: the tensor's version and the number of the capture that is under way
-    (None: the tensor counts no versions)."""
+    (None: the tensor counts no versions).  And the stream: who uses rows on another one says so to the allocator of ``codes`` and ``scales``, which are all that they know of."""
     if scales.is_inference():
         return None
-    return scales._version, bind("mx4", "lcu_capture_id", "")(stream)
+    return scales._version, bind("mx4", "lcu_capture_id", "")(stream), stream
 
 
 def mx4_quantize(x: torch.Tensor) -> Mx4:

@@ -387,3 +387,22 @@ def test_two_streams_at_once():
                 got[i].append(ops.gemm_mx4(xs[i], w))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+
+
+def test_rows_in_4_bits_on_another_stream():
+    """Rows that another stream made: what their maker keeps beside the codes and scales is not read, for nobody can tell its allocator of that use."""
+    from llama_cu_amd.kernels import ops
+    n, k, m = 64, 288, 200
+    w, _ = weight(n, k)
+    q = ops.mx4_quantize(rnd(m, k, seed=1).bfloat16().cuda())
+    want = ops.gemm_mx4(q, w, out_dtype=torch.float32)
+    blocks = q.scales.shape[1]
+    whole = ops._mx4_whole(q, blocks)
+    assert ops._mx4_by_pair(whole, blocks, ops.raw_stream()) is q._by_pair
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = ops._mx4_by_pair(whole, blocks, ops.raw_stream())
+        got = ops.gemm_mx4(q, w, out_dtype=torch.float32)
+    torch.cuda.current_stream().wait_stream(side)
+    assert there.data_ptr() != q._by_pair.data_ptr() and torch.equal(there, q._by_pair) and torch.equal(got, want)
