@@ -7,21 +7,21 @@
 //   count   a histogram of the distances (l_0 - l) / T, counts alone;
 //   write   a bin's weights are known to within its width, so the bins in which the cut can lie are known from the counts, and which entries are kept in full.  Rows
 //           without a cut are written.  Of the others what is not kept becomes zero; entries that are, or may be, are gathered;
-//   cut     one workgroup a row finds the cut among the gathered entries, eight bits of their order at a time, on sums of 64-bit fixed-point
-//           weights (w 2^44: no order of additions changes them), and writes their shares.
+//   cut     one workgroup a row finds the cut among the gathered entries of those bins, eight bits of their order at a time until few are left, and among these
+//           by what precedes each, on sums of 64-bit fixed-point weights (w 2^44: no order of additions changes them), and writes the gathered ones' shares.
 // Where more entries are kept than are gathered (a flat row) only those near the cut are, with the exact sum of what lies above, and the
 // last launch
 //   store   writes the whole row.
 // Where even those near the cut are too many (tens of thousands of equal logits) `cut` searches the row itself.
 //
 // Bound by memory where there are many rows, and each launch's latency where there are few: 320 rows of 128,256 with cuts of every kind 185 us out of memory (max 55, the logits' one
-// trip; count 28, out of the last cache; write 62, at a copy's rate; cut 18 to 23; store 14), 5 rows 30 (5.7, 5.9, 10, 9 and the gaps between them).
+// trip; count 28, out of the last cache; write 62, at a copy's rate; cut 18 to 22; store 14), 5 rows 28 (5.7, 5.9, 10.5, 7 and the gaps between them).
 //
 // A NaN counts as -inf, which has no share; a row of nothing else becomes zeros.  Infinities of the one sign share alike.  A temperature
 // that is not positive leaves the first of the largest logits.
 #include "common.h"
 
-constexpr int TP_THREADS = 512, TP_CUT_THREADS = 1024, TP_BINS = 8192, TP_GATHER = 8192, TP_EACH = TP_GATHER / TP_CUT_THREADS, TP_MAX_PARTS = 32, TP_MAX_VOCAB = 1 << 19, TP_SMALL = 8 * TP_CUT_THREADS;
+constexpr int TP_THREADS = 512, TP_CUT_THREADS = 1024, TP_BINS = 8192, TP_GATHER = 8192, TP_EACH = TP_GATHER / TP_CUT_THREADS, TP_MAX_PARTS = 32, TP_MAX_VOCAB = 1 << 19, TP_SMALL = 8 * TP_CUT_THREADS, TP_FEW = 32;
 constexpr double TP_ONE = 17592186044416.0;          // 2^44: 2^19 weights of 1 are 2^63
 constexpr float TP_NOTHING = 126.f;                  // the exponential ends at 2^-126
 constexpr float TP_LOG2E = 1.44269504088896341f;
@@ -35,6 +35,7 @@ struct TpRow {
     unsigned long long mass_above;                   // of entries kept in full that are not gathered
     unsigned int gathered;
     unsigned int before, upto;                       // how many entries lie in the bins before those in which the cut can lie, and up to the last of them
+    int first_bin;                                   // of those bins
     // the cut: which key, which of the equal ones is the last that is kept, and the part that it has, the scale of what is kept whole
     unsigned int border;
     int last, store;                                 // store: the row is yet to be written
@@ -334,7 +335,7 @@ tp_write_kernel(const float *__restrict__ logits, size_t ld, int vocab, const fl
     __shared__ __attribute__((aligned(16))) TpEntry mine[TP_GATHER / 2];
     static_assert(sizeof(mine) >= TP_BINS * sizeof(unsigned int), "the counts, and then the entries");
     const TpBracket b = tp_bracket(c, hist + (size_t)r * TP_BINS, (uint4 *)mine);
-    if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].before = b.before; rows[r].upto = b.upto; }
+    if (blockIdx.y == 0 && threadIdx.x == 0) { rows[r].before = b.before; rows[r].upto = b.upto; rows[r].first_bin = b.lo; }
     const int how = tp_how(b);
     if (how == TP_SEARCH) return;
     const int from = how == TP_ALL ? 0 : b.lo;
@@ -392,19 +393,23 @@ struct TpShared {
     unsigned long long mass[256];
     unsigned int count[256], found[2];
     TpSum found_above;
+    TpEntry few[TP_FEW];
+    unsigned int n_few;
+    TpRow cut;
 };
 
 // The cut among the entries that `each` goes through (f(key, index, weight)); above: what lies over all of them, base and span: the smallest key of them and how far the largest lies from
-// it.  Every thread of the workgroup (256 or more) calls it and gets the answer.
+// it; left: how many they are, or more than that.  Every thread of the workgroup (256 or more) calls it and gets the answer.
 template <class Each>
-__device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum above, unsigned int base, unsigned int span, Each each) {
+__device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum above, unsigned int base, unsigned int span, unsigned int left, Each each) {
     const int lane = threadIdx.x & 63;
-    const unsigned long long limit_p = c.limit_p < 524288.0 ? (unsigned long long)(c.limit_p * TP_ONE) : ~0ull;
+    // (at least a unit, of which the first entry then has all)
+    const unsigned long long limit_p = c.limit_p < 524288.0 ? max(1ull, (unsigned long long)(c.limit_p * TP_ONE)) : ~0ull;
     // the digits of the largest key at which the entries down to it reach one of the limits; `above`: what lies over the keys with the digits so far
     unsigned int border = 0;                           // (less the smallest key)
     bool all = false;                                  // (the limits lie a rounding beyond all there is)
     int open = span ? 32 - __clz(span) : 1;            // bits that are not decided yet
-    while (open > 0) {
+    while (open > 0 && left > TP_FEW) {
         const int shift = max(0, open - 8);
         const unsigned int digits = 1u << (open - shift);       // (the last ones may be fewer than 256: a key above them has been counted)
         __syncthreads();
@@ -454,7 +459,56 @@ __device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum a
         above = sh.found_above;
         if (sh.found[0] == 256u) { all = true; break; }
         border |= sh.found[0] << shift;
+        left = sh.count[sh.found[0]];
         open = shift;
+    }
+    if (!all && left <= TP_FEW) {                      // a lane an entry: what precedes it, and itself, in one turn (digit by digit to the end: the launch 9.2 us of 5 rows and 24.5 of 320, so 7.0 and 21.9)
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n_few = 0;
+        __syncthreads();
+        each([&](unsigned int k, int i, float) {
+            if ((unsigned long long)((k - base) ^ border) >> open == 0) {
+                const unsigned int place = atomicAdd(&sh.n_few, 1u);
+                if (place < TP_FEW) sh.few[place] = {k, i};
+            }
+        });
+        __syncthreads();
+        if (threadIdx.x < WAVE) {
+            const unsigned int n = min((unsigned int)__builtin_amdgcn_readfirstlane(sh.n_few), (unsigned int)TP_FEW);
+            const TpEntry mine = lane < (int)n ? sh.few[lane] : TpEntry{0u, 0x7fffffff};
+            const unsigned long long w = lane < (int)n ? tp_fixed(tp_weight(tp_distance(c, tp_logit(mine.key)))) : 0ull;
+            TpSum before = above;
+            for (unsigned int j = 0; j < n; ++j) {
+                const unsigned int k = __builtin_amdgcn_readlane(mine.key, j);
+                const int i = __builtin_amdgcn_readlane(mine.at, j);
+                const unsigned long long w_j = (unsigned long long)(unsigned int)__builtin_amdgcn_readlane((int)(w >> 32), j) << 32 | (unsigned int)__builtin_amdgcn_readlane((int)w, j);
+                if (k > mine.key || (k == mine.key && i < mine.at)) { before.mass += w_j; ++before.count; }
+            }
+            const unsigned long long with = before.mass + w;
+            const bool by_k = before.count + 1 >= (unsigned int)c.k, reached = lane < (int)n && (by_k || with >= limit_p);
+            const bool first = reached && before.count < (unsigned int)c.k && before.mass < limit_p;      // (and none before it)
+            TpRow t = {};
+            t.last = 0x7fffffff;
+            t.kept = -1.f;
+            if (first) {
+                const unsigned long long limit = by_k ? min(limit_p, with) : limit_p, kept = limit - before.mass;
+                if (kept < w) t.kept = (float)((double)kept / (double)limit);
+                t.border = mine.key;
+                t.last = mine.at;
+                t.inv = (float)(TP_ONE / (double)limit);
+                sh.cut = t;
+            }
+            if (__ballot(first) == 0) {                // (the limits lie a rounding beyond all there is)
+                unsigned long long total = w;
+#pragma unroll
+                for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, WAVE);
+                total += above.mass;
+                t.inv = total ? (float)(TP_ONE / (double)total) : 0.f;
+                if (lane == 0) sh.cut = t;
+            }
+        }
+        __syncthreads();
+        return sh.cut;
     }
     TpRow t = {};
     t.last = 0x7fffffff;
@@ -471,48 +525,39 @@ __device__ __forceinline__ TpRow tp_search(const TpCut &c, TpShared &sh, TpSum a
         const unsigned long long kept = limit - above.mass - (unsigned long long)(rank - 1) * each_mass;
         if (kept < each_mass) t.kept = (float)((double)kept / (double)limit);
         t.border = border;
-        // the rank-th smallest index among the equal ones, eight bits at a time
+        // the rank-th smallest index among the equal ones (more than a few), eight bits at a time
         unsigned int index = 0;
-        if (equal > 1) {
-            unsigned int left = rank;
-            for (int shift = 16; shift >= 0; shift -= 8) {
-                __syncthreads();
-                if (threadIdx.x < 256) sh.count[threadIdx.x] = 0;
-                __syncthreads();
-                each([&](unsigned int k, int i, float) {
-                    if (k == border && (shift == 16 || ((unsigned int)i ^ index) >> (shift + 8) == 0)) atomicAdd(&sh.count[(unsigned int)i >> shift & 255], 1u);
-                });
-                __syncthreads();
-                if (threadIdx.x < WAVE) {
-                    unsigned int mine = 0, n[4];
+        left = rank;
+        for (int shift = 16; shift >= 0; shift -= 8) {
+            __syncthreads();
+            if (threadIdx.x < 256) sh.count[threadIdx.x] = 0;
+            __syncthreads();
+            each([&](unsigned int k, int i, float) {
+                if (k == border && (shift == 16 || ((unsigned int)i ^ index) >> (shift + 8) == 0)) atomicAdd(&sh.count[(unsigned int)i >> shift & 255], 1u);
+            });
+            __syncthreads();
+            if (threadIdx.x < WAVE) {
+                unsigned int mine = 0, n[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { n[e] = sh.count[4 * lane + e]; mine += n[e]; }
-                    unsigned int scan = mine;
+                for (int e = 0; e < 4; ++e) { n[e] = sh.count[4 * lane + e]; mine += n[e]; }
+                unsigned int scan = mine;
 #pragma unroll
-                    for (int off = 1; off < WAVE; off <<= 1) {
-                        const unsigned int up = __shfl_up(scan, off, WAVE);
-                        if (lane >= off) scan += up;
-                    }
-                    unsigned int so_far = scan - mine;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (so_far < left && left <= so_far + n[e]) { sh.found[0] = 4 * lane + e; sh.found[1] = so_far; }
-                        so_far += n[e];
-                    }
+                for (int off = 1; off < WAVE; off <<= 1) {
+                    const unsigned int up = __shfl_up(scan, off, WAVE);
+                    if (lane >= off) scan += up;
                 }
-                __syncthreads();
-                index |= sh.found[0] << shift;
-                left -= sh.found[1];
+                unsigned int so_far = scan - mine;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (so_far < left && left <= so_far + n[e]) { sh.found[0] = 4 * lane + e; sh.found[1] = so_far; }
+                    so_far += n[e];
+                }
             }
-            t.last = (int)index;
-        }
-        // (a single one: whatever its index, it is the last)
-        if (equal == 1) {
             __syncthreads();
-            each([&](unsigned int k, int i, float) { if (k == border) sh.found[0] = (unsigned int)i; });
-            __syncthreads();
-            t.last = (int)sh.found[0];
+            index |= sh.found[0] << shift;
+            left -= sh.found[1];
         }
+        t.last = (int)index;
     }
     t.inv = limit ? (float)(TP_ONE / (double)limit) : 0.f;
     return t;
@@ -536,6 +581,7 @@ tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
     // gridDim.y workgroups a row, which all find its cut: with more than one each writes its part of a row that is yet to be written
     __shared__ TpShared sh;
     __shared__ unsigned int key_lo, key_hi;
+    __shared__ unsigned long long mass_before;
     const int r = blockIdx.x, lane = threadIdx.x & 63;
     const TpCut c = tp_row(part + (size_t)r * parts, parts, vocab, temperature[r], top_p[r], top_k[r]);
     if (c.empty || c.greedy || !c.cuts) {
@@ -556,19 +602,30 @@ tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
         key[e] = t.key;
         at[e] = t.at;
     }
-    // the digits are those of the distance from the smallest key: the keys' own first digit is the exponent, which nearly all share, and their additions
-    // would wait for each other
-    if (threadIdx.x == 0) { key_lo = 0xffffffffu; key_hi = 0; }
+    // What lies in the bins before those of the cut is added up, and only the others are searched (of 8,192 gathered entries all searched: their additions by digits wait for each other).  The digits are
+    // those of the distance from the smallest key: the keys' own first digit is the exponent, which nearly all share.
+    if (threadIdx.x == 0) { key_lo = 0xffffffffu; key_hi = 0; mass_before = 0; }
     __syncthreads();
-    unsigned int lowest = 0xffffffffu, highest = 0;
+    unsigned int lowest = 0xffffffffu, highest = 0, near = 0;         // near: a bit an entry of the thread's
+    unsigned long long mass = 0;
 #pragma unroll
     for (int e = 0; e < TP_EACH; ++e)
-        if (e * TP_CUT_THREADS + threadIdx.x < gathered) { lowest = min(lowest, key[e]); highest = max(highest, key[e]); }
+        if (e * TP_CUT_THREADS + threadIdx.x < gathered) {
+            const float d = tp_distance(c, tp_logit(key[e]));
+            if (tp_bin(c, d) >= b.first_bin) { near |= 1u << e; lowest = min(lowest, key[e]); highest = max(highest, key[e]); }
+            else mass += tp_fixed(tp_weight(d));
+        }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) { lowest = min(lowest, (unsigned int)__shfl_xor(lowest, off, WAVE)); highest = max(highest, (unsigned int)__shfl_xor(highest, off, WAVE)); }
+    for (int off = 32; off > 0; off >>= 1) {
+        lowest = min(lowest, (unsigned int)__shfl_xor(lowest, off, WAVE));
+        highest = max(highest, (unsigned int)__shfl_xor(highest, off, WAVE));
+        mass += __shfl_xor(mass, off, WAVE);
+    }
     if (lane == 0 && highest) { atomicMin(&key_lo, lowest); atomicMax(&key_hi, highest); }
+    if (lane == 0 && mass) atomicAdd(&mass_before, mass);
     __syncthreads();
-    const unsigned int base = how == TP_SEARCH || gathered == 0 ? 0u : key_lo, span = how == TP_SEARCH || gathered == 0 ? ~0u : key_hi - key_lo;
+    const bool any = how != TP_SEARCH && key_hi;
+    const unsigned int base = any ? key_lo : 0u, span = any ? key_hi - key_lo : ~0u;
     // f(key, index, weight) of every entry that is looked at
     auto each = [&](auto f) {
         if (how == TP_SEARCH) {
@@ -579,10 +636,11 @@ tp_cut_kernel(const float *__restrict__ logits, size_t ld, int vocab, const floa
         } else {
 #pragma unroll
             for (int e = 0; e < TP_EACH; ++e)
-                if (e * TP_CUT_THREADS + threadIdx.x < gathered) f(key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
+                if (near >> e & 1) f(key[e], at[e], tp_weight(tp_distance(c, tp_logit(key[e]))));
         }
     };
-    TpRow t = tp_search(c, sh, how == TP_NEAR ? TpSum{b.mass_above, b.before} : TpSum{0, 0}, base, span, each);
+    TpRow t = tp_search(c, sh, how == TP_SEARCH ? TpSum{0, 0} : TpSum{how == TP_NEAR ? b.mass_above : mass_before, b.before}, base, span,
+                        how == TP_SEARCH ? ~0u : b.upto - b.before, each);
     t.store = how != TP_ALL;
     if (how == TP_ALL) {
         if (blockIdx.y > 0) return;
@@ -682,7 +740,7 @@ tp_small_kernel(const float *__restrict__ logits, size_t ld, int vocab, TpOption
     t.kept = -1.f;
     t.inv = (float)(1.0 / c.sum);
     if (!c.empty && !c.greedy && c.cuts)
-        t = tp_search(c, sh, TpSum{0, 0}, key_lo, key_hi - key_lo, [&](auto f) {
+        t = tp_search(c, sh, TpSum{0, 0}, key_lo, key_hi - key_lo, (unsigned int)vocab, [&](auto f) {
 #pragma unroll
             for (int e = 0; e < EACH; ++e) {
                 const float d = tp_distance(c, l[e]);

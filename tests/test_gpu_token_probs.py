@@ -167,6 +167,17 @@ def test_logits_a_few_steps_apart_at_the_cut(vocab, apart):
             assert ((got[i].cpu()[kept] / want - 1).abs() <= 5.2e-6).all()
 
 
+@pytest.mark.parametrize("vocab", [5, 300, 6000, 30000])
+def test_a_top_p_of_nearly_nothing(vocab):
+    """The first entry has all, however small the part of the sum is that is asked for."""
+    logits = rnd(4, vocab, seed=vocab)
+    logits[1] = 0.0
+    for p in (1e-12, 1e-14, 1e-20, 1e-38):
+        for k in (vocab, 3):
+            got = run(logits, [1.0] * 4, [p] * 4, [k] * 4).cpu()
+            assert torch.equal(got, torch.nn.functional.one_hot(logits.argmax(1), vocab).float()), (p, k)
+
+
 def test_masked_logits():
     inf, low = float("inf"), torch.finfo(torch.float32).min
     v = 5000
