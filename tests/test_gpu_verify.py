@@ -198,3 +198,64 @@ def test_strides_and_capture():
         torch.cuda.synchronize()
         want = sampling.verify_drafts(*args, 4, qs)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("v", [700, 9000, 40000])
+def test_two_graphs_and_two_streams(v):
+    """Distributions and their verification: two graphs replayed in turn and at once on two streams, with calls of the program's own between them."""
+    from llama_cu_amd.sampling import token_probs, verify_drafts
+    requests, most = 30, 4
+    rows, n = requests * (most + 1), requests * most            # (more than 64 rows: options go through pinned memory outside a graph)
+    starts = torch.arange(0, rows + 1, most + 1, dtype=torch.int32).cuda()
+    opts = ([0.6 + 0.01 * (r % 70) for r in range(rows)], [0.8 + 0.001 * (r % 200) for r in range(rows)], [v if r % 3 else 1 + r for r in range(rows)])
+    there = [torch.tensor(opts[0]).cuda(), torch.tensor(opts[1]).cuda(), torch.tensor(opts[2], dtype=torch.int32).cuda()]
+
+    def fill(state, seed):
+        g = torch.Generator().manual_seed(seed)
+        state["logits"].copy_(torch.randn(rows, v, generator=g) * 2.5)
+        state["drafts"].copy_(torch.randint(0, v, (n,), generator=g, dtype=torch.int32))
+        # some drafts that the target likes
+        best = state["logits"].argmax(1).view(requests, most + 1)[:, :most].reshape(-1).int()
+        state["drafts"][::2] = best[::2]
+        for name in ("accept", "final"):
+            state[name].copy_(torch.randint(0, 1 << 24, state[name].shape, generator=g).float() / (1 << 24))
+
+    def make():
+        return dict(logits=torch.empty(rows, v, device="cuda"), drafts=torch.empty(n, dtype=torch.int32, device="cuda"), accept=torch.empty(n, device="cuda"), final=torch.empty(requests, device="cuda"))
+
+    def work(s, options):
+        probs = token_probs(s["logits"], *options)
+        return (probs,) + verify_drafts(probs, starts, s["drafts"], s["accept"], s["final"], most)
+
+    states, graphs, outs = [make(), make()], [], []
+    for i, s in enumerate(states):
+        fill(s, i)
+        work(s, there)
+    torch.cuda.synchronize()
+    for s in states:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(work(s, there))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(4):
+        for i, s in enumerate(states):
+            fill(s, 10 * turn + i)
+        torch.cuda.synchronize()
+        if turn % 2:
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        else:
+            graphs[1].replay()
+            graphs[0].replay()
+        eager = []
+        for s, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                eager.append([work(s, opts) for _ in range(3)])
+        torch.cuda.synchronize()
+        for s, out, calls in zip(states, outs, eager):
+            want = work(s, there)
+            for got in [out] + calls:
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+        assert int(outs[0][1].sum()) > 0
