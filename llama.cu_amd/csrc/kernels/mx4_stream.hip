@@ -1,14 +1,14 @@
 // Y[M, N] = X[M, K] * W[N, K]^T with W in microscaled 4-bit numbers (mx4.h), 32-bit sums: the kernels that stream W past up to 64 rows.
 //
-// A workgroup takes NT tiles of 16 features (for SwiGLU the gate rows of a tile and the up rows that meet them) and 16 MT rows; its eight waves share
-// out K in pairs of macro-steps (256 k) and add their partial sums through LDS in a fixed order.  Rows of bfloat16: the codes become bfloat16
+// A workgroup takes NT tiles of 16 features (for SwiGLU the gate rows of a tile and the up rows that meet them) and 16 MT rows; its eight waves (four where there are more workgroups than
+// the card holds at once) share out K in pairs of macro-steps (256 k) and add their partial sums through LDS in a fixed order.  Rows of bfloat16: the codes become bfloat16
 // in registers, exactly and with their scale, two a conversion, in the order in which the matrix instruction of 16 x 16 x 32 wants its operand.  Rows of
 // float32 come as three planes of bfloat16 whose sum they are, each multiplied with the same codes.  Rows in 4 bits: the scaled instruction of 16 x 16 x 128
 // takes both sides' codes and scales as they are.
 //
 // Bound by memory where the weight is large, by the latency of a wave's chain of loads where it is not (a wave has K / 8, of which two pairs of macro-steps are on their way; K is
-// split over the waves of one workgroup and no further, so that no second launch adds the parts).  One row: 6144 x 4096 5.2 us (2.6 TB/s), 128256 x 4096 59 (4.7 TB/s); 8 rows: 28672 x
-// 4096 with the activation 15.1 us (4.1 TB/s), 57344 x 8192 54 (4.6).  Beyond 8 rows every workgroup's reading of all rows out of the L2 caches weighs more and the products in tiles take over.
+// split over the waves of one workgroup and no further, so that no second launch adds the parts).  One row: 6144 x 4096 5.2 us (2.6 TB/s), 128256 x 4096 48 (5.8 TB/s); 8 rows: 28672 x
+// 4096 with the activation 13.6 to 14.9 us (4.2 to 4.6 TB/s), 57344 x 8192 51 (4.9).  Beyond 8 rows every workgroup's reading of all rows out of the L2 caches weighs more and the products in tiles take over.
 #include "mx4.h"
 #include "mx4/matrix.h"
 #include "gate_act.h"
@@ -240,6 +240,17 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
     mx4_finish<NT, MT, EPI>(a, row0, acc, red, [](int c) { return c; });
 }
 
+// How many workgroups of eight waves the card holds at once.
+static long long mx4_held(const void *kernel) {
+    int each = 0, device = 0, units = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, MX4_WAVES * WAVE, 0) != hipSuccess || hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) {
+        (void)hipGetLastError();
+        return 1ll << 40;
+    }
+    return (long long)each * units;
+}
+
 // codes, scales: W in the products' order, [ceil(N / 16)][pairs] blocks, 16-byte aligned.  x_kind: 1 bfloat16 rows [M, ldx]; 3 float32 rows as
 // planes [M][3][ldx / 3]; 4 codes [M, ldx] bytes with scales xs [M, lds] bytes; all of
 // them in whole macro-steps of 128 k, zeros behind K.  epi: MX4_EPI_*; SwiGLU: N counts gate and up rows.
@@ -254,15 +265,24 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
         : x_kind == 4 ? ldx % 16 || lds % 4 || !xs || (uintptr_t)xs % 4 || lds >= MX4_MAX_LDX || (M > 1 && (ldx < 64ll * macros || lds < 4ll * macros)) : true)
         return LCU_BAD_ARGUMENT;
     const Mx4Args a = {(const uint8_t *)codes, (const uint8_t *)scales, pairs, macros, y, ldy, M, N, ((uintptr_t)y | (uintptr_t)(ldy * elem)) % (4 * elem) == 0};
-    const int tiles = (cols + 15) / 16, waves = min(MX4_WAVES, x_kind == 4 ? macros : (macros + 1) / 2);
-    const dim3 block(waves * WAVE);
+    const int tiles = (cols + 15) / 16, work = x_kind == 4 ? macros : (macros + 1) / 2;
     // two tiles of features a workgroup where there are many, and more than four rows are read for them (us, one tile / two: 16384 x 2048 16 rows 10.8 / 9.5, 28672 x 4096 16 rows 26.1 / 24.9,
     // 128256 x 4096 8 rows 70.6 / 65.1; one row 58.9 / 59.7; 4096 x 14336 8 rows 13.1 / 15.6)
     const bool pairs_of = x_kind == 1 && M > 4 && M <= 16 && N > 8192 && epi < MX4_EPI_SWIGLU;
     auto grid = [&](int nt, int mt) { return dim3(epi >= MX4_EPI_SWIGLU ? tiles : (tiles + nt - 1) / nt, (M + 16 * mt - 1) / (16 * mt)); };
     if ((M + 15) / 16 > 65535) return LCU_BAD_ARGUMENT;
-#define GO(NT, MT, PLANES, EPI, LOADS) mx4_stream_kernel<NT, MT, PLANES, EPI, LOADS><<<grid(NT, MT), block, 0, stream>>>((const bf16_t *)x, (int)ldx, (int)(PLANES == 3 ? ldx / 3 : 0), a)
-#define GO4(NT, MT, EPI) mx4_stream4_kernel<NT, MT, EPI><<<grid(NT, MT), block, 0, stream>>>((const uint8_t *)x, (int)ldx, (const uint8_t *)xs, (int)lds, a)
+    // Eight waves a workgroup, four where the card does not hold all workgroups of eight at once: half as many waves then go through twice the K each, and there are fewer rounds, the last of
+    // them fuller (us, eight / four: 28672 x 4096 with the activation, 8 rows, 17.7 / 15.6; 128256 x 4096, one row, 55.7 / 48.1; 57344 x 8192 50.7 / 46.4; held at once: 6144 x 4096 5.5 / 6.5,
+    // 4096 x 14336 11.3 / 14.9).  Over 595 shapes and kinds of rows 1.01 times the best of two to eight waves.
+    auto block = [&](dim3 g, long long held) { return dim3(min((long long)g.x * g.y > held ? MX4_WAVES / 2 : MX4_WAVES, work) * WAVE); };
+#define RUN(NT, MT, KERNEL, ...)                                                      \
+    do {                                                                              \
+        static const long long held = mx4_held((const void *)KERNEL);                 \
+        const dim3 g = grid(NT, MT);                                                  \
+        KERNEL<<<g, block(g, held), 0, stream>>>(__VA_ARGS__);                        \
+    } while (0)
+#define GO(NT, MT, PLANES, EPI, LOADS) RUN(NT, MT, (mx4_stream_kernel<NT, MT, PLANES, EPI, LOADS>), (const bf16_t *)x, (int)ldx, (int)(PLANES == 3 ? ldx / 3 : 0), a)
+#define GO4(NT, MT, EPI) RUN(NT, MT, (mx4_stream4_kernel<NT, MT, EPI>), (const uint8_t *)x, (int)ldx, (const uint8_t *)xs, (int)lds, a)
 #define ROWS(NT, EPI)                                      \
     do {                                                   \
         if (x_kind == 4) {                                 \
@@ -286,6 +306,7 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
     else if (pairs_of) { if (epi == MX4_EPI_BF16) ROWS(2, MX4_EPI_BF16); else ROWS(2, MX4_EPI_F32); }
     else if (epi == MX4_EPI_BF16) ROWS(1, MX4_EPI_BF16);
     else ROWS(1, MX4_EPI_F32);
+#undef RUN
 #undef GO
 #undef GO4
 #undef ROWS

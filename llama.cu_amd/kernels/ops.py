@@ -2927,8 +2927,8 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
 
 
 # What the kernels of the 4-bit products take, us, fitted to 193,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory): the choice by
-# these numbers takes 1.02 times what the best choice takes, geometric mean; 1.01 of many rows, 1.06 where the streaming kernel and the tiles meet (48 and 64 rows).  Up to 8 rows (4 in
-# float32) the streaming kernel takes 1.01 to 1.03 times the best without being asked; at 16 it would be 1.09, 1.42 and 1.06.
+# these numbers takes 1.02 times what the best choice takes, geometric mean; of 10 to 64 rows, where the streaming kernel and the tiles meet, 1.01 (10,183 shapes drawn at random).  Up to 8 rows
+# of bfloat16, 4 of float32 and 12 in 4 bits the streaming kernel is taken unasked: 1.01 to 1.03 times the best; at 16 it would be 1.03, 1.37 and 1.03.
 # Tiles (features, tokens) by the kind of the rows and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three, four workgroups
 # on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
 _MX4_TILES = {
@@ -2947,7 +2947,8 @@ _MX4_TILES = {
 }
 # The kernel that streams the weight, by the kind of the rows: us a launch; a workgroup alone, and for each macro-step of a wave; a macro-step where workgroups share a compute unit, and what four
 # rows add to that.
-_MX4_STREAM = {1: (1.45, 0.87, 0.33, 0.29, 0.12), 3: (0.91, 1.87, 0.77, 0.35, 0.33), 4: (0.92, 2.56, 0.19, 0.22, 0.09)}
+_MX4_STREAM = {1: (0.88, 0.53, 0.67, 0.00, 0.13), 3: (0.91, 1.87, 0.77, 0.35, 0.33), 4: (0.92, 2.56, 0.19, 0.22, 0.09)}
+_MX4_UNASKED = {1: 8, 3: 4, 4: 12}
 _MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
 
 
@@ -2955,7 +2956,7 @@ _MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
 def _mx4_choice(m: int, n: int, k: int, kind: int, cu: int) -> Tuple[int, int]:
     macros = -(-k // 128)
     best = (float("inf"), -1, 1)
-    if m <= (4 if kind == 3 else 8):
+    if m <= _MX4_UNASKED[kind]:
         return -1, 1
     if m <= 64:
         tiles = 1 if m <= 16 else 2 if m <= 32 or kind == 3 else 4        # of 16 rows, together
