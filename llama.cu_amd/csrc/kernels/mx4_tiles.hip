@@ -38,9 +38,10 @@ template <bool FOUR_, int FT_, int TT_, int WF_, int WT_, int SF_, int ST_, int 
     static constexpr int FP = FOUR ? 8 : 2, TP = 8;                    // pieces (16 bytes) of a row a stage
     static constexpr int STEP_CODES = 256 * FP;                        // bytes of a tile of 16 features a step
     static constexpr int LF = F * FP / WAVE / WAVES, LT = P * T * TP / WAVE / WAVES;       // loads of a wave a stage
-    static constexpr int LS = FOUR ? FT + TT : FT;                     // and of scales, into registers
     static constexpr int LDS = SF * F * FP + ST * P * T * TP;              // pieces
-    static constexpr int LEFT = (SF > ST ? LF : 0) + (ST - 2) * (LF + LT + LS);        // loads that may be on their way when a step begins
+    // Loads that may be on their way when a step begins: the rings' that are asked for behind the last of the step's own stages (a turn asks for tokens and then for features, and of the first step's
+    // stages the features, further ahead, come first).  Scales' loads are not counted, wherever the compiler puts them among these: more of them on their way make the wait longer, never shorter.
+    static constexpr int LEFT = (SF > ST ? LF : 0) + (ST - 2) * (LF + LT);
     static_assert(FT % 2 == 0 && F * FP % (WAVE * WAVES) == 0 && T * P * TP % (WAVE * WAVES) == 0 && (P == 1 || !FOUR) && SF >= ST && ST >= 2 && LDS * 16 <= 160 * 1024, "whole loads, and room for the stages");
 };
 
@@ -236,17 +237,17 @@ mx4_tiles_kernel(MtArgs a) {
     // the features' ring's step (behind the last one: the first, which nobody reads)
     int wf_step = first;
     auto next_w = [&](int s) { return s + 1 == a.steps ? 0 : s + 1; };
-    // what SF - 1 turns before the first would have asked for
+    // what SF - 1 turns before the first would have asked for, in the turns' order
     int s_step = wf_step;
     fetch_scales(next, first, s_step);
 #pragma unroll
     for (int j = 1 - S::SF; j < 0; ++j) {
         if (j + S::ST - 1 >= 0) {
 #pragma unroll
-            for (int i = 0; i < S::LT; ++i) issue_t(lds_t + (j + S::ST - 1) * S::P * S::T * S::TP, j + S::ST - 1, i);
+            for (int i = 0; i < S::LT; ++i) { issue_t(lds_t + (j + S::ST - 1) * S::P * S::T * S::TP, j + S::ST - 1, i); __builtin_amdgcn_sched_barrier(0); }
         }
 #pragma unroll
-        for (int i = 0; i < S::LF; ++i) issue_f(lds_f + (j + S::SF - 1) * S::F * S::FP, wf_step, i);
+        for (int i = 0; i < S::LF; ++i) { issue_f(lds_f + (j + S::SF - 1) * S::F * S::FP, wf_step, i); __builtin_amdgcn_sched_barrier(0); }
         wf_step = next_w(wf_step);
     }
     int rf = 0, rt = 0, df = S::SF - 1, dt = S::ST - 1;
