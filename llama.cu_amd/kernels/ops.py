@@ -3048,7 +3048,7 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         rows, kind = _mx4_rows(x, k)
         ld, lds, xs = rows.stride(0) if m > 1 else rows.shape[1], 0, None
         row_bytes = 2 * ld
-    shape, slices = _mx4_choice(m, n, k, kind, TUNING.compute_units)
+    shape, slices = mx4_choice(m, n, k, kind)
     most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
     if shape >= 0 and (most < 512 or (n + 528) * w.pairs * 128 >= 1 << 32):
         shape = -1
