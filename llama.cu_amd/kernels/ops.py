@@ -2950,6 +2950,8 @@ _MX4_TILES = {
 _MX4_STREAM = {1: (0.88, 0.53, 0.67, 0.00, 0.13), 3: (0.91, 1.87, 0.77, 0.35, 0.33), 4: (0.92, 2.56, 0.19, 0.22, 0.09)}
 _MX4_UNASKED = {1: 8, 3: 4, 4: 12}
 _MX4_SLICES = (1, 2, 3, 4, 5, 6, 8, 10, 12, 16)
+_MX4_PLACES = 1 << 32             # a load's place in the products in tiles has 32 bits: the bytes of one call's rows, of their scales and of the weight
+_MX4_STREAM_ROWS = 65535 * 16     # rows of one call of the kernel that streams the weight: tiles of 16 in a launch's second dimension
 
 
 @functools.lru_cache(maxsize=8192)
@@ -2989,6 +2991,10 @@ def _mx4_by_pair(q: Mx4, blocks: int, stream: int) -> torch.Tensor:
     scales = q._scales
     if q._by_pair is not None and q._of == _mx4_state(scales, stream):
         return q._by_pair
+    return _mx4_lay_by_pair(scales, blocks, stream)
+
+
+def _mx4_lay_by_pair(scales: torch.Tensor, blocks: int, stream: int) -> torch.Tensor:
     rows, pairs = scales.shape[0], -(-blocks // 8)
     out = torch.empty_strided((pairs, rows, 8), (8 * rows, 8, 1), dtype=torch.uint8, device=scales.device)
     _check(bind("mx4", "lcu_mx4_by_pair", "pllip")(scales.data_ptr(), scales.stride(0), rows, pairs, out.data_ptr(), stream), "gemm_mx4 scales")
@@ -3049,23 +3055,34 @@ def gemm_mx4(x, w: PackedMx4, out: Optional[torch.Tensor] = None, out_dtype: Opt
         ld, lds, xs = rows.stride(0) if m > 1 else rows.shape[1], 0, None
         row_bytes = 2 * ld
     shape, slices = mx4_choice(m, n, k, kind)
-    most = ((1 << 32) - 1) // max(row_bytes, lds) - 512        # rows of one call of the product in tiles, whose loads' places are 32 bits
-    if shape >= 0 and (most < 512 or (n + 528) * w.pairs * 128 >= 1 << 32):
+    most = (_MX4_PLACES - 1) // row_bytes - 512        # rows of one call of the product in tiles (the last tile's beyond their end count too)
+    if shape >= 0 and (most < 512 or (n + 528) * w.pairs * 128 >= _MX4_PLACES):
         shape = -1
     of_out = out.stride(0) if m > 1 else cols
+    out_bytes = of_out * out.element_size()
     epilogue = (2 if swiglu else 0) + (1 if dtype == torch.float32 else 0)
     if shape < 0:
-        _check(bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")(rows.data_ptr(), ld, kind, xs, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs, out.data_ptr(), of_out, m, n, k,
-                                                                      epilogue, stream), "gemm_mx4")
+        f = bind("mx4_stream", "lcu_mx4_stream", "pliplppipliiii")
+        for r in range(0, m, _MX4_STREAM_ROWS):
+            _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + r * lds if four else None, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs, out.data_ptr() + r * out_bytes, of_out,
+                     min(_MX4_STREAM_ROWS, m - r), n, k, epilogue, stream), "gemm_mx4")
         return out
     steps = w.pairs if four else -(-k // 128) * 2
     slices = max(1, min(slices, steps))
     planes = torch.empty_strided((slices * min(m, most) * (n + 3 & -4),), (1,), dtype=torch.float32, device=device) if slices > 1 else None
-    if four:
+    # all rows' scales by pairs of macro-steps, unless their last ones lie too far from the first
+    together = not four or w.pairs * 8 * m + 4096 < _MX4_PLACES
+    if four and together:
         scales = _mx4_by_pair(q, blocks, stream)
-        xs, lds = scales.data_ptr(), 8 * m
+        first_xs, lds = scales.data_ptr(), 8 * m
     f = bind("mx4_tiles", "lcu_mx4_tiles", "pliplppipliiiiiip")
     for r in range(0, m, most):
-        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs + 8 * r if four else None, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs,
-                 out.data_ptr() + r * of_out * out.element_size(), of_out, min(most, m - r), n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), stream), "gemm_mx4")
+        piece = min(most, m - r)
+        if four and together:
+            xs = first_xs + 8 * r
+        elif four:
+            scales = _mx4_lay_by_pair(q._scales[r:r + piece], blocks, stream)
+            xs, lds = scales.data_ptr(), 8 * piece
+        _check(f(rows.data_ptr() + r * row_bytes, ld, kind, xs, lds, w.codes.data_ptr(), w.scales.data_ptr(), w.pairs,
+                 out.data_ptr() + r * out_bytes, of_out, piece, n, k, epilogue, shape, slices, None if planes is None else planes.data_ptr(), stream), "gemm_mx4")
     return out

@@ -147,3 +147,41 @@ def test_the_kernel_that_streams_the_weight(n, k, kind, force):
                 gate, up = want[:m].chunk(2, 1)
                 assert_close(ops.gemm_mx4(rows, w, out_dtype=dtype, swiglu=True), gate * torch.sigmoid(gate) * up, REL[dtype] + 2e-5, f"swiglu of {m} rows to {dtype}")
     assert asked == []
+
+
+@pytest.mark.parametrize("kind", list(SHAPES))
+@pytest.mark.parametrize("m", [1500, 17001])
+def test_rows_in_pieces(m, kind, force, monkeypatch):
+    """Rows beyond what one call takes, with a small limit in the place of the 4 GiB: the same bits in pieces as at once.  In 4 bits with the scales of all rows laid out together, and (17,001
+    rows) for each piece by itself."""
+    from llama_cu_amd.kernels import ops
+    n, k = 40, 512
+    w, exact = weight(n, k)
+    rows, mine = operands(kind, m, k)
+    row_bytes = {"bfloat16": 2, "float32": 6, "four": 0.5}[kind] * k
+    mine = mine @ exact.T
+    for slices in (1, 2):
+        asked = force(2, slices)
+        want = ops.gemm_mx4(rows, w, out_dtype=torch.float32)
+        assert_close(want, mine, REL[torch.float32], f"{kind} {slices}")
+        assert len(asked) == 1
+        with monkeypatch.context() as limit:
+            limit.setattr(ops, "_MX4_PLACES", int(row_bytes) * (512 + 513) + 1)
+            room = torch.full((m + 2, n + 5), 7.0, device="cuda")
+            got = ops.gemm_mx4(rows, w, out=room[1:1 + m, 3:3 + n])
+        assert len(asked) == 1 + -(-m // 513)
+        assert torch.equal(got, want) and (room[0] == 7).all() and (room[m + 1:] == 7).all() and (room[:, :3] == 7).all() and (room[:, 3 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", list(SHAPES))
+def test_rows_in_pieces_past_a_streamed_weight(kind, force, monkeypatch):
+    from llama_cu_amd.kernels import ops
+    m, n, k = 201, 72, 512
+    w, exact = weight(n, k)
+    rows, mine = operands(kind, m, k)
+    asked = force(-1, 1)
+    monkeypatch.setattr(ops, "_MX4_STREAM_ROWS", 64)
+    room = torch.full((m + 2, n + 5), 7.0, device="cuda")
+    got = ops.gemm_mx4(rows, w, out=room[1:1 + m, 3:3 + n])
+    assert_close(got, mine @ exact.T, REL[torch.float32], kind)
+    assert asked == [] and (room[0] == 7).all() and (room[m + 1:] == 7).all() and (room[:, :3] == 7).all() and (room[:, 3 + n:] == 7).all()

@@ -53,3 +53,59 @@ def test_the_choice_is_what_is_called(kind, shape, calls, monkeypatch):
     name, args = calls[-1]
     assert name == ("lcu_mx4_stream" if shape[0] < 0 else "lcu_mx4_tiles")
     assert shape[0] < 0 or (args["shape"], args["slices"]) == shape
+
+
+def allowed(name, a):
+    """What the library asks of sizes (``lcu_mx4_tiles``, ``lcu_mx4_stream``, ``lcu_mx4_by_pair``)."""
+    if name == "lcu_mx4_by_pair":
+        return a["lds"] >= 8 * a["pairs"] and a["rows"] > 0
+    macros = -(-a["k"] // 128)
+    if name == "lcu_mx4_stream":
+        return -(-a["m"] // 16) <= 65535 and a["ldx"] < 1 << 24
+    row_bytes = a["ldx"] * (1 if a["kind"] == 4 else 2)
+    return ((a["m"] + 512) * row_bytes < 1 << 32 and (-(-a["n"] // 16) * 16 + 512) * a["pairs"] * 128 < 1 << 32
+            and (a["kind"] != 4 or (a["lds"] >= 8 * a["m"] and (macros + 1) // 2 * a["lds"] + 4096 < 1 << 32)))
+
+
+def pieces(calls, name, m, row_bytes, out_bytes):
+    """The rows of the products' calls: all of them, one after the other, each where it belongs."""
+    at = 0
+    for entry, a in calls:
+        assert allowed(entry, a), (entry, a)
+        if entry == name:
+            assert (a["x"], a["y"]) == (at * row_bytes, at * out_bytes)
+            at += a["m"]
+    assert at == m
+
+
+@pytest.mark.parametrize("m,k", [(4_700_000, 28672), (4_900_000, 28672), (30_000_000, 4096), (40_000_001, 4096), (600_000_000, 256)])
+def test_any_number_of_rows_in_4_bits(m, k, calls):
+    """The scales of all rows are more than 32 bits say from some number of rows on: each piece of the rows then has its own laid out."""
+    w = weight(32, k)
+    ops.gemm_mx4(rows("four", m, k), w)
+    assert {name for name, _ in calls} == {"lcu_mx4_tiles", "lcu_mx4_by_pair"}
+    pieces(calls, "lcu_mx4_tiles", m, k // 2, 2 * 32)
+    laid = [a for name, a in calls if name == "lcu_mx4_by_pair"]
+    together = k // 256 * 8 * m + 4096 < 1 << 32
+    assert sum(a["rows"] for a in laid) == m and (len(laid) == 1) == together
+    of = 0
+    for name, a in calls:
+        if name == "lcu_mx4_by_pair":
+            assert together or a["scales"] == of * k // 32
+            rows_of = a["rows"]
+        else:
+            assert a["xs"] == (8 * of if together else 0) and a["lds"] == 8 * (m if together else a["m"]) and (together or rows_of == a["m"])
+            of += a["m"]
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "four"])
+def test_any_number_of_rows_of_a_large_weight(kind, calls):
+    """A weight of more than 4 GiB is streamed, whatever the rows, so many of them at a time as a launch takes."""
+    n, k, m = 300_000, 28672, 2_500_001
+    ops.gemm_mx4(rows(kind, m, k), weight(n, k))
+    assert {name for name, _ in calls} == {"lcu_mx4_stream"}
+    pieces(calls, "lcu_mx4_stream", m, k // 2 if kind == "four" else 2 * k, 2 * n)
+    at = 0
+    for _, a in calls:
+        assert a["xs"] == (at * k // 32 if kind == "four" else None)
+        at += a["m"]
