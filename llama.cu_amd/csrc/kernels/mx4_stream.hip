@@ -13,6 +13,7 @@
 #include "mx4/matrix.h"
 #include "gate_act.h"
 #include "quad_rows.h"
+#include "../shared/per_device.h"
 
 enum { MX4_EPI_BF16 = 0, MX4_EPI_F32 = 1, MX4_EPI_SWIGLU = 2, MX4_EPI_SWIGLU_F32 = 3 };
 
@@ -240,15 +241,18 @@ mx4_stream4_kernel(const uint8_t *__restrict__ X, int ldx, const uint8_t *__rest
     mx4_finish<NT, MT, EPI>(a, row0, acc, red, [](int c) { return c; });
 }
 
-// How many workgroups of eight waves the card holds at once.
-static long long mx4_held(const void *kernel) {
-    int each = 0, device = 0, units = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, MX4_WAVES * WAVE, 0) != hipSuccess || hipGetDevice(&device) != hipSuccess ||
-        hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) {
-        (void)hipGetLastError();
-        return 1ll << 40;
-    }
-    return (long long)each * units;
+// How many workgroups of eight waves the current device holds at once (more than any launch has, where it does not say).
+static long long mx4_held(const void *kernel, LcuPerDevice &known) {
+    constexpr long long UNKNOWN = 1ll << 40;
+    int device = -1;
+    if (hipGetDevice(&device) != hipSuccess) device = -1;
+    const long long held = known.get(device, [kernel](int of) {
+        int each = 0, units = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, kernel, MX4_WAVES * WAVE, 0) != hipSuccess || hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, of) != hipSuccess) return 0ll;
+        return (long long)each * units;
+    }, UNKNOWN);
+    if (held == UNKNOWN) (void)hipGetLastError();
+    return held;
 }
 
 // codes, scales: W in the products' order, [ceil(N / 16)][pairs] blocks, 16-byte aligned.  x_kind: 1 bfloat16 rows [M, ldx]; 3 float32 rows as
@@ -277,9 +281,9 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
     auto block = [&](dim3 g, long long held) { return dim3(min((long long)g.x * g.y > held ? MX4_WAVES / 2 : MX4_WAVES, work) * WAVE); };
 #define RUN(NT, MT, KERNEL, ...)                                                      \
     do {                                                                              \
-        static const long long held = mx4_held((const void *)KERNEL);                 \
+        static LcuPerDevice held;                                                     \
         const dim3 g = grid(NT, MT);                                                  \
-        KERNEL<<<g, block(g, held), 0, stream>>>(__VA_ARGS__);                        \
+        KERNEL<<<g, block(g, mx4_held((const void *)KERNEL, held)), 0, stream>>>(__VA_ARGS__); \
     } while (0)
 #define GO(NT, MT, PLANES, EPI, LOADS) RUN(NT, MT, (mx4_stream_kernel<NT, MT, PLANES, EPI, LOADS>), (const bf16_t *)x, (int)ldx, (int)(PLANES == 3 ? ldx / 3 : 0), a)
 #define GO4(NT, MT, EPI) RUN(NT, MT, (mx4_stream4_kernel<NT, MT, EPI>), (const uint8_t *)x, (int)ldx, (const uint8_t *)xs, (int)lds, a)
