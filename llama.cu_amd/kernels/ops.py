@@ -84,11 +84,15 @@ def here(what: str, first: torch.Tensor, *more: Optional[torch.Tensor]) -> None:
 
 def apart(what: str, out: torch.Tensor, *read: Optional[torch.Tensor]) -> None:
     """Refuses a result over what is still read for it (rows, or vectors: from the first byte of each to its last)."""
-    lo = out.data_ptr()
-    hi = lo + ((out.shape[0] - 1) * out.stride(0) + out.shape[-1]) * out.element_size()
+    def bytes_of(t):
+        rows = (t.shape[0] - 1) * t.stride(0) + (t.shape[1] if t.dim() > 1 else 1)
+        return t.data_ptr(), t.data_ptr() + rows * t.element_size()
+    lo, hi = bytes_of(out)
     for t in read:
-        if t is not None and t.data_ptr() < hi and lo < t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t.shape[-1]) * t.element_size() and t.numel():
-            raise KernelError(f"{what}: out lies over an operand")
+        if t is not None and t.numel():
+            first, end = bytes_of(t)
+            if first < hi and lo < end:
+                raise KernelError(f"{what}: out lies over an operand")
 
 
 _LETTERS = {"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int}
