@@ -2752,6 +2752,7 @@ def decay_state_floats(heads: int, key_dim: int, value_dim: int, gated: bool) ->
 
 MX4_BLOCK = 32            # numbers along k that share a scale
 _MX4_PAIR = 256           # k that the products' order is filled up to
+_MX4_UNITS = 1 << 31      # units of 8 numbers, fewer than which a launch of the conversions takes: more rows go in pieces
 
 
 class Mx4:
@@ -2828,11 +2829,14 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     pairs, blocks, device, stream = -(-k // _MX4_PAIR), -(-k // MX4_BLOCK), x.device, raw_stream()
     codes = torch.empty_strided((m, 128 * pairs), (128 * pairs, 1), dtype=torch.uint8, device=device)
     scales = torch.empty_strided((m, 8 * pairs), (8 * pairs, 1), dtype=torch.uint8, device=device)
+    step = (_MX4_UNITS - 1) // (32 * pairs) if pairs else m
     # (rows for the product that streams the weight need no second copy; a weight's is not used, 1 / 136 of what is written)
-    by_pair = torch.empty_strided((pairs, m, 8), (8 * m, 8, 1), dtype=torch.uint8, device=device) if m > 16 and not scales.is_inference() else None
+    by_pair = torch.empty_strided((pairs, m, 8), (8 * m, 8, 1), dtype=torch.uint8, device=device) if 16 < m <= step and not scales.is_inference() else None
     if m and k:
-        _check(bind("mx4", "lcu_mx4_quantize", "plilippp")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], m, k, codes.data_ptr(), scales.data_ptr(),
-                                                           None if by_pair is None else by_pair.data_ptr(), stream), "mx4_quantize")
+        f = bind("mx4", "lcu_mx4_quantize", "plilippp")
+        for r in range(0, m, step):
+            _check(f(x.data_ptr() + r * x.stride(0) * x.element_size(), x.stride(0), _TYPE[x.dtype], min(step, m - r), k, codes.data_ptr() + r * 128 * pairs, scales.data_ptr() + r * 8 * pairs,
+                     None if by_pair is None else by_pair.data_ptr(), stream), "mx4_quantize")
     if blocks % 8:
         codes, scales = codes.as_strided((m, 16 * blocks), (128 * pairs, 1)), scales.as_strided((m, blocks), (8 * pairs, 1))
     q = Mx4(codes, scales, k)
@@ -2851,8 +2855,10 @@ def mx4_values(q: Mx4, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     here("mx4_values", codes, scales)
     out = torch.empty_strided((m, k), (k, 1), dtype=out_dtype, device=codes.device)
     if m and k:
-        _check(bind("mx4", "lcu_mx4_values", "plpllipli")(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), m, k, out.data_ptr(), k,
-                                                          _TYPE[out_dtype], raw_stream()), "mx4_values")
+        f, step = bind("mx4", "lcu_mx4_values", "plpllipli"), (_MX4_UNITS - 1) // -(-k // 8)
+        for r in range(0, m, step):
+            _check(f(codes.data_ptr() + r * codes.stride(0), codes.stride(0), scales.data_ptr() + r * scales.stride(0), scales.stride(0), min(step, m - r), k,
+                     out.data_ptr() + r * k * out.element_size(), k, _TYPE[out_dtype], raw_stream()), "mx4_values")
     return out
 
 
@@ -2909,8 +2915,11 @@ def _mx4_rows(x: torch.Tensor, k: int) -> Tuple[torch.Tensor, int]:
         return x, 1
     x = _mx4_source(x, "gemm_mx4")
     planes = 3 if x.dtype == torch.float32 else 1
-    out = torch.empty((x.shape[0], planes * (-(-k // _MX4_PAIR) * _MX4_PAIR)), dtype=torch.bfloat16, device=x.device)
-    _check(bind("mx4", "lcu_mx4_rows", "plilip")(x.data_ptr(), x.stride(0), _TYPE[x.dtype], x.shape[0], k, out.data_ptr(), raw_stream()), "gemm_mx4 rows")
+    units = -(-k // _MX4_PAIR) * 32
+    out = torch.empty((x.shape[0], planes * 8 * units), dtype=torch.bfloat16, device=x.device)
+    f, step = bind("mx4", "lcu_mx4_rows", "plilip"), (_MX4_UNITS - 1) // units
+    for r in range(0, x.shape[0], step):
+        _check(f(x.data_ptr() + r * x.stride(0) * x.element_size(), x.stride(0), _TYPE[x.dtype], min(step, x.shape[0] - r), k, out.data_ptr() + r * planes * 16 * units, raw_stream()), "gemm_mx4 rows")
     return out, planes
 
 

@@ -185,3 +185,23 @@ def test_rows_in_pieces_past_a_streamed_weight(kind, force, monkeypatch):
     got = ops.gemm_mx4(rows, w, out=room[1:1 + m, 3:3 + n])
     assert_close(got, mine @ exact.T, REL[torch.float32], kind)
     assert asked == [] and (room[0] == 7).all() and (room[m + 1:] == 7).all() and (room[:, :3] == 7).all() and (room[:, 3 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(41, 300), (7, 1024), (200, 40)])
+def test_conversions_in_pieces(m, k, dtype, monkeypatch):
+    """Rows beyond what one launch takes, with a small limit in the place of 2^31 units: the same bits in pieces as at once."""
+    from llama_cu_amd.kernels import ops
+    wide = rnd(m, k + 8, seed=m).to(dtype).cuda()
+    x = wide[:, 3:3 + k]
+    want = ops.mx4_quantize(x)
+    values_of, w = ops.mx4_values(want, dtype), weight(40, k)[0]
+    laid_out = ops._mx4_rows(x, k)
+    product, of_four = ops.gemm_mx4(x, w), ops.gemm_mx4(want, w)
+    monkeypatch.setattr(ops, "_MX4_UNITS", 3 * 32 * -(-k // 256) + 5)
+    got = ops.mx4_quantize(x)
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales) and got._by_pair is None
+    assert torch.equal(ops.mx4_values(want, dtype), values_of)
+    again = ops._mx4_rows(x, k)
+    assert again[1] == laid_out[1] and torch.equal(again[0], laid_out[0])
+    assert torch.equal(ops.gemm_mx4(x, w), product) and torch.equal(ops.gemm_mx4(got, w), of_four)

@@ -9,7 +9,9 @@ from llama_cu_amd.kernels import ops
 ENTRY = {"lcu_mx4_tiles": "x ldx kind xs lds codes scales pairs y ldy m n k epilogue shape slices planes stream",
          "lcu_mx4_stream": "x ldx kind xs lds codes scales pairs y ldy m n k epilogue stream",
          "lcu_mx4_by_pair": "scales lds rows pairs out stream",
-         "lcu_mx4_rows": "x ldx type rows k out stream"}
+         "lcu_mx4_rows": "x ldx type rows k out stream",
+         "lcu_mx4_quantize": "x ldx type rows k codes scales by_pair stream",
+         "lcu_mx4_values": "codes ldc scales lds rows k y ldy type stream"}
 
 
 @pytest.fixture
@@ -109,3 +111,40 @@ def test_any_number_of_rows_of_a_large_weight(kind, calls):
     for _, a in calls:
         assert a["xs"] == (at * k // 32 if kind == "four" else None)
         at += a["m"]
+
+
+def covered(calls, name, m, most, **bytes_of):
+    """The rows of the calls of ``name``: all of them, one after the other, at most ``most`` at a time, each at the bytes a row that are said for its arguments."""
+    at = 0
+    for entry, a in calls:
+        if entry == name:
+            assert 0 < a["rows"] <= most and {what: a[what] for what in bytes_of} == {what: at * size for what, size in bytes_of.items()}
+            at += a["rows"]
+    assert at == m
+
+
+@pytest.mark.parametrize("m,k", [(1, 1), (16, 4096), (4_194_303, 4096), (4_194_304, 4096), (10_000_001, 4096), (70_000_000, 1000), (3, 2_000_000_000), (20, 2_000_000_000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_conversions_of_any_number_of_rows(m, k, dtype, calls):
+    """A launch counts its units of 8 numbers in 31 bits: more of them go in pieces of the rows."""
+    size = torch.empty(0, dtype=dtype).element_size()
+    x = torch.empty(m, k, dtype=dtype, device="meta")
+    whole = -(-k // 256) * 256
+    q = ops.mx4_quantize(x)
+    assert q.shape == (m, k) and q.codes.shape == (m, -(-k // 32) * 16)
+    covered(calls, "lcu_mx4_quantize", m, ((1 << 31) - 1) * 8 // whole, x=k * size, codes=whole // 2, scales=whole // 32)
+    calls.clear()
+    ops.mx4_values(q, dtype)
+    covered(calls, "lcu_mx4_values", m, ((1 << 31) - 1) // -(-k // 8), codes=whole // 2, scales=whole // 32, y=k * size)
+    calls.clear()
+    if k < 1 << 20 and (dtype == torch.float32 or k % 128):
+        planes = 3 if dtype == torch.float32 else 1
+        out, kind = ops._mx4_rows(x, k)
+        assert out.shape == (m, planes * whole) and kind == planes
+        covered(calls, "lcu_mx4_rows", m, ((1 << 31) - 1) * 8 // whole, x=k * size, out=planes * whole * 2)
+
+
+def test_the_second_copy_of_scales_is_of_all_rows(calls):
+    """The scales as the products in tiles read them are written by one launch or not at all."""
+    assert ops.mx4_quantize(torch.empty(4_194_303, 4096, dtype=torch.bfloat16, device="meta"))._by_pair is not None
+    assert ops.mx4_quantize(torch.empty(4_194_304, 4096, dtype=torch.bfloat16, device="meta"))._by_pair is None
