@@ -2785,6 +2785,11 @@ class Mx4:
         self.__init__(*state)
 
 
+def _mx4_length(k: int, what: str) -> None:
+    if k >= 1 << 30:                      # (the kernels' own counts along k are 32 bits, and go past its end)
+        raise KernelError(f"{what}: rows of {k} numbers are not supported (less than 2^30)")
+
+
 def _mx4_checked(q: Mx4, what: str) -> Tuple[int, int]:
     """``(rows, blocks)`` of a well-formed Mx4."""
     if not isinstance(q, Mx4):
@@ -2793,6 +2798,7 @@ def _mx4_checked(q: Mx4, what: str) -> Tuple[int, int]:
     blocks = -(-k // MX4_BLOCK)
     if q._filled:                         # (made so)
         return codes.shape[0], blocks
+    _mx4_length(k, what)
     if k < 0 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 \
             or codes.shape[1] != 16 * blocks or scales.shape != (codes.shape[0], blocks):
         raise KernelError(f"{what}: codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not those of rows of {k} numbers")
@@ -2826,6 +2832,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     number goes to the nearest code, ties to the even one, and beyond 6 scales to 6.  A block that holds an infinity or a NaN becomes NaN."""
     x = _mx4_source(x, "mx4_quantize")
     m, k = x.shape
+    _mx4_length(k, "mx4_quantize")
     pairs, blocks, device, stream = -(-k // _MX4_PAIR), -(-k // MX4_BLOCK), x.device, raw_stream()
     codes = torch.empty_strided((m, 128 * pairs), (128 * pairs, 1), dtype=torch.uint8, device=device)
     scales = torch.empty_strided((m, 8 * pairs), (8 * pairs, 1), dtype=torch.uint8, device=device)
@@ -2871,6 +2878,9 @@ class PackedMx4:
         self.codes, self.scales, self.n, self.k = codes, scales, n, k
         self.pairs = -(-k // _MX4_PAIR)
         size = -(-n // 16) * self.pairs * 2048
+        _mx4_length(k, "PackedMx4")
+        if n >= 1 << 30:
+            raise KernelError(f"PackedMx4: a weight of {n} features is not supported (less than 2^30)")
         if n < 1 or k < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.shape != (size,) or scales.shape != (size // 16,) \
                 or not codes.is_contiguous() or not scales.is_contiguous():
             raise KernelError(f"PackedMx4: a weight of {n} x {k} has {size} bytes of codes and {size // 16} scales, got {codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")

@@ -123,7 +123,7 @@ def covered(calls, name, m, most, **bytes_of):
     assert at == m
 
 
-@pytest.mark.parametrize("m,k", [(1, 1), (16, 4096), (4_194_303, 4096), (4_194_304, 4096), (10_000_001, 4096), (70_000_000, 1000), (3, 2_000_000_000), (20, 2_000_000_000)])
+@pytest.mark.parametrize("m,k", [(1, 1), (16, 4096), (4_194_303, 4096), (4_194_304, 4096), (10_000_001, 4096), (70_000_000, 1000), (3, 1_000_000_000), (20, 1_000_000_000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_conversions_of_any_number_of_rows(m, k, dtype, calls):
     """A launch counts its units of 8 numbers in 31 bits: more of them go in pieces of the rows."""
@@ -148,3 +148,22 @@ def test_the_second_copy_of_scales_is_of_all_rows(calls):
     """The scales as the products in tiles read them are written by one launch or not at all."""
     assert ops.mx4_quantize(torch.empty(4_194_303, 4096, dtype=torch.bfloat16, device="meta"))._by_pair is not None
     assert ops.mx4_quantize(torch.empty(4_194_304, 4096, dtype=torch.bfloat16, device="meta"))._by_pair is None
+
+
+def test_lengths_that_no_kernel_counts(calls):
+    """Counts along k, and of features, go to the libraries as 32-bit numbers: longer ones would arrive as others."""
+    def refused(f, *args):
+        with pytest.raises(ops.KernelError, match="less than 2\\^30"):
+            f(*args)
+    empty = lambda *shape: torch.empty(*shape, dtype=torch.uint8, device="meta")
+    longest = (1 << 30) - 1
+    for k in (1 << 30, (1 << 31) + 5, (1 << 32) + 256):
+        q = ops.Mx4(empty(1, -(-k // 32) * 16), empty(1, -(-k // 32)), k)
+        refused(ops.mx4_quantize, torch.empty(1, k, dtype=torch.bfloat16, device="meta"))
+        refused(ops.mx4_values, q)
+        refused(ops.pack_mx4, q)
+        refused(weight, 16, k)
+        refused(weight, k, 16)
+    ops.mx4_values(ops.mx4_quantize(torch.empty(1, longest, dtype=torch.bfloat16, device="meta")))
+    assert all(a["k"] == longest for _, a in calls) and len(calls) == 2
+    assert weight(16, longest).k == longest and weight(longest, 16).n == longest
