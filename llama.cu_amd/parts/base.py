@@ -210,6 +210,10 @@ class BuildContext:
                                      # in the experts' kernels' order; of a bfloat16 shared expert a third, in theirs)
     weights: str = "file"            # "mx4": matrices that can be are held in microscaled 4-bit numbers (attention's and the dense feed-forward's)
 
+    def __post_init__(self):
+        if self.weights not in ("file", "mx4"):
+            raise ValueError(f"weights {self.weights!r} are neither file nor mx4")
+
 
 @dataclass
 class ScaledRows:

@@ -167,3 +167,14 @@ def test_lengths_that_no_kernel_counts(calls):
     ops.mx4_values(ops.mx4_quantize(torch.empty(1, longest, dtype=torch.bfloat16, device="meta")))
     assert all(a["k"] == longest for _, a in calls) and len(calls) == 2
     assert weight(16, longest).k == longest and weight(longest, 16).n == longest
+
+
+@pytest.mark.parametrize("weights", ["MX4", "4bit", "", None])
+def test_how_matrices_are_held(weights):
+    """A word that is none of the ways is refused wherever it comes in, not taken for the file's."""
+    from llama_cu_amd.engine.config import EngineConfig
+    from llama_cu_amd.parts.base import BuildContext
+    for make in (lambda w: BuildContext(torch.bfloat16, torch.device("cpu"), 64, 16, weights=w), lambda w: EngineConfig(weights=w)):
+        assert make("file").weights == "file" and make("mx4").weights == "mx4"
+        with pytest.raises(ValueError, match="neither file nor mx4"):
+            make(weights)
