@@ -7,8 +7,10 @@
 // takes both sides' codes and scales as they are.
 //
 // Bound by memory where the weight is large, by the latency of a wave's chain of loads where it is not (a wave has K / 8, of which two pairs of macro-steps are on their way; K is
-// split over the waves of one workgroup and no further, so that no second launch adds the parts).  One row: 6144 x 4096 5.2 us (2.6 TB/s), 128256 x 4096 48 (5.8 TB/s); 8 rows: 28672 x
-// 4096 with the activation 13.6 to 14.9 us (4.2 to 4.6 TB/s), 57344 x 8192 51 (4.9).  Beyond 8 rows every workgroup's reading of all rows out of the L2 caches weighs more and the products in tiles take over.
+// split over the waves of one workgroup and no further, so that no second launch adds the parts).  One row: 6144 x 4096 4.8 us (2.8 TB/s), 128256 x 4096 45 to 48 (5.8 to 6.2 TB/s); 8 rows:
+// 28672 x 4096 with the activation 14.6 to 16 us (3.9 to 4.3 TB/s), 57344 x 8192 46 to 49 (5.1 to 5.4).  Rows in float32 and in 4 bits, weights out of memory, the gap between launches and the rows' planes
+// included: 6144 x 4096 one row 9.7 and 6.2 us, 28672 x 4096 four rows in float32 24, eight in 4 bits 18, 4104 x 11008 four rows in float32 18, 4096 x 14336 twelve in 4 bits 14.  Beyond 8 rows every workgroup's reading of
+// all rows out of the L2 caches weighs more and the products in tiles take over.
 #include "mx4.h"
 #include "mx4/matrix.h"
 #include "gate_act.h"
@@ -270,8 +272,8 @@ LCU_API int lcu_mx4_stream(const void *x, long long ldx, int x_kind, const void 
         return LCU_BAD_ARGUMENT;
     const Mx4Args a = {(const uint8_t *)codes, (const uint8_t *)scales, pairs, macros, y, ldy, M, N, ((uintptr_t)y | (uintptr_t)(ldy * elem)) % (4 * elem) == 0};
     const int tiles = (cols + 15) / 16, work = x_kind == 4 ? macros : (macros + 1) / 2;
-    // two tiles of features a workgroup where there are many, and more than four rows are read for them (us, one tile / two: 16384 x 2048 16 rows 10.8 / 9.5, 28672 x 4096 16 rows 26.1 / 24.9,
-    // 128256 x 4096 8 rows 70.6 / 65.1; one row 58.9 / 59.7; 4096 x 14336 8 rows 13.1 / 15.6)
+    // two tiles of features a workgroup where there are many, and more than four rows are read for them (us, one tile / two, weights out of memory: 16384 x 2048 16 rows 9.5 / 8.1, 28672 x 4096
+    // 16 rows 24.8 / 20.6, 128256 x 4096 8 rows 61.8 / 51.6; one row 45.3 / 47.9; 4096 x 14336 8 rows 12.4 / 14.7)
     const bool pairs_of = x_kind == 1 && M > 4 && M <= 16 && N > 8192 && epi < MX4_EPI_SWIGLU;
     auto grid = [&](int nt, int mt) { return dim3(epi >= MX4_EPI_SWIGLU ? tiles : (tiles + nt - 1) / nt, (M + 16 * mt - 1) / (16 * mt)); };
     if ((M + 15) / 16 > 65535) return LCU_BAD_ARGUMENT;

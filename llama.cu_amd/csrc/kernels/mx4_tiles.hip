@@ -12,11 +12,15 @@
 //   rows in 4 bits     a step is 256 k, a slice 64 (32 x 32 x 64, scaled); the scales, four bytes a lane and step, come into registers.  Steps of 128 k, which the rings hold more of,
 //                      took a tenth longer: half a line a row and load.
 //
+// The rings are waited for by counting their own loads (MtShape::LEFT).  The scales come into registers a step ahead, and waits are for everything asked for before: the compiler's wait for a
+// step's scales is one for all loads of the steps before the last.  So a load has a step's time, also in rings of four stages, whose count alone would leave it two.
+//
 // Which tile: the largest that fills the card, and where none does slices of K beside each other, whose sums a second launch adds (the rule and its figures stand where the kernel is
 // chosen).  Rows in 4 bits have waves of 128 x 128 and one a SIMD, which read half of what waves of 64 x 128 do out of LDS a product (8192 x 28672 with 4,096 rows 480 us, so 430).
-// Bound by the matrix cores and, with many rows, the power that they draw: 28672 x 4096 with the activation, 2,048 rows in bfloat16 360 to 390 us (1.23 to 1.34 PFLOP/s; the library's
-// bfloat16 product alone 354 to 399); 8192 x 28672, 4,096 rows in 4 bits 420 to 430 us (4.5 PFLOP/s).  With few rows by latency: 28672 x 4096, 24 rows 22 us; 4096 x 14336, 64 rows in 4
-// bits 11.2 us and 3.8 for the slices' sums; 4104 x 11008, 37 rows in float32 20.5 us and 3.9.
+// Many rows are bound by the matrix cores at the clock that the power limit leaves, and by what waves wait for each other: 28672 x 4096 with the activation, 2,048 rows in bfloat16 371 to 390 us
+// (1.23 to 1.30 PFLOP/s; the library's bfloat16 product alone 354 to 399): matrix cores busy 64 % of the time at 1.6 to 1.8 GHz, a quarter of the waves' time waiting for loads; 8192 x 28672, 4,096
+// rows in 4 bits 412 to 430 us (4.5 to 4.7 PFLOP/s), 65 % at 1.6 to 1.7 GHz, a fifth.  Few rows by the loads' latency: 4096 x 14336, 64 rows in 4 bits 9.5 to 10.9 us and 3.9 for the slices' sums
+// (matrix cores 5 % busy, 57 % of the waves' time waiting for loads); 28672 x 4096, 24 rows, with the activation 18.4 us; 4104 x 11008, 37 rows in float32 20.4 us and 4 (30 %, 25 %).
 #include <type_traits>
 #include "mx4.h"
 #include "mx4/matrix.h"

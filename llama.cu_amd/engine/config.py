@@ -24,7 +24,7 @@ class EngineConfig:
     max_model_len: Optional[int] = None     # most tokens a request may hold (default, and at most: the model's positions)
     use_graphs: bool = True                 # replay decode steps from captured graphs
     pack_weights: Optional[bool] = None     # a second copy of the matrices in the decode kernels' order (default: if memory allows)
-    weights: str = "file"                   # "mx4": attention's and the dense feed-forward's matrices are multiplied in microscaled 4-bit numbers, a quarter of bfloat16's bytes a step (the file's stay beside them)
+    weights: str = "file"                   # "mx4": attention's and the dense feed-forward's matrices are multiplied in microscaled 4-bit numbers, a quarter of bfloat16's bytes a step (the file's stay beside them, so it saves no memory)
     run_ahead: bool = True                  # launch a round before the round before has been read
     logprobs: bool = False                  # every sampled token comes with the log of the probability the model gave it
     poison_freed: bool = False              # debugging: fill pages that change hands with NaN

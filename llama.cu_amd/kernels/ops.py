@@ -2949,9 +2949,10 @@ def _mx4_whole(q: Mx4, blocks: int) -> Mx4:
     return Mx4(codes, scales, 32 * whole)
 
 
-# What the kernels of the 4-bit products take, us, fitted to 193,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory): the choice by
-# these numbers takes 1.02 times what the best choice takes, geometric mean; of 10 to 64 rows, where the streaming kernel and the tiles meet, 1.01 (10,183 shapes drawn at random).  Up to 8 rows
-# of bfloat16, 4 of float32 and 12 in 4 bits the streaming kernel is taken unasked: 1.01 to 1.03 times the best; at 16 it would be 1.03, 1.37 and 1.03.
+# What the kernels of the 4-bit products take, us, fitted to 193,000 timed products (4 to 3,200 rows, 64 to 128,256 features, K 128 to 28,672, weights out of memory).  The tiles have become up to
+# a tenth faster since (the order of their loads); the choice by these numbers takes 1.02 times what the best of all shapes and slices does, geometric mean of 792 shapes drawn at random (64 to
+# 40,000 features, K 128 to 20,480), at most 1.38; of 9 to 64 rows, where the streaming kernel and the tiles meet, 1.02 too (303 shapes), of 9 to 16 rows of bfloat16 1.05.  Up to 8 rows of bfloat16, 4 of float32 and 12
+# in 4 bits the streaming kernel is taken unasked: 1.00 to 1.01 times the best.
 # Tiles (features, tokens) by the kind of the rows and the shape's number: workgroups a compute unit holds, us a launch, us a workgroup, us a step with one, two, three, four workgroups
 # on a compute unit; us a launch that joins slices of K, us for each 2^20 bytes that it moves.
 _MX4_TILES = {
